@@ -84,6 +84,10 @@ extern "C" {
                                        instead of reading rows nobody wrote. */
 #define SRWM_FLAG_NORM_EPS 2048u   /* delta_layer_prologue_f32 only: 1e-5 is added to the normalisers of q and k (the RL
                                      tree's layers, reinforcement_learning/torchbeast/layer.py:30-33) */
+/* selective_scan_*, causal_conv_*, residual_rms_norm_*: */
+#define SRWM_FLAG_SOFTPLUS 16384u      /* selective_scan_*: dt = softplus(delta + delta_bias); without it their sum itself */
+#define SRWM_FLAG_SILU 32768u          /* causal_conv_*: silu behind the convolution */
+#define SRWM_FLAG_RESIDUAL_F32 65536u  /* residual_rms_norm_*_bf16: the residual and the sum are fp32 (else bf16) */
 /* srwm_layer_forward_* / srwm_layer_backward_* only: */
 #define SRWM_FLAG_STATE_SHIFT 64u    /* W_y..w_b hold the state MINUS the head's shared weights, on entry and on
                                         exit (how the RL layers carry it, torchbeast/layer.py:389-418) */
@@ -517,6 +521,149 @@ SRWM_API int delta_layer_prologue_grad_bf16(const uint16_t *gq, const int64_t gq
                                    const uint16_t *q, const uint16_t *k, const uint16_t *beta, const float *sums,
                                    uint16_t *grad_rows,
                                    int N, int H, int L, int E, int M, unsigned flags, void *stream);
+
+/*
+ * Selective state-space scan: the recurrence with a decay that depends on the step.  No counterpart in the reference.
+ * Heads as in the delta rule; a channel (h, e) has S states, the heads h of a group g = h / (H / G) share B and C:
+ *     dt_t = softplus(delta_t + delta_bias)           (the sum itself without SRWM_FLAG_SOFTPLUS)
+ *     h_t  = exp(dt_t A) h_{t-1} + dt_t u_t B_t       (h_{t-1} counts as zero where keep[n][t] == 0)
+ *     out_t = (C_t . h_t + D u_t) silu(z_t)           (no gate without z)
+ *   u, delta, z, out   strided [N,H,L,E];  B, C strided [N,G,L,S];  fp32 or bf16, all alike; z may be NULL
+ *   A                  dense [H,E,S];  D, delta_bias dense [H,E] or NULL
+ *   state              dense [N,H,E,S], before the first step, or NULL (zeros);  last: the same, after the last step
+ *   keep               dense [N,L] or NULL.  Sequences packed one behind the other in a row: 0 at the first step of each
+ *   lengths            [N] or NULL: steps of each row (values outside 0..L are taken as the nearer bound).  Steps behind
+ *                      are not read, their rows of out are written as zeros, and last is the state after the row's end
+ *   saved              dense [N, ceil(L/16), H*E, S]: states for the backward, or NULL
+ * S up to 64 (SRWM_ESIZE beyond).  A, state, last, saved, workspace and their gradients start at multiples of 16 bytes.
+ * Arithmetic, states and the sums are fp32.
+ */
+SRWM_API int selective_scan_forward_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                             const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                             const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
+                             const float *A, const float *D, const float *delta_bias, const float *state,
+                             const float *keep, const int *lengths, float *out, const int64_t out_strides[3],
+                             float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags,
+                             void *stream);
+SRWM_API int selective_scan_forward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                             const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                             const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                             const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                             const float *state, const float *keep, const int *lengths, uint16_t *out,
+                             const int64_t out_strides[3], float *last, float *saved, int N, int H, int L, int E,
+                             int S, int G, unsigned flags, void *stream);
+
+/*
+ * Backward of the scan.  saved as the forward left it; grad_out strided [N,H,L,E]; grad_last dense [N,H,E,S] or NULL.
+ * grad_u, grad_delta, grad_z strided [N,H,L,E] and grad_B, grad_C strided [N,G,L,S] in the type of the inputs (rows
+ * behind a row's length are written as zeros); grad_A [H,E,S], grad_D and grad_bias [H,E], grad_state [N,H,E,S] fp32, the
+ * last three may be NULL.  workspace: selective_scan_workspace() floats, contents ignored.  Sums over channels and over
+ * the batch are formed in a fixed order (the same call gives the same bits).
+ */
+SRWM_API int selective_scan_backward_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                             const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                             const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
+                             const float *A, const float *D, const float *delta_bias, const float *keep,
+                             const int *lengths, const float *saved, const float *grad_out,
+                             const int64_t grad_out_strides[3], const float *grad_last, float *grad_u,
+                             const int64_t grad_u_strides[3], float *grad_delta, const int64_t grad_delta_strides[3],
+                             float *grad_z, const int64_t grad_z_strides[3], float *grad_B,
+                             const int64_t grad_b_strides[3], float *grad_C, const int64_t grad_c_strides[3],
+                             float *grad_A, float *grad_D, float *grad_bias, float *grad_state, float *workspace,
+                             int N, int H, int L, int E, int S, int G, unsigned flags, void *stream);
+SRWM_API int selective_scan_backward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                             const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                             const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                             const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                             const float *keep, const int *lengths, const float *saved, const uint16_t *grad_out,
+                             const int64_t grad_out_strides[3], const float *grad_last, uint16_t *grad_u,
+                             const int64_t grad_u_strides[3], uint16_t *grad_delta,
+                             const int64_t grad_delta_strides[3], uint16_t *grad_z, const int64_t grad_z_strides[3],
+                             uint16_t *grad_B, const int64_t grad_b_strides[3], uint16_t *grad_C,
+                             const int64_t grad_c_strides[3], float *grad_A, float *grad_D, float *grad_bias,
+                             float *grad_state, float *workspace, int N, int H, int L, int E, int S, int G,
+                             unsigned flags, void *stream);
+SRWM_API int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G);
+
+/* One token: u, delta, z, out strided as above with L = 1 (the third stride is not used); keep [N] or NULL; state dense
+ * [N,H,E,S], overwritten in place. */
+SRWM_API int selective_scan_step_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                             const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                             const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
+                             const float *A, const float *D, const float *delta_bias, const float *keep, float *state,
+                             float *out, const int64_t out_strides[3], int N, int H, int E, int S, int G,
+                             unsigned flags, void *stream);
+SRWM_API int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                             const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                             const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                             const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                             const float *keep, float *state, uint16_t *out, const int64_t out_strides[3], int N,
+                             int H, int E, int S, int G, unsigned flags, void *stream);
+
+/*
+ * Short causal depthwise convolution: out_t = f(bias + sum_j weight[j] x_{t-W+1+j}), f = silu with SRWM_FLAG_SILU.
+ *   x, out     strided [N,H,L,E], fp32 or bf16;  weight dense [H,E,W], W in 2..4 (else SRWM_ESIZE);  bias [H,E] or NULL
+ *   state      dense [N,H,W-1,E] in the type of x: the inputs before the first step, the newest last; NULL: zeros
+ *   last       the same behind the last step
+ *   keep, lengths as above; inputs before a reset count as zero, in out and in last
+ * Backward: grad_x strided [N,H,L,E], grad_last / grad_state like state (either may be NULL), grad_weight [H,E,W] and
+ * grad_bias [H,E] (or NULL) fp32; workspace: causal_conv_workspace() floats.  Step: state overwritten in place.
+ */
+SRWM_API int causal_conv_forward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const float *state, const float *keep, const int *lengths, float *out,
+                             const int64_t out_strides[3], float *last, int N, int H, int L, int E, int W,
+                             unsigned flags, void *stream);
+SRWM_API int causal_conv_forward_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const uint16_t *state, const float *keep, const int *lengths, uint16_t *out,
+                             const int64_t out_strides[3], uint16_t *last, int N, int H, int L, int E, int W,
+                             unsigned flags, void *stream);
+SRWM_API int causal_conv_backward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const float *state, const float *keep, const int *lengths, const float *grad_out,
+                             const int64_t grad_out_strides[3], const float *grad_last, float *grad_x,
+                             const int64_t grad_x_strides[3], float *grad_weight, float *grad_bias, float *grad_state,
+                             float *workspace, int N, int H, int L, int E, int W, unsigned flags, void *stream);
+SRWM_API int causal_conv_backward_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const uint16_t *state, const float *keep, const int *lengths, const uint16_t *grad_out,
+                             const int64_t grad_out_strides[3], const uint16_t *grad_last, uint16_t *grad_x,
+                             const int64_t grad_x_strides[3], float *grad_weight, float *grad_bias,
+                             uint16_t *grad_state, float *workspace, int N, int H, int L, int E, int W,
+                             unsigned flags, void *stream);
+SRWM_API int causal_conv_step_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const float *keep, float *state, float *out, const int64_t out_strides[3], int N, int H,
+                             int E, int W, unsigned flags, void *stream);
+SRWM_API int causal_conv_step_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const float *keep, uint16_t *state, uint16_t *out, const int64_t out_strides[3], int N,
+                             int H, int E, int W, unsigned flags, void *stream);
+SRWM_API int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E, int W);
+
+/*
+ * Root-mean-square norm with the residual's addition, over dense rows of D elements:
+ *     s = x + residual;   out = s / sqrt(mean(s^2) + eps) * weight
+ *   x, out     [rows, D] fp32 or bf16;  residual, sum [rows, D] fp32, or bf16 with x (see SRWM_FLAG_RESIDUAL_F32); both
+ *              NULL: s = x.  The norm is taken of s before it is rounded to the type of sum.  weight [D] fp32
+ *   rstd       [rows] fp32 for the backward, or NULL;  eps: one float in HOST memory
+ * residual_rms_norm_e4m3_*: out holds e4m3 (OCP) bytes of the result divided by scale[row] = max|result| / 448 of the row
+ * (1 for a row of zeros), rounded to nearest even.
+ * Backward: `sum` is what was normalised, as stored (x without a residual); grad_x like x, grad_residual and grad_sum like
+ * sum (either may be NULL) -- both gradients have the same values; grad_weight [D];  D up to 16384 (SRWM_ESIZE beyond);
+ * workspace: residual_rms_norm_workspace() floats.
+ */
+SRWM_API int residual_rms_norm_forward_f32(const float *x, const void *residual, const float *weight, float *out, void *sum,
+                             float *rstd, const float eps[1], int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_forward_bf16(const uint16_t *x, const void *residual, const float *weight, uint16_t *out, void *sum,
+                             float *rstd, const float eps[1], int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_e4m3_f32(const float *x, const void *residual, const float *weight, uint8_t *out, float *scale,
+                             void *sum, const float eps[1], int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_e4m3_bf16(const uint16_t *x, const void *residual, const float *weight, uint8_t *out, float *scale,
+                             void *sum, const float eps[1], int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_backward_f32(const void *sum, const float *weight, const float *rstd, const float *grad_out,
+                             const void *grad_sum, float *grad_x, void *grad_residual, float *grad_weight,
+                             float *workspace, int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_backward_bf16(const void *sum, const float *weight, const float *rstd, const uint16_t *grad_out,
+                             const void *grad_sum, uint16_t *grad_x, void *grad_residual, float *grad_weight,
+                             float *workspace, int rows, int D, unsigned flags, void *stream);
+SRWM_API int residual_rms_norm_workspace(int64_t floats[1], int rows, int D);
+
 
 /* Largest E the SRWM entry points accept (forward / backward), and the largest
  * E == M the delta entry points accept, on the current device. */

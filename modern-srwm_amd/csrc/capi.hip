@@ -113,6 +113,126 @@ bool refuses_fallback(unsigned flags) {
     return false;
 }
 
+// ---- selective scan, short convolution, norm
+Strided3 s3(const int64_t s[3]) { return s ? Strided3{s[0], s[1], s[2]} : Strided3{0, 0, 0}; }
+bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int64_t kMaxGrid = 1 << 23;   // workgroups along x: 256 threads each must stay below 2^32
+int64_t scan_part_a_floats(int N, int H, int E, int S) { return N * scan_part_a_row((int64_t)H * E, S); }
+int64_t scan_tiles(int H, int E, int G) { return ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile; }
+
+int scan_dims(int N, int H, int L, int E, int S, int G) {
+    if (!dims_ok(N, H, L, E) || S <= 0 || G <= 0 || H % G) return SRWM_EINVAL;
+    if (S > 64 || L > (1 << 30) || (int64_t)H * E > (1 << 30) || G > 65535 || scan_tiles(H, E, G) * N > kMaxGrid) return SRWM_ESIZE;
+    return SRWM_OK;
+}
+int conv_dims(int N, int H, int L, int E, int W) {
+    if (!dims_ok(N, H, L, E) || W <= 0) return SRWM_EINVAL;
+    if (W < 2 || W > 4 || L > (1 << 30) || (int64_t)H * E > (1 << 20) || conv_parts(N, L) > kMaxGrid ||
+        (int64_t)N * H * E > ((int64_t)1 << 31))
+        return SRWM_ESIZE;
+    return SRWM_OK;
+}
+int norm_dims(int rows, int D) {
+    if (rows <= 0 || D <= 0) return SRWM_EINVAL;
+    return rows > kMaxGrid ? SRWM_ESIZE : SRWM_OK;
+}
+
+int scan_forward(const void *u, const int64_t *us, const void *delta, const int64_t *ds, const void *z, const int64_t *zs,
+                 const void *B, const int64_t *Bs, const void *C, const int64_t *Cs, const float *A, const float *D,
+                 const float *bias, const float *state, const float *keep, const int *lengths, void *out, const int64_t *os,
+                 float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags, void *stream,
+                 bool bf16, bool step) {
+    if (!u || !delta || !B || !C || !A || !out || !last || !us || !ds || !Bs || !Cs || !os || (z && !zs)) return SRWM_EINVAL;
+    if (flags & ~SRWM_FLAG_SOFTPLUS) return SRWM_EINVAL;
+    if (const int r = scan_dims(N, H, L, E, S, G)) return r;
+    if (!stride_ok(us, N, H, L, E) || !stride_ok(ds, N, H, L, E) || (z && !stride_ok(zs, N, H, L, E)) ||
+        !stride_ok(Bs, N, G, L, S) || !stride_ok(Cs, N, G, L, S) || !out_stride_ok(os, N, H, L, E) || !al16(A) ||
+        !al16(state) || !al16(last) || !al16(saved))
+        return SRWM_ESTRIDE;
+    const ScanParams p{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, state, keep, lengths,
+                       out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS};
+    return step ? launch_scan_step(p, bf16, (hipStream_t)stream) : launch_scan_fwd(p, bf16, (hipStream_t)stream);
+}
+
+int scan_backward(const void *u, const int64_t *us, const void *delta, const int64_t *ds, const void *z, const int64_t *zs,
+                  const void *B, const int64_t *Bs, const void *C, const int64_t *Cs, const float *A, const float *D,
+                  const float *bias, const float *keep, const int *lengths, const float *saved, const void *go,
+                  const int64_t *gos, const float *glast, void *gu, const int64_t *gus, void *gdelta, const int64_t *gds,
+                  void *gz, const int64_t *gzs, void *gB, const int64_t *gBs, void *gC, const int64_t *gCs, float *gA,
+                  float *gD, float *gbias, float *gstate, float *workspace, int N, int H, int L, int E, int S, int G,
+                  unsigned flags, void *stream, bool bf16) {
+    if (!u || !delta || !B || !C || !A || !us || !ds || !Bs || !Cs || (z && (!zs || !gz || !gzs)) || !saved || !go || !gos ||
+        !gu || !gus || !gdelta || !gds || !gB || !gBs || !gC || !gCs || !gA || !workspace)
+        return SRWM_EINVAL;
+    if (flags & ~SRWM_FLAG_SOFTPLUS) return SRWM_EINVAL;
+    if (const int r = scan_dims(N, H, L, E, S, G)) return r;
+    if ((int64_t)N * G * L * 2 * S + (int64_t)H * E * (S + 2) > kMaxGrid * 256) return SRWM_ESIZE;
+    if (!stride_ok(us, N, H, L, E) || !stride_ok(ds, N, H, L, E) || (z && !stride_ok(zs, N, H, L, E)) ||
+        !stride_ok(Bs, N, G, L, S) || !stride_ok(Cs, N, G, L, S) || !stride_ok(gos, N, H, L, E) ||
+        !out_stride_ok(gus, N, H, L, E) || !out_stride_ok(gds, N, H, L, E) || (z && !out_stride_ok(gzs, N, H, L, E)) ||
+        !out_stride_ok(gBs, N, G, L, S) || !out_stride_ok(gCs, N, G, L, S) || !al16(A) || !al16(saved) || !al16(glast) ||
+        !al16(gstate) || !al16(workspace))
+        return SRWM_ESTRIDE;
+    ScanBwdParams b{};
+    b.f = ScanParams{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, nullptr, keep, lengths,
+                     nullptr, {}, nullptr, const_cast<float *>(saved), N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS};
+    b.go = go, b.gos = s3(gos), b.glast = glast;
+    b.gu = gu, b.gus = s3(gus), b.gdelta = gdelta, b.gds = s3(gds), b.gz = z ? gz : nullptr, b.gzs = s3(z ? gzs : nullptr);
+    b.gB = gB, b.gBs = s3(gBs), b.gC = gC, b.gCs = s3(gCs);
+    b.gA = gA, b.gD = gD, b.gbias = gbias, b.gstate = gstate;
+    b.part_a = workspace;                                                   // [N, H*E, S + 2]
+    b.part_bc = workspace + scan_part_a_floats(N, H, E, S);
+    return launch_scan_bwd(b, bf16, (hipStream_t)stream);
+}
+
+int conv_forward(const void *x, const int64_t *xs, const float *weight, const float *bias, const void *state,
+                 const float *keep, const int *lengths, void *out, const int64_t *os, void *last, int N, int H, int L, int E,
+                 int W, unsigned flags, void *stream, bool bf16, bool step) {
+    if (!x || !xs || !weight || !out || !os || !last || (flags & ~SRWM_FLAG_SILU)) return SRWM_EINVAL;
+    if (const int r = conv_dims(N, H, L, E, W)) return r;
+    if (!stride_ok(xs, N, H, L, E) || !out_stride_ok(os, N, H, L, E)) return SRWM_ESTRIDE;
+    const ConvParams p{x, s3(xs), weight, bias, state, keep, lengths, out, s3(os), last, N, H, L, E, W, flags & SRWM_FLAG_SILU};
+    const int r = step ? launch_conv_step(p, bf16, (hipStream_t)stream) : launch_conv_fwd(p, bf16, (hipStream_t)stream);
+    return r >= 0 ? r : SRWM_ESIZE;
+}
+
+int conv_backward(const void *x, const int64_t *xs, const float *weight, const float *bias, const void *state,
+                  const float *keep, const int *lengths, const void *go, const int64_t *gos, const void *glast, void *gx,
+                  const int64_t *gxs, float *gweight, float *gbias, void *gstate, float *workspace, int N, int H, int L,
+                  int E, int W, unsigned flags, void *stream, bool bf16) {
+    if (!x || !xs || !weight || !go || !gos || !gx || !gxs || !gweight || !workspace || (flags & ~SRWM_FLAG_SILU))
+        return SRWM_EINVAL;
+    if (const int r = conv_dims(N, H, L, E, W)) return r;
+    if (!stride_ok(xs, N, H, L, E) || !stride_ok(gos, N, H, L, E) || !out_stride_ok(gxs, N, H, L, E)) return SRWM_ESTRIDE;
+    ConvBwdParams b{};
+    b.f = ConvParams{x, s3(xs), weight, bias, state, keep, lengths, nullptr, {}, nullptr, N, H, L, E, W, flags & SRWM_FLAG_SILU};
+    b.go = go, b.gos = s3(gos), b.glast = glast, b.gx = gx, b.gxs = s3(gxs);
+    b.gweight = gweight, b.gbias = gbias, b.gstate = gstate, b.part = workspace;
+    const int r = launch_conv_bwd(b, bf16, (hipStream_t)stream);
+    return r >= 0 ? r : SRWM_ESIZE;
+}
+
+int norm_forward(const void *x, const void *residual, const float *weight, void *out, float *scale, void *sum, float *rstd,
+                 const float *eps, int rows, int D, unsigned flags, void *stream, bool bf16, bool e4m3) {
+    if (!x || !weight || !out || !eps || (e4m3 && !scale) || (residual && !sum) || (flags & ~SRWM_FLAG_RESIDUAL_F32))
+        return SRWM_EINVAL;
+    if (const int r = norm_dims(rows, D)) return r;
+    const bool r_bf16 = bf16 && !(residual && (flags & SRWM_FLAG_RESIDUAL_F32));
+    const NormParams p{x, residual, weight, out, residual ? sum : nullptr, rstd, scale, rows, D, eps[0]};
+    return launch_norm_fwd(p, bf16, r_bf16, e4m3, (hipStream_t)stream);
+}
+
+int norm_backward(const void *sum, const float *weight, const float *rstd, const void *go, const void *gsum, void *gx,
+                  void *gresidual, float *gweight, float *workspace, int rows, int D, unsigned flags, void *stream, bool bf16) {
+    if (!sum || !weight || !rstd || !go || !gx || !gweight || !workspace || (flags & ~SRWM_FLAG_RESIDUAL_F32))
+        return SRWM_EINVAL;
+    if (const int r = norm_dims(rows, D)) return r;
+    if (D > kNormBwdMax) return SRWM_ESIZE;
+    const NormBwdParams p{sum, weight, rstd, go, gsum, gx, gresidual, gweight, workspace, rows, D, norm_bwd_blocks(rows, D)};
+    const int r = launch_norm_bwd(p, bf16, bf16 && !(flags & SRWM_FLAG_RESIDUAL_F32), (hipStream_t)stream);
+    return r >= 0 ? r : SRWM_ESIZE;
+}
+
 size_t srwm_fwd_sq(int e) { return srwm_fwd_generic_lds_bytes(e, e); }
 size_t srwm_bwd_sq(int e) { return srwm_bwd_generic_lds_bytes(e, e); }
 size_t delta_fwd_sq(int e) { return delta_fwd_generic_lds_bytes(e, e); }
@@ -122,7 +242,7 @@ size_t delta_bwd_sq(int e) { return delta_bwd_generic_lds_bytes(e, e); }
 
 extern "C" {
 
-int srwm_hip_abi_version(void) { return 17; }
+int srwm_hip_abi_version(void) { return 18; }
 
 uint64_t srwm_hip_fallback_calls(void) { return g_fallback_calls.load(std::memory_order_relaxed); }
 
@@ -414,6 +534,188 @@ int delta_layer_prologue_grad_bf16(const uint16_t *gq, const int64_t gqs[3], con
                                                   {gvs[0], gvs[1], gvs[2]}, gbeta, {gbs[0], gbs[1], gbs[2]}, q, k,
                                                   beta, sums, grad_rows, N, H, L, E, M, (hipStream_t)stream);
     return r >= 0 ? r : SRWM_ESIZE;
+}
+
+int selective_scan_forward_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                               const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                               const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
+                               const float *A, const float *D, const float *delta_bias, const float *state,
+                               const float *keep, const int *lengths, float *out, const int64_t out_strides[3],
+                               float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags,
+                               void *stream) {
+    return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        state, keep, lengths, out, out_strides, last, saved, N, H, L, E, S, G, flags, stream, false, false);
+}
+
+int selective_scan_forward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                                const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                                const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                                const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                                const float *state, const float *keep, const int *lengths, uint16_t *out,
+                                const int64_t out_strides[3], float *last, float *saved, int N, int H, int L, int E,
+                                int S, int G, unsigned flags, void *stream) {
+    return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        state, keep, lengths, out, out_strides, last, saved, N, H, L, E, S, G, flags, stream, true, false);
+}
+
+int selective_scan_backward_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                                const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                                const float *B, const int64_t b_strides[3], const float *C,
+                                const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                                const float *keep, const int *lengths, const float *saved, const float *grad_out,
+                                const int64_t grad_out_strides[3], const float *grad_last, float *grad_u,
+                                const int64_t grad_u_strides[3], float *grad_delta,
+                                const int64_t grad_delta_strides[3], float *grad_z, const int64_t grad_z_strides[3],
+                                float *grad_B, const int64_t grad_b_strides[3], float *grad_C,
+                                const int64_t grad_c_strides[3], float *grad_A, float *grad_D, float *grad_bias,
+                                float *grad_state, float *workspace, int N, int H, int L, int E, int S, int G,
+                                unsigned flags, void *stream) {
+    return scan_backward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        keep, lengths, saved, grad_out, grad_out_strides, grad_last, grad_u, grad_u_strides, grad_delta,
+        grad_delta_strides, grad_z, grad_z_strides, grad_B, grad_b_strides, grad_C, grad_c_strides, grad_A, grad_D,
+        grad_bias, grad_state, workspace, N, H, L, E, S, G, flags, stream, false);
+}
+
+int selective_scan_backward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                                 const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                                 const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                                 const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                                 const float *keep, const int *lengths, const float *saved, const uint16_t *grad_out,
+                                 const int64_t grad_out_strides[3], const float *grad_last, uint16_t *grad_u,
+                                 const int64_t grad_u_strides[3], uint16_t *grad_delta,
+                                 const int64_t grad_delta_strides[3], uint16_t *grad_z,
+                                 const int64_t grad_z_strides[3], uint16_t *grad_B, const int64_t grad_b_strides[3],
+                                 uint16_t *grad_C, const int64_t grad_c_strides[3], float *grad_A, float *grad_D,
+                                 float *grad_bias, float *grad_state, float *workspace, int N, int H, int L, int E,
+                                 int S, int G, unsigned flags, void *stream) {
+    return scan_backward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        keep, lengths, saved, grad_out, grad_out_strides, grad_last, grad_u, grad_u_strides, grad_delta,
+        grad_delta_strides, grad_z, grad_z_strides, grad_B, grad_b_strides, grad_C, grad_c_strides, grad_A, grad_D,
+        grad_bias, grad_state, workspace, N, H, L, E, S, G, flags, stream, true);
+}
+
+int selective_scan_step_f32(const float *u, const int64_t u_strides[3], const float *delta,
+                            const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],
+                            const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
+                            const float *A, const float *D, const float *delta_bias, const float *keep, float *state,
+                            float *out, const int64_t out_strides[3], int N, int H, int E, int S, int G,
+                            unsigned flags, void *stream) {
+    return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        nullptr, keep, nullptr, out, out_strides, state, nullptr, N, H, 1, E, S, G, flags, stream, false, true);
+}
+
+int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
+                             const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
+                             const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
+                             const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
+                             const float *keep, float *state, uint16_t *out, const int64_t out_strides[3], int N,
+                             int H, int E, int S, int G, unsigned flags, void *stream) {
+    return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
+        nullptr, keep, nullptr, out, out_strides, state, nullptr, N, H, 1, E, S, G, flags, stream, true, true);
+}
+
+int causal_conv_forward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                            const float *state, const float *keep, const int *lengths, float *out,
+                            const int64_t out_strides[3], float *last, int N, int H, int L, int E, int W,
+                            unsigned flags, void *stream) {
+    return conv_forward(x, x_strides, weight, bias, state, keep, lengths, out, out_strides, last, N, H, L, E, W, flags,
+        stream, false, false);
+}
+
+int causal_conv_forward_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const uint16_t *state, const float *keep, const int *lengths, uint16_t *out,
+                             const int64_t out_strides[3], uint16_t *last, int N, int H, int L, int E, int W,
+                             unsigned flags, void *stream) {
+    return conv_forward(x, x_strides, weight, bias, state, keep, lengths, out, out_strides, last, N, H, L, E, W, flags,
+        stream, true, false);
+}
+
+int causal_conv_backward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                             const float *state, const float *keep, const int *lengths, const float *grad_out,
+                             const int64_t grad_out_strides[3], const float *grad_last, float *grad_x,
+                             const int64_t grad_x_strides[3], float *grad_weight, float *grad_bias, float *grad_state,
+                             float *workspace, int N, int H, int L, int E, int W, unsigned flags, void *stream) {
+    return conv_backward(x, x_strides, weight, bias, state, keep, lengths, grad_out, grad_out_strides, grad_last, grad_x,
+        grad_x_strides, grad_weight, grad_bias, grad_state, workspace, N, H, L, E, W, flags, stream, false);
+}
+
+int causal_conv_backward_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                              const uint16_t *state, const float *keep, const int *lengths, const uint16_t *grad_out,
+                              const int64_t grad_out_strides[3], const uint16_t *grad_last, uint16_t *grad_x,
+                              const int64_t grad_x_strides[3], float *grad_weight, float *grad_bias,
+                              uint16_t *grad_state, float *workspace, int N, int H, int L, int E, int W,
+                              unsigned flags, void *stream) {
+    return conv_backward(x, x_strides, weight, bias, state, keep, lengths, grad_out, grad_out_strides, grad_last, grad_x,
+        grad_x_strides, grad_weight, grad_bias, grad_state, workspace, N, H, L, E, W, flags, stream, true);
+}
+
+int causal_conv_step_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                         const float *keep, float *state, float *out, const int64_t out_strides[3], int N, int H,
+                         int E, int W, unsigned flags, void *stream) {
+    return conv_forward(x, x_strides, weight, bias, nullptr, keep, nullptr, out, out_strides, state, N, H, 1, E, W,
+        flags, stream, false, true);
+}
+
+int causal_conv_step_bf16(const uint16_t *x, const int64_t x_strides[3], const float *weight, const float *bias,
+                          const float *keep, uint16_t *state, uint16_t *out, const int64_t out_strides[3], int N,
+                          int H, int E, int W, unsigned flags, void *stream) {
+    return conv_forward(x, x_strides, weight, bias, nullptr, keep, nullptr, out, out_strides, state, N, H, 1, E, W,
+        flags, stream, true, true);
+}
+
+int residual_rms_norm_forward_f32(const float *x, const void *residual, const float *weight, float *out, void *sum,
+                                  float *rstd, const float eps[1], int rows, int D, unsigned flags, void *stream) {
+    return norm_forward(x, residual, weight, out, nullptr, sum, rstd, eps, rows, D, flags, stream, false, false);
+}
+
+int residual_rms_norm_forward_bf16(const uint16_t *x, const void *residual, const float *weight, uint16_t *out,
+                                   void *sum, float *rstd, const float eps[1], int rows, int D, unsigned flags,
+                                   void *stream) {
+    return norm_forward(x, residual, weight, out, nullptr, sum, rstd, eps, rows, D, flags, stream, true, false);
+}
+
+int residual_rms_norm_e4m3_f32(const float *x, const void *residual, const float *weight, uint8_t *out, float *scale,
+                               void *sum, const float eps[1], int rows, int D, unsigned flags, void *stream) {
+    return norm_forward(x, residual, weight, out, scale, sum, nullptr, eps, rows, D, flags, stream, false, true);
+}
+
+int residual_rms_norm_e4m3_bf16(const uint16_t *x, const void *residual, const float *weight, uint8_t *out,
+                                float *scale, void *sum, const float eps[1], int rows, int D, unsigned flags,
+                                void *stream) {
+    return norm_forward(x, residual, weight, out, scale, sum, nullptr, eps, rows, D, flags, stream, true, true);
+}
+
+int residual_rms_norm_backward_f32(const void *sum, const float *weight, const float *rstd, const float *grad_out,
+                                   const void *grad_sum, float *grad_x, void *grad_residual, float *grad_weight,
+                                   float *workspace, int rows, int D, unsigned flags, void *stream) {
+    return norm_backward(sum, weight, rstd, grad_out, grad_sum, grad_x, grad_residual, grad_weight, workspace, rows, D,
+        flags, stream, false);
+}
+
+int residual_rms_norm_backward_bf16(const void *sum, const float *weight, const float *rstd, const uint16_t *grad_out,
+                                    const void *grad_sum, uint16_t *grad_x, void *grad_residual, float *grad_weight,
+                                    float *workspace, int rows, int D, unsigned flags, void *stream) {
+    return norm_backward(sum, weight, rstd, grad_out, grad_sum, grad_x, grad_residual, grad_weight, workspace, rows, D,
+        flags, stream, true);
+}
+
+int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G) {
+    if (!floats) return SRWM_EINVAL;
+    if (const int r = scan_dims(N, H, L, E, S, G)) return r;
+    floats[0] = scan_part_a_floats(N, H, E, S) + scan_tiles(H, E, G) * N * G * L * 2 * S;
+    return SRWM_OK;
+}
+int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E, int W) {
+    if (!floats) return SRWM_EINVAL;
+    if (const int r = conv_dims(N, H, L, E, W)) return r;
+    floats[0] = conv_parts(N, L) * (W + 1) * H * E;
+    return SRWM_OK;
+}
+int residual_rms_norm_workspace(int64_t floats[1], int rows, int D) {
+    if (!floats) return SRWM_EINVAL;
+    if (const int r = norm_dims(rows, D)) return r;
+    floats[0] = (int64_t)norm_bwd_blocks(rows, D) * D;
+    return SRWM_OK;
 }
 
 int srwm_backward_wide_f32(const float *x, const int64_t xs[3], const float *q, const float *k,

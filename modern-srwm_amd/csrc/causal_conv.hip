@@ -1,0 +1,306 @@
+// Short causal depthwise convolution over whole sequences and for one token:
+//     out_t = f(bias + sum_j w[j] x_{t-W+1+j}),   f = silu or the identity
+// Inputs before the first step come from the carried rows, inputs before a reset count as zero.
+#include "common.h"
+#include "gates.h"
+#include "vec_io.h"
+
+namespace fw {
+namespace {
+
+constexpr int kConvLanes = 32, kConvRuns = 8, kConvSteps = 16;   // a workgroup: 32 vectors of channels x 8 runs of 16 steps
+
+template <int V>
+__device__ __forceinline__ void zero(float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+}
+
+// x at step t of a row: before the first step the carried rows (t = -1 the newest), zero without them.
+template <typename T, int W, int V>
+__device__ __forceinline__ void load_input(const T *x, int64_t stride, const T *state, int E, int64_t t, float (&v)[V]) {
+    if (t >= 0) load_vec<V>(x + t * stride, v);
+    else if (state) load_vec<V>(state + (W - 1 + t) * E, v);
+    else zero<V>(v);
+}
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs) {
+    const int64_t D = (int64_t)p.H * p.E;
+    const int64_t d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
+    const int n = blockIdx.x / runs;
+    const int64_t t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
+    if (d >= D || (t0 >= p.L && t0 > 0)) return;
+    const int h = d / p.E, e = d % p.E;
+    int Ln = p.L;
+    if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
+    const T *x = (const T *)p.x + n * p.xs.n + h * p.xs.h + e;
+    const T *state = p.state ? (const T *)p.state + ((int64_t)n * p.H + h) * (W - 1) * p.E + e : nullptr;
+    T *out = (T *)p.out + n * p.os.n + h * p.os.h + e;
+    const float *keep = p.keep ? p.keep + (int64_t)n * p.L : nullptr;
+
+    float w[W][V], bias[V], win[W][V];   // win: the last W inputs, the newest last
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j][i] = p.weight[(d + i) * W + j];
+        bias[i] = p.bias ? p.bias[d + i] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < W; ++j) zero<V>(win[j]);
+    auto push = [&](int64_t t) {
+        const bool reset = keep && t >= 0 && is_reset(keep[t]);
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) win[j][i] = reset ? 0.f : win[j + 1][i];
+        load_input<T, W, V>(x, p.xs.l, state, p.E, t, win[W - 1]);
+    };
+    const int64_t end = min(t0 + kConvSteps, (int64_t)Ln);
+    if (t0 < Ln || t0 == 0)
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j) push(t0 - (W - 1) + j);
+    for (int64_t t = t0; t < end; ++t) {
+        push(t);
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            o[i] = bias[i];
+#pragma unroll
+            for (int j = 0; j < W; ++j) o[i] = fmaf(w[j][i], win[j][i], o[i]);
+            if (p.silu) o[i] *= sigmoid(o[i]);
+        }
+        store_vec<V>(out + t * p.os.l, o);
+    }
+    float none[V];
+    zero<V>(none);
+    for (int64_t t = max(t0, (int64_t)Ln); t < min(t0 + kConvSteps, (int64_t)p.L); ++t) store_vec<V>(out + t * p.os.l, none);
+    // the run with the row's last step hands the carried rows on
+    if (Ln > 0 ? (t0 < Ln && Ln <= t0 + kConvSteps) : t0 == 0) {
+        T *last = (T *)p.last + ((int64_t)n * p.H + h) * (W - 1) * p.E + e;
+#pragma unroll
+        for (int j = 0; j + 1 < W; ++j) store_vec<V>(last + (int64_t)j * p.E, win[j + 1]);
+    }
+}
+
+// gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre); a run walks its steps and the W - 1 behind them, carrying the
+// gradients of the last W inputs, each complete when the window leaves it.
+template <typename T, int W, int V>
+__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs) {
+    const ConvParams &p = b.f;
+    const int64_t D = (int64_t)p.H * p.E;
+    const int64_t d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
+    const int n = blockIdx.x / runs;
+    const int64_t t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
+    __shared__ float red[kConvRuns][kConvLanes][V];
+    float gw[W + 1][V];
+#pragma unroll
+    for (int j = 0; j <= W; ++j) zero<V>(gw[j]);
+    if (d < D && t0 < p.L) {
+        const int h = d / p.E, e = d % p.E;
+        int Ln = p.L;
+        if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
+        const T *x = (const T *)p.x + n * p.xs.n + h * p.xs.h + e;
+        const T *go = (const T *)b.go + n * b.gos.n + h * b.gos.h + e;
+        T *gx = (T *)b.gx + n * b.gxs.n + h * b.gxs.h + e;
+        const int64_t srow = ((int64_t)n * p.H + h) * (W - 1) * p.E + e;
+        const T *state = p.state ? (const T *)p.state + srow : nullptr;
+        const T *glast = b.glast ? (const T *)b.glast + srow : nullptr;
+        T *gstate = b.gstate ? (T *)b.gstate + srow : nullptr;
+        const float *keep = p.keep ? p.keep + (int64_t)n * p.L : nullptr;
+
+        float w[W][V], bias[V], win[W][V], acc[W][V];   // acc[j]: gradient of the input j steps back
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j][i] = p.weight[(d + i) * W + j];
+            bias[i] = p.bias ? p.bias[d + i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) zero<V>(win[j]), zero<V>(acc[j]);
+        int since = W;   // steps since the last reset, at most W
+        for (int64_t t = t0 - (W - 1); t < t0 + kConvSteps + W - 1; ++t) {
+            const bool reset = keep && t >= 0 && t < Ln && is_reset(keep[t]);
+            since = reset ? 0 : min(since + 1, W);
+#pragma unroll
+            for (int j = 0; j + 1 < W; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[j][i] = reset ? 0.f : win[j + 1][i];
+            zero<V>(win[W - 1]);
+            if (t < Ln) load_input<T, W, V>(x, p.xs.l, state, p.E, t, win[W - 1]);
+#pragma unroll
+            for (int j = W - 1; j > 0; --j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[j][i] = acc[j - 1][i];
+            zero<V>(acc[0]);
+            if (t >= t0 && t < Ln) {
+                float g[V];
+                load_vec<V>(go + t * b.gos.l, g);
+                if (p.silu) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        float o = bias[i];
+#pragma unroll
+                        for (int j = 0; j < W; ++j) o = fmaf(w[j][i], win[j][i], o);
+                        const float q = sigmoid(o);
+                        g[i] *= q * fmaf(o, 1.f - q, 1.f);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (j <= since)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[j][i] = fmaf(w[W - 1 - j][i], g[i], acc[j][i]);
+                if (t < t0 + kConvSteps) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) gw[j][i] = fmaf(g[i], win[j][i], gw[j][i]);
+                        gw[W][i] += g[i];
+                    }
+                }
+            } else if (t == Ln && glast) {
+                // one step behind the end: the carried rows are the inputs 1 .. W-1 steps back
+#pragma unroll
+                for (int j = 1; j < W; ++j)
+                    if (j <= since) {   // `since` already counts this step
+                        float g[V];
+                        load_vec<V>(glast + (int64_t)(W - 1 - j) * p.E, g);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) acc[j][i] += g[i];
+                    }
+            }
+            const int64_t done = t - (W - 1);   // the input that leaves the window
+            if (done >= t0 && done < p.L) store_vec<V>(gx + done * b.gxs.l, acc[W - 1]);
+            if (done < 0 && t >= 0 && t0 == 0 && gstate) store_vec<V>(gstate + (W - 1 + done) * p.E, acc[W - 1]);
+        }
+    }
+    float *part = b.part + (int64_t)blockIdx.x * (W + 1) * D;
+#pragma unroll
+    for (int j = 0; j <= W; ++j) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < V; ++i) red[threadIdx.y][threadIdx.x][i] = gw[j][i];
+        __syncthreads();
+        for (int i = threadIdx.y * kConvLanes + threadIdx.x; i < kConvLanes * V; i += kConvLanes * kConvRuns) {
+            const int64_t at = (int64_t)blockIdx.y * kConvLanes * V + i;
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < kConvRuns; ++r) v += red[r][i / V][i % V];
+            if (at < D) part[j * D + at] = v;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void conv_join_kernel(const float *part, float *gweight, float *gbias, int64_t D, int W,
+                                                        int parts) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= D * (W + 1)) return;
+    const int j = i / D;
+    const int64_t d = i % D;
+    if (j == W && !gbias) return;
+    float v = 0.f;
+    for (int r = 0; r < parts; ++r) v += part[((int64_t)r * (W + 1) + j) * D + d];
+    if (j < W) gweight[d * W + j] = v;
+    else gbias[d] = v;
+}
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(256) void conv_step_kernel(ConvParams p) {
+    const int64_t D = (int64_t)p.H * p.E;
+    const int64_t i0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t per = D / V;
+    if (i0 >= p.N * per) return;
+    const int64_t n = i0 / per, d = i0 % per * V;
+    const int h = d / p.E, e = d % p.E;
+    T *state = (T *)p.last + (n * p.H + h) * (W - 1) * p.E + e;
+    float win[W][V], o[V];
+    const bool reset = p.keep && is_reset(p.keep[n]);
+#pragma unroll
+    for (int j = 0; j + 1 < W; ++j) {
+        load_vec<V>(state + (int64_t)j * p.E, win[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = reset ? 0.f : win[j][i];
+    }
+    load_vec<V>((const T *)p.x + n * p.xs.n + h * p.xs.h + e, win[W - 1]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        o[i] = p.bias ? p.bias[d + i] : 0.f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[i] = fmaf(p.weight[(d + i) * W + j], win[j][i], o[i]);
+        if (p.silu) o[i] *= sigmoid(o[i]);
+    }
+    store_vec<V>((T *)p.out + n * p.os.n + h * p.os.h + e, o);
+#pragma unroll
+    for (int j = 0; j + 1 < W; ++j) store_vec<V>(state + (int64_t)j * p.E, win[j + 1]);
+}
+
+// Rows that can be read V elements at a time: E and every stride a multiple of V, bases aligned.
+bool vec_ok(const void *q, int64_t bytes) { return ((uintptr_t)q & (bytes - 1)) == 0; }
+template <typename T, int V>
+bool rows_ok(const void *q, const Strided3 &s) {
+    return vec_ok(q, sizeof(T) * V) && s.n % V == 0 && s.h % V == 0 && s.l % V == 0;
+}
+template <typename T, int V>
+bool conv_vec(const ConvParams &p) {
+    return p.E % V == 0 && rows_ok<T, V>(p.x, p.xs) && rows_ok<T, V>(p.out, p.os) && vec_ok(p.state, sizeof(T) * V) &&
+           vec_ok(p.last, sizeof(T) * V);
+}
+
+int conv_runs(int L) { return (L + kConvRuns * kConvSteps - 1) / (kConvRuns * kConvSteps); }
+
+template <typename T, int W>
+int fwd(const ConvParams &p, hipStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t D = (int64_t)p.H * p.E;
+    const dim3 block(kConvLanes, kConvRuns);
+    const int runs = conv_runs(p.L);
+    auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
+    if (conv_vec<T, V>(p)) conv_fwd_kernel<T, W, V><<<grid(V), block, 0, s>>>(p, runs);
+    else conv_fwd_kernel<T, W, 1><<<grid(1), block, 0, s>>>(p, runs);
+    return (int)hipGetLastError();
+}
+template <typename T, int W>
+int bwd(const ConvBwdParams &b, hipStream_t s) {
+    constexpr int V = 4;
+    const ConvParams &p = b.f;
+    const int64_t D = (int64_t)p.H * p.E;
+    const dim3 block(kConvLanes, kConvRuns);
+    const int runs = conv_runs(p.L);
+    auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
+    if (p.E % V == 0 && rows_ok<T, V>(p.x, p.xs) && rows_ok<T, V>(b.go, b.gos) && rows_ok<T, V>(b.gx, b.gxs) &&
+        vec_ok(p.state, sizeof(T) * V) && vec_ok(b.glast, sizeof(T) * V) && vec_ok(b.gstate, sizeof(T) * V))
+        conv_bwd_kernel<T, W, V><<<grid(V), block, 0, s>>>(b, runs);
+    else conv_bwd_kernel<T, W, 1><<<grid(1), block, 0, s>>>(b, runs);
+    const int r = (int)hipGetLastError();
+    if (r) return r;
+    conv_join_kernel<<<(unsigned)((D * (W + 1) + 255) / 256), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);
+    return (int)hipGetLastError();
+}
+template <typename T, int W>
+int step(const ConvParams &p, hipStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t D = (int64_t)p.H * p.E;
+    auto grid = [&](int v) { return (unsigned)((p.N * (D / v) + 255) / 256); };
+    if (conv_vec<T, V>(p)) conv_step_kernel<T, W, V><<<grid(V), 256, 0, s>>>(p);
+    else conv_step_kernel<T, W, 1><<<grid(1), 256, 0, s>>>(p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+int64_t conv_parts(int N, int L) { return (int64_t)N * conv_runs(L); }
+
+#define FW_BY_TAPS(FN, W, P)                                        \
+    switch (W) {                                                    \
+        case 2: return bf16 ? FN<__bf16, 2>(P, s) : FN<float, 2>(P, s); \
+        case 3: return bf16 ? FN<__bf16, 3>(P, s) : FN<float, 3>(P, s); \
+        case 4: return bf16 ? FN<__bf16, 4>(P, s) : FN<float, 4>(P, s); \
+    }                                                               \
+    return -1;
+
+int launch_conv_fwd(const ConvParams &p, bool bf16, hipStream_t s) { FW_BY_TAPS(fwd, p.W, p) }
+int launch_conv_bwd(const ConvBwdParams &b, bool bf16, hipStream_t s) { FW_BY_TAPS(bwd, b.f.W, b) }
+int launch_conv_step(const ConvParams &p, bool bf16, hipStream_t s) { FW_BY_TAPS(step, p.W, p) }
+
+}  // namespace fw

@@ -153,6 +153,84 @@ struct DeltaBwdParamsBf16 {
     unsigned bf16_grads;       // chunkwise kernels: gQ, gK, gV are bf16 buffers behind the float pointers
 };
 
+// Selective scan (selective_scan.hip, selective_scan_bwd.hip); io tensors are fp32 or bf16, all of one type.
+struct ScanParams {
+    const void *u, *delta, *z, *B, *C;   // fp32 or bf16; z may be null
+    Strided3 us, ds, zs, Bs, Cs;
+    const float *A, *D, *bias;           // [H,E,S], [H,E], [H,E]; D and bias may be null
+    const float *state, *keep;           // [N,H,E,S] or null (zeros), [N,L] or null (no resets)
+    const int *lengths;                  // [N] or null (all L)
+    void *out;
+    Strided3 os;
+    float *last;                         // [N,H,E,S]
+    float *saved;                        // [N, ceil(L/16), H*E, S] states before each block of 16 steps, or null
+    int N, H, L, E, S, G;
+    unsigned softplus;
+};
+
+struct ScanBwdParams {
+    ScanParams f;                        // the forward's inputs; `saved` as it left it; out and last are not used
+    const void *go;                      // gradient of out
+    Strided3 gos;
+    const float *glast;                  // gradient of last, or null
+    void *gu, *gdelta, *gz;              // strided like the outputs they are (gz null without z)
+    Strided3 gus, gds, gzs;
+    void *gB, *gC;                       // strided [N,G,L,S]
+    Strided3 gBs, gCs;
+    float *gA, *gD, *gbias, *gstate;     // gD, gbias, gstate may be null
+    float *part_bc;                      // [tiles of a group, N, G, L, 2, S]
+    float *part_a;                       // [N, scan_part_a_row]: gA [H*E, S], gD [H*E], gbias [H*E]
+};
+
+// Short causal convolution (causal_conv.hip)
+struct ConvParams {
+    const void *x;
+    Strided3 xs;
+    const float *weight, *bias;          // [H,E,W], [H,E] or null
+    const void *state;                   // [N,H,W-1,E] like x, or null (zeros)
+    const float *keep;                   // [N,L] or null
+    const int *lengths;                  // [N] or null
+    void *out;
+    Strided3 os;
+    void *last;                          // [N,H,W-1,E] like x
+    int N, H, L, E, W;
+    unsigned silu;
+};
+
+struct ConvBwdParams {
+    ConvParams f;                        // the forward's inputs
+    const void *go;
+    Strided3 gos;
+    const void *glast;                   // [N,H,W-1,E] like x, or null
+    void *gx;
+    Strided3 gxs;
+    float *gweight, *gbias;              // gbias may be null
+    void *gstate;                        // [N,H,W-1,E] like x, or null
+    float *part;                         // [parts, W + 1, H*E]
+};
+
+// Root-mean-square norm of a sum (residual_norm.hip); rows are dense
+struct NormParams {
+    const void *x, *residual;            // residual may be null
+    const float *weight;
+    void *out, *sum;                     // sum: like residual; null without one
+    float *rstd;                         // [rows] or null
+    float *scale;                        // e4m3 output: [rows]
+    int64_t rows;
+    int D;
+    float eps;
+};
+
+struct NormBwdParams {
+    const void *sum;                     // what the forward normalised, as it was stored
+    const float *weight, *rstd;
+    const void *go, *gsum;               // gsum may be null
+    void *gx, *gres;                     // gres may be null
+    float *gweight, *part;               // part: [blocks, D]
+    int64_t rows;
+    int D, blocks;
+};
+
 // ---- bf16 <-> fp32 (16-bit patterns; round to nearest even on the way down)
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t h) { return __uint_as_float(h << 16); }
 __device__ __forceinline__ uint16_t f32_to_bf16_bits(float f) {
@@ -235,6 +313,22 @@ int launch_delta_prologue_grad_bf16(const uint16_t *gq, const Strided3 &gqs, con
                                     uint16_t *gx, int N, int H, int L, int E, int M, hipStream_t s);
 int launch_delta_fwd_generic(const DeltaFwdParams &p, hipStream_t s);
 int launch_delta_bwd_generic(const DeltaBwdParams &p, hipStream_t s);
+
+// Selective scan, short convolution, norm.  bf16: the io tensors' type (else fp32).
+constexpr int kScanTile = 64;       // channels of a workgroup of the scan kernels
+// floats of a row of ScanBwdParams::part_a, a multiple of four so that every row can be written as float4
+inline __host__ __device__ int64_t scan_part_a_row(int64_t D, int S) { return (D * (S + 2) + 3) / 4 * 4; }
+int launch_scan_fwd(const ScanParams &p, bool bf16, hipStream_t s);
+int launch_scan_step(const ScanParams &p, bool bf16, hipStream_t s);   // u ... out: rows of one step; `last` is the state, in place
+int launch_scan_bwd(const ScanBwdParams &b, bool bf16, hipStream_t s);
+int64_t conv_parts(int N, int L);
+int launch_conv_fwd(const ConvParams &p, bool bf16, hipStream_t s);    // -1: no kernel for this number of taps
+int launch_conv_step(const ConvParams &p, bool bf16, hipStream_t s);   // as launch_scan_step
+int launch_conv_bwd(const ConvBwdParams &b, bool bf16, hipStream_t s);
+constexpr int kNormBwdMax = 16384;  // longest row that the norm's backward holds
+int norm_bwd_blocks(int64_t rows, int D);
+int launch_norm_fwd(const NormParams &p, bool x_bf16, bool r_bf16, bool e4m3, hipStream_t s);
+int launch_norm_bwd(const NormBwdParams &p, bool x_bf16, bool r_bf16, hipStream_t s);
 
 // Register-resident kernels for the head sizes that are compiled in; return -1
 // when E (E, M) has no specialisation so the caller can fall back to the generic kernel.

@@ -35,11 +35,14 @@ FLAG_EXACT_PRODUCTS = 512   # chunkwise kernels with bf16 inputs: every product 
 FLAG_BF16_GRADS = 1024      # chunkwise delta backward with bf16 inputs: grad_q, grad_k, grad_v written as bf16 by the library
 FLAG_SPARSE_V_OLD = 4096    # chunkwise delta forward: v_old only for steps with |beta| < 2^-24 (all a chunkwise backward reads of it)
 FLAG_NORM_EPS = 2048        # delta_layer_prologue: 1e-5 added to the normalisers of q and k
+FLAG_SOFTPLUS = 16384       # selective_scan: dt = softplus(delta + delta_bias)
+FLAG_SILU = 32768           # causal_conv: silu behind the convolution
+FLAG_RESIDUAL_F32 = 65536   # residual_rms_norm with bfloat16 rows: the residual and the sum are float32
 FLAG_STATE_SHIFT = 64      # layer entry points: the state tensors hold W minus the shared weights
 FLAG_FRESH_STATE = 128     # layer forward: start from the shared weights
 FLAG_SOFTMAX_INPUT = 256   # layer entry points: x is given before its softmax
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 # True: a call that the register-resident kernels do not take (head size without an instantiation, misaligned
 # base or strides) raises instead of running on the several times slower LDS-resident kernels
@@ -79,6 +82,27 @@ _SIGNATURES = {
     "delta_layer_prologue_grad_f32": [_F, _S] * 4 + [_F] * 5 + [_I] * 5 + [_U, ctypes.c_void_p],
     "delta_layer_prologue_bf16": [_F] * 6 + [_I] * 5 + [_U, ctypes.c_void_p],
     "delta_layer_prologue_grad_bf16": [_F, _S] * 4 + [_F] * 5 + [_I] * 5 + [_U, ctypes.c_void_p],
+    "selective_scan_forward_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_forward_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_backward_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 5 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_backward_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 5 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_step_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 6 + [_S] + [_I] * 5 + [_U, ctypes.c_void_p],
+    "selective_scan_step_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 6 + [_S] + [_I] * 5 + [_U, ctypes.c_void_p],
+    "causal_conv_forward_f32": [_F] + [_S] + [_F] * 6 + [_S] + [_F] + [_I] * 5 + [_U, ctypes.c_void_p],
+    "causal_conv_forward_bf16": [_F] + [_S] + [_F] * 6 + [_S] + [_F] + [_I] * 5 + [_U, ctypes.c_void_p],
+    "causal_conv_backward_f32": [_F] + [_S] + [_F] * 6 + [_S] + [_F] * 2 + [_S] + [_F] * 4 + [_I] * 5 + [_U, ctypes.c_void_p],
+    "causal_conv_backward_bf16": [_F] + [_S] + [_F] * 6 + [_S] + [_F] * 2 + [_S] + [_F] * 4 + [_I] * 5 + [_U, ctypes.c_void_p],
+    "causal_conv_step_f32": [_F] + [_S] + [_F] * 5 + [_S] + [_I] * 4 + [_U, ctypes.c_void_p],
+    "causal_conv_step_bf16": [_F] + [_S] + [_F] * 5 + [_S] + [_I] * 4 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_forward_f32": [_F] * 7 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_forward_bf16": [_F] * 7 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_e4m3_f32": [_F] * 7 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_e4m3_bf16": [_F] * 7 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_backward_f32": [_F] * 9 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "residual_rms_norm_backward_bf16": [_F] * 9 + [_I] * 2 + [_U, ctypes.c_void_p],
+    "selective_scan_workspace": [_S] + [_I] * 6,
+    "causal_conv_workspace": [_S] + [_I] * 5,
+    "residual_rms_norm_workspace": [_S] + [_I] * 2,
 }
 
 
@@ -842,3 +866,365 @@ def fast_weight_backward(q, k, v, beta, v_old, v_insert, grad_out, kv, grad_q, g
         for dst, src in zip(bf_outs, (grad_q, grad_k, grad_v, grad_beta)):
             if dst is not src:
                 dst.copy_(src)
+
+
+# ---- selective scan, short causal convolution, norm -------------------------------------------------------------------
+# These functions allocate what they return.  Optional tensors may be None.
+
+_I3 = ctypes.c_int64 * 3
+
+
+def _io_dtype(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not torch.float32 and t.dtype is not torch.bfloat16:
+        raise TypeError(f"{name} must be torch.float32 or torch.bfloat16 (got {t.dtype})")
+    return t.dtype
+
+
+def _on(t, name, shape, dtype, device):
+    """_require, and on the device of the call's other tensors."""
+    _require(t, name, shape, dtype)
+    if t.device != device:
+        raise RuntimeError(f"{name} lives on {t.device}, the call's other tensors on {device}")
+
+
+def _rows_in(t, name, shape, dtype, device):
+    """A (N, H, L, E) tensor, or the (N, H, E) rows of one step, as the kernels read it: any strides with a contiguous
+    last axis (other layouts are copied).  Returns the tensor, which the caller keeps until the launch, and its strides."""
+    _on(t, name, shape, dtype, device)
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, _I3(st[0], st[1], st[2] if len(shape) == 4 else 0)
+
+
+def _dense_in(t, name, shape, dtype, device):
+    """A dense tensor that starts at a multiple of 16 bytes (copied where it is not), or None."""
+    if t is None:
+        return None
+    _on(t, name, shape, dtype, device)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    if t.data_ptr() % 16:
+        t = t.clone()
+    return t
+
+
+class _InPlace:
+    """A dense, 16-byte aligned stand-in for a tensor that a kernel overwrites; anything else is written back on exit."""
+
+    def __init__(self, t):
+        self.t = t
+        self.work = t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+    def __enter__(self):
+        return self.work
+
+    def __exit__(self, *exc):
+        if self.work is not self.t and exc[0] is None:
+            self.t.copy_(self.work)
+        return False
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def rows_like(t):
+    """An empty tensor of t's shape and type in the memory order of t's rows, its last axis contiguous."""
+    out = torch.empty_like(t)
+    if out.stride(-1) != 1 and out.shape[-1] != 1:
+        out = torch.empty(t.shape, device=t.device, dtype=t.dtype)
+    return out
+
+
+def _workspace(fn, device, *dims):
+    n = (ctypes.c_int64 * 1)()
+    _check(fn(n, *dims), fn.__name__)
+    return torch.empty(n[0], device=device, dtype=torch.float32)
+
+
+def _masks(keep, lengths, N, L, device):
+    return _dense_in(keep, "keep", (N, L), torch.float32, device), _dense_in(lengths, "lengths", (N,), torch.int32, device)
+
+
+def _scan_sizes(u, A, B):
+    if u.dim() != 4 or A.dim() != 3 or B.dim() != 4:
+        raise ValueError("u must be (N, H, L, E), A (H, E, S), B and C (N, G, L, S)")
+    N, H, L, E = u.shape
+    G, S = B.shape[1], A.shape[-1]
+    if G == 0 or H % G:
+        raise ValueError(f"the {H} heads must divide into the {G} groups of B and C")
+    return N, H, L, E, S, G
+
+
+def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus, save):
+    """The scan over whole sequences.  Returns out (in the memory order of u's rows), last (N, H, E, S) and, with `save`,
+    the states that selective_scan_backward starts from (else None)."""
+    io = _io_dtype(u, "u")
+    for t, nm in ((A, "A"), (B, "B")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{nm} must be a torch.Tensor")
+    N, H, L, E, S, G = _scan_sizes(u, A, B)
+    dev = u.device
+    us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
+    ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
+    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
+    Bs, bstr = _rows_in(B, "B", (N, G, L, S), io, dev)
+    Cs, cstr = _rows_in(C, "C", (N, G, L, S), io, dev)
+    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
+    D = _dense_in(D, "D", (H, E), torch.float32, dev)
+    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
+    state = _dense_in(state, "state", (N, H, E, S), torch.float32, dev)
+    keep, lengths = _masks(keep, lengths, N, L, dev)
+    out = rows_like(u)
+    last = torch.empty((N, H, E, S), device=dev, dtype=torch.float32)
+    saved = torch.empty((N, (L + 15) // 16, H * E, S), device=dev, dtype=torch.float32) if save else None
+    if u.numel() == 0 or S == 0:
+        out.zero_()
+        last.zero_() if state is None else last.copy_(state)
+        return out, last, saved
+    fn = lib().selective_scan_forward_bf16 if io is torch.bfloat16 else lib().selective_scan_forward_f32
+    with torch.cuda.device(dev):
+        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(state),
+                  _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]), _p(last), _p(saved), N, H, L, E, S, G,
+                  FLAG_SOFTPLUS if softplus else 0, _stream(dev))
+    _check(code, fn.__name__)
+    return out, last, saved
+
+
+def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, saved, grad_out, grad_last, softplus,
+                            with_state):
+    """Gradients of selective_scan_forward, from the states it saved.  grad_last may be None.  Returns those of u, delta,
+    A, B, C, D, z, delta_bias and (with `with_state`) state; None for what was None."""
+    io = _io_dtype(u, "u")
+    N, H, L, E, S, G = _scan_sizes(u, A, B)
+    dev = u.device
+    us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
+    ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
+    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
+    Bs, bstr = _rows_in(B, "B", (N, G, L, S), io, dev)
+    Cs, cstr = _rows_in(C, "C", (N, G, L, S), io, dev)
+    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
+    Dd = _dense_in(D, "D", (H, E), torch.float32, dev)
+    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
+    keep, lengths = _masks(keep, lengths, N, L, dev)
+    saved = _dense_in(saved, "saved", (N, (L + 15) // 16, H * E, S), torch.float32, dev)
+    gos, gostr = _rows_in(grad_out, "grad_out", (N, H, L, E), io, dev)
+    glast = _dense_in(grad_last, "grad_last", (N, H, E, S), torch.float32, dev)
+    gu, gdelta, gz = rows_like(u), rows_like(delta), None if z is None else rows_like(z)
+    gB, gC = rows_like(B), rows_like(C)
+    gA = torch.empty_like(A)
+    gD, gbias = None if D is None else torch.empty_like(Dd), None if bias is None else torch.empty_like(bias)
+    gstate = torch.empty((N, H, E, S), device=dev, dtype=torch.float32) if with_state else None
+    if u.numel() == 0 or S == 0:
+        for t in (gu, gdelta, gz, gB, gC, gA, gD, gbias):
+            if t is not None:
+                t.zero_()
+        if gstate is not None:
+            gstate.zero_() if glast is None else gstate.copy_(glast)
+        return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
+    fn = lib().selective_scan_backward_bf16 if io is torch.bfloat16 else lib().selective_scan_backward_f32
+    work = _workspace(lib().selective_scan_workspace, dev, N, H, L, E, S, G)
+    st = lambda t: _I3(*t.stride()[:3])
+    with torch.cuda.device(dev):
+        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(Dd), _p(bias), _p(keep),
+                  _p(lengths), _p(saved), _p(gos), gostr, _p(glast), _p(gu), st(gu), _p(gdelta), st(gdelta), _p(gz),
+                  None if gz is None else st(gz), _p(gB), st(gB), _p(gC), st(gC), _p(gA), _p(gD), _p(gbias), _p(gstate),
+                  _p(work), N, H, L, E, S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
+    _check(code, fn.__name__)
+    return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
+
+
+def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus):
+    """One token: u, delta, z (N, H, E), B, C (N, G, S), keep (N,); state (N, H, E, S) is overwritten.  Returns out."""
+    io = _io_dtype(u, "u")
+    if u.dim() != 3 or not isinstance(A, torch.Tensor) or A.dim() != 3 or not isinstance(B, torch.Tensor) or B.dim() != 3:
+        raise ValueError("u must be (N, H, E), A (H, E, S), B and C (N, G, S)")
+    N, H, E = u.shape
+    G, S = B.shape[1], A.shape[-1]
+    if G == 0 or H % G:
+        raise ValueError(f"the {H} heads must divide into the {G} groups of B and C")
+    dev = u.device
+    us, ustr = _rows_in(u, "u", (N, H, E), io, dev)
+    ds, dstr = _rows_in(delta, "delta", (N, H, E), io, dev)
+    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, E), io, dev)
+    Bs, bstr = _rows_in(B, "B", (N, G, S), io, dev)
+    Cs, cstr = _rows_in(C, "C", (N, G, S), io, dev)
+    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
+    D = _dense_in(D, "D", (H, E), torch.float32, dev)
+    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
+    keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
+    _on(state, "state", (N, H, E, S), torch.float32, dev)
+    out = torch.empty((N, H, E), device=dev, dtype=io)
+    if u.numel() == 0 or S == 0:
+        return out.zero_()
+    fn = lib().selective_scan_step_bf16 if io is torch.bfloat16 else lib().selective_scan_step_f32
+    with torch.cuda.device(dev), _InPlace(state) as h:
+        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(keep),
+                  _p(h), _p(out), _I3(H * E, E, 0), N, H, E, S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
+    _check(code, fn.__name__)
+    return out
+
+
+def causal_conv_forward(x, weight, bias, state, keep, lengths, silu):
+    """Short causal depthwise convolution.  Returns out (in the memory order of x's rows) and last (N, H, W-1, E)."""
+    io = _io_dtype(x, "x")
+    if x.dim() != 4 or not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+        raise ValueError("x must be (N, H, L, E), weight (H, E, W)")
+    N, H, L, E = x.shape
+    W = weight.shape[-1]
+    dev = x.device
+    xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
+    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
+    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
+    if not 2 <= W <= 4:
+        raise ValueError(f"the convolution has 2 to 4 taps (got {W})")
+    state = _dense_in(state, "state", (N, H, W - 1, E), io, dev)
+    keep, lengths = _masks(keep, lengths, N, L, dev)
+    out = rows_like(x)
+    last = torch.empty((N, H, W - 1, E), device=dev, dtype=io)
+    if x.numel() == 0:
+        last.zero_() if state is None else last.copy_(state)
+        return out, last
+    fn = lib().causal_conv_forward_bf16 if io is torch.bfloat16 else lib().causal_conv_forward_f32
+    with torch.cuda.device(dev):
+        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]),
+                  _p(last), N, H, L, E, W, FLAG_SILU if silu else 0, _stream(dev))
+    _check(code, fn.__name__)
+    return out, last
+
+
+def causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_last, silu):
+    """Gradients of causal_conv_forward: x, weight, bias, state (None for what was None).  grad_last may be None."""
+    io = _io_dtype(x, "x")
+    N, H, L, E = x.shape
+    W = weight.shape[-1]
+    dev = x.device
+    xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
+    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
+    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
+    state = _dense_in(state, "state", (N, H, W - 1, E), io, dev)
+    keep, lengths = _masks(keep, lengths, N, L, dev)
+    gos, gostr = _rows_in(grad_out, "grad_out", (N, H, L, E), io, dev)
+    glast = _dense_in(grad_last, "grad_last", (N, H, W - 1, E), io, dev)
+    gx, gw = rows_like(x), torch.empty_like(weight)
+    gb = None if bias is None else torch.empty_like(bias)
+    gstate = None if state is None else torch.empty_like(state)
+    if x.numel() == 0:
+        gw.zero_()
+        if gb is not None:
+            gb.zero_()
+        if gstate is not None:
+            gstate.zero_() if glast is None else gstate.copy_(glast)
+        return gx, gw, gb, gstate
+    fn = lib().causal_conv_backward_bf16 if io is torch.bfloat16 else lib().causal_conv_backward_f32
+    work = _workspace(lib().causal_conv_workspace, dev, N, H, L, E, W)
+    with torch.cuda.device(dev):
+        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(gos), gostr, _p(glast), _p(gx),
+                  _I3(*gx.stride()[:3]), _p(gw), _p(gb), _p(gstate), _p(work), N, H, L, E, W, FLAG_SILU if silu else 0,
+                  _stream(dev))
+    _check(code, fn.__name__)
+    return gx, gw, gb, gstate
+
+
+def causal_conv_step(x, state, weight, bias, keep, silu):
+    """One token: x (N, H, E), keep (N,); state (N, H, W-1, E) is overwritten.  Returns out."""
+    io = _io_dtype(x, "x")
+    if x.dim() != 3 or not isinstance(weight, torch.Tensor) or weight.dim() != 3:
+        raise ValueError("x must be (N, H, E), weight (H, E, W)")
+    N, H, E = x.shape
+    W = weight.shape[-1]
+    dev = x.device
+    xs, xstr = _rows_in(x, "x", (N, H, E), io, dev)
+    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
+    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
+    if not 2 <= W <= 4:
+        raise ValueError(f"the convolution has 2 to 4 taps (got {W})")
+    keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
+    _on(state, "state", (N, H, W - 1, E), io, dev)
+    out = torch.empty((N, H, E), device=dev, dtype=io)
+    if x.numel() == 0:
+        return out
+    fn = lib().causal_conv_step_bf16 if io is torch.bfloat16 else lib().causal_conv_step_f32
+    with torch.cuda.device(dev), _InPlace(state) as h:
+        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(keep), _p(h), _p(out), _I3(H * E, E, 0), N, H, E, W,
+                  FLAG_SILU if silu else 0, _stream(dev))
+    _check(code, fn.__name__)
+    return out
+
+
+def _norm_rows(x, residual, weight):
+    io = _io_dtype(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must have a last axis to normalise over")
+    D, dev = x.shape[-1], x.device
+    xs = _dense_in(x, "x", None, io, dev)
+    rdt = io
+    if residual is not None:
+        rdt = _io_dtype(residual, "residual")
+        if io is torch.float32 and rdt is not torch.float32:
+            raise TypeError("a float32 x takes a float32 residual")
+        residual = _dense_in(residual, "residual", tuple(x.shape), rdt, dev)
+    weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
+    if D == 0:
+        raise ValueError("the norm's rows are empty")
+    flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
+    return xs, residual, weight, io, rdt, x.numel() // D, D, dev, flags
+
+
+def residual_rms_norm_forward(x, residual, weight, eps, save):
+    """Root-mean-square norm of x + residual over the last axis.  Returns out (like x), the sum (like residual; x itself
+    without one) and, with `save`, the rows' reciprocal norms for the backward (else None)."""
+    xs, residual, weight, io, rdt, rows, D, dev, flags = _norm_rows(x, residual, weight)
+    out = torch.empty(x.shape, device=dev, dtype=io)
+    total = xs if residual is None else torch.empty(x.shape, device=dev, dtype=rdt)
+    rstd = torch.empty(rows, device=dev, dtype=torch.float32) if save else None
+    if rows:
+        fn = lib().residual_rms_norm_forward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_forward_f32
+        with torch.cuda.device(dev):
+            code = fn(_p(xs), _p(residual), _p(weight), _p(out), None if residual is None else _p(total), _p(rstd),
+                      (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
+        _check(code, fn.__name__)
+    return out, total, rstd
+
+
+def residual_rms_norm_e4m3(x, residual, weight, eps):
+    """The same with out in torch.float8_e4m3fn.  Returns out, scale (the rows' scales, last axis 1), sum."""
+    xs, residual, weight, io, rdt, rows, D, dev, flags = _norm_rows(x, residual, weight)
+    out = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
+    scale = torch.empty((*x.shape[:-1], 1), device=dev, dtype=torch.float32)
+    total = xs if residual is None else torch.empty(x.shape, device=dev, dtype=rdt)
+    if rows:
+        fn = lib().residual_rms_norm_e4m3_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_e4m3_f32
+        with torch.cuda.device(dev):
+            code = fn(_p(xs), _p(residual), _p(weight), _p(out), _p(scale), None if residual is None else _p(total),
+                      (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
+        _check(code, fn.__name__)
+    return out, scale, total
+
+
+def residual_rms_norm_backward(total, weight, rstd, grad_out, grad_total, with_residual):
+    """Gradients of residual_rms_norm_forward from the sum it returned: x (like grad_out), residual (like the sum; None
+    without `with_residual`), weight.  grad_total may be None."""
+    io, rdt, D, dev = _io_dtype(grad_out, "grad_out"), _io_dtype(total, "total"), total.shape[-1], total.device
+    total = _dense_in(total, "total", None, rdt, dev)
+    weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
+    go = _dense_in(grad_out, "grad_out", tuple(total.shape), io, dev)
+    gt = _dense_in(grad_total, "grad_total", tuple(total.shape), rdt, dev)
+    rows = total.numel() // D
+    gx = torch.empty(total.shape, device=dev, dtype=io)
+    gr = torch.empty(total.shape, device=dev, dtype=rdt) if with_residual else None
+    gw = torch.empty_like(weight)
+    if not rows:
+        return gx, gr, gw.zero_()
+    fn = lib().residual_rms_norm_backward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_backward_f32
+    work = _workspace(lib().residual_rms_norm_workspace, dev, rows, D)
+    flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
+    with torch.cuda.device(dev):
+        code = fn(_p(total), _p(weight), _p(rstd), _p(go), _p(gt), _p(gx), _p(gr), _p(gw), _p(work), rows, D, flags,
+                  _stream(dev))
+    _check(code, fn.__name__)
+    return gx, gr, gw

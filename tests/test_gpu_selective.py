@@ -1,0 +1,404 @@
+"""Selective scan, short causal convolution and their single-token forms on the GPU against the oracle in 64 bits.
+
+Tolerances, relative to the largest value of the tensor: 1e-5 with float32 inputs (the bar of the other operators: a
+result here is a sum of at most some thousand products whose factors carry a few roundings of 2^-24 each).  With bfloat16
+inputs the oracle sees the same rounded inputs and a bfloat16 result is off by at most half a step more, 2^-8 of its own
+value; the float32 results (states, gradients of parameters) keep the first bar."""
+import pytest
+import torch
+
+from oracle import selective
+from residual_norm import residual_rms_norm
+from selective_scan import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+HALF_STEP = torch.finfo(torch.bfloat16).eps / 2
+
+
+def check(got, want, name):
+    want = want.detach()
+    got64 = got.detach().cpu().double()
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    assert torch.isfinite(got64).all() or not torch.isfinite(want).all(), name
+    top = float(want.abs().max()) if want.numel() else 0.0
+    tol = 1e-5 * top + 1e-30 + (HALF_STEP * want.abs() if got.dtype == torch.bfloat16 else 0)
+    worst = float(((got64 - want).abs() - tol).max()) if want.numel() else 0.0
+    assert worst <= 0, f"{name}: over the tolerance by {worst:.3g} (largest value {top:.3g})"
+
+
+def rows(g, N, H, L, E, dtype, order):
+    """(N, H, L, E): dense; the view of step-major storage; or that of a wider row that starts at an odd element."""
+    if order == "dense":
+        t = torch.randn(N, H, L, E, generator=g)
+    elif order == "steps":
+        t = torch.randn(L, N, H, E, generator=g).permute(1, 2, 0, 3)
+    else:
+        t = torch.randn(L, N, H, 2 * E + 3, generator=g)[..., 1:E + 1].permute(1, 2, 0, 3)
+    return t.to(dtype)
+
+
+def place(t, like=None):
+    """On the GPU with the strides of the CPU tensor."""
+    base = torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=DEV)
+    return base.copy_(t)
+
+
+def scan_case(N, H, L, E, S, G, dtype=torch.float32, order="steps", gate=True, D=True, bias=True, state=True, keep=False,
+              lengths=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    a = dict(u=rows(g, N, H, L, E, dtype, order), delta=rows(g, N, H, L, E, dtype, order),
+             A=-torch.exp(torch.randn(H, E, S, generator=g) * 0.7), B=rows(g, N, G, L, S, dtype, order),
+             C=rows(g, N, G, L, S, dtype, order), D=torch.randn(H, E, generator=g) if D else None,
+             z=rows(g, N, H, L, E, dtype, order) if gate else None,
+             delta_bias=torch.randn(H, E, generator=g) - 1 if bias else None,
+             state=torch.randn(N, H, E, S, generator=g) if state else None)
+    m = dict(keep=(torch.rand(N, L, generator=g) > 0.15).float() if keep else None,
+             lengths=torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None)
+    go = rows(g, N, H, L, E, dtype, order)
+    return a, m, go, torch.randn(N, H, E, S, generator=g)
+
+
+def run_scan(a, m, go, gl, softplus=True):
+    """(got, want): dicts of the outputs and of every gradient."""
+    want_in = {k: None if v is None else v.double().requires_grad_() for k, v in a.items()}
+    out, last = selective.scan(**want_in, **m, softplus=softplus)
+    leaves = [k for k in a if a[k] is not None]
+    grads = torch.autograd.grad((out * go.double()).sum() + (last * gl.double()).sum(), [want_in[k] for k in leaves],
+                                allow_unused=True)
+    want = dict(out=out, last=last, **{"g_" + k: torch.zeros_like(want_in[k]) if v is None else v for k, v in zip(leaves, grads)})
+    got_in = {k: None if v is None else place(v).requires_grad_() for k, v in a.items()}
+    md = {k: None if v is None else v.to(DEV) for k, v in m.items()}
+    out, last = selective_scan(**got_in, **md, softplus=softplus)
+    grads = torch.autograd.grad((out, last), [got_in[k] for k in leaves], (place(go), gl.to(DEV)))
+    got = dict(out=out, last=last, **{"g_" + k: v for k, v in zip(leaves, grads)})
+    with torch.no_grad():      # the path without the saved states gives the same bits
+        o2, l2 = selective_scan(**got_in, **md, softplus=softplus)
+    assert torch.equal(o2, out) and torch.equal(l2, last)
+    return got, want
+
+
+SHAPES = [(1, 1, 1, 1, 16, 1), (2, 3, 17, 5, 16, 3), (1, 6, 33, 20, 8, 2), (3, 2, 50, 32, 12, 1), (2, 1, 40, 130, 32, 1),
+          (1, 2, 20, 9, 64, 2), (1, 1, 16, 64, 4, 1), (2, 8, 31, 32, 16, 8), (1, 1, 2, 3, 1, 1), (1, 2, 19, 7, 37, 1)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_scan_and_gradients(shape, dtype):
+    got, want = run_scan(*scan_case(*shape, dtype=dtype))
+    for k in want:
+        check(got[k], want[k], k)
+
+
+@pytest.mark.parametrize("options", [
+    dict(gate=False), dict(D=False), dict(bias=False), dict(state=False), dict(gate=False, D=False, bias=False, state=False),
+    dict(keep=True), dict(lengths=[23, 0, 1]), dict(keep=True, lengths=[23, 16, 17]), dict(lengths=[40, -3, 5]),
+    dict(order="dense"), dict(order="offset"), dict(order="offset", keep=True, gate=False)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_scan_options(options, dtype):
+    got, want = run_scan(*scan_case(3, 2, 23, 13, 16, 2, dtype=dtype, **options))
+    for k in want:
+        check(got[k], want[k], k)
+
+
+def test_scan_without_softplus_and_with_growing_states():
+    a, m, go, gl = scan_case(2, 2, 20, 6, 16, 1, bias=False)
+    a["delta"] = a["delta"].abs() * 0.1
+    a["A"] = -a["A"]                                       # a decay above one is allowed
+    got, want = run_scan(a, m, go, gl, softplus=False)
+    for k in want:
+        check(got[k], want[k], k)
+
+
+def test_scan_step_sizes_from_tiny_to_large():
+    """softplus over its whole range: for large negative arguments the step is exp of them, to full relative precision."""
+    L = 24
+    a, m, go, gl = scan_case(1, 1, L, 8, 16, 1, bias=False, gate=False, D=False, state=False)
+    a["delta"] = torch.linspace(-60, 40, L)[None, None, :, None].expand(1, 1, L, 8).contiguous()
+    a["u"] = torch.randn(1, 1, L, 8, generator=torch.Generator().manual_seed(2)) * torch.exp(-a["delta"].clamp(max=0))
+    got, want = run_scan(a, m, go, gl)
+    for k in ("out", "last", "g_u", "g_B", "g_C", "g_A"):
+        check(got[k], want[k], k)
+    ratio = got["g_delta"].cpu().double() / want["g_delta"]
+    assert float((ratio[:, :, :14] - 1).abs().max()) < 1e-4    # tiny steps: the gradient is relative to themselves
+
+
+@pytest.mark.parametrize("N,H,L,E,S,G", [(1, 1, 700, 96, 16, 1), (2, 2, 333, 40, 8, 1)])
+def test_scan_long_rows(N, H, L, E, S, G):
+    got, want = run_scan(*scan_case(N, H, L, E, S, G, keep=True, lengths=[L, L - 100][:N]))
+    for k in want:
+        check(got[k], want[k], k)
+
+
+def test_masked_places_may_hold_anything():
+    """NaN behind a row's length and in a state that a reset drops change nothing and reach no result."""
+    a, m, go, gl = scan_case(2, 2, 21, 6, 16, 1, lengths=[21, 9])
+    m["keep"] = torch.ones(2, 21)
+    m["keep"][:, 0] = 0
+    m["keep"][0, 11] = 0
+    base, _ = run_scan(a, m, go, gl)
+    bad = {k: None if v is None else v.clone(memory_format=torch.preserve_format) for k, v in a.items()}
+    for k in ("u", "delta", "z", "B", "C"):
+        bad[k][1, :, 9:] = float("nan")
+    bad["state"][:] = float("inf")
+    gob = go.clone(memory_format=torch.preserve_format)
+    gob[1, :, 9:] = float("nan")
+    leaves = {k: place(v).requires_grad_() for k, v in bad.items()}
+    out, last = selective_scan(**leaves, keep=m["keep"].to(DEV), lengths=m["lengths"].to(DEV))
+    grads = torch.autograd.grad((out, last), list(leaves.values()), (place(gob), gl.to(DEV)))
+    assert torch.equal(out, base["out"]) and torch.equal(last, base["last"])
+    for k, v in zip(leaves, grads):
+        assert torch.equal(v, base["g_" + k]), k
+
+
+def test_nan_passes_where_it_is_not_masked():
+    a, m, _, _ = scan_case(1, 1, 8, 4, 16, 1)
+    a = {k: v if v is None else place(v) for k, v in a.items()}
+    a["delta"][0, 0, 3, 2] = float("nan")
+    out, last = selective_scan(**a)
+    nan = torch.isnan(out[0, 0])
+    assert nan[3:, 2].all() and not nan[:, [0, 1, 3]].any() and not nan[:3].any() and torch.isnan(last[0, 0, 2]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_packed_rows_equal_single_sequences(dtype):
+    a, _, _, _ = scan_case(1, 2, 45, 24, 16, 1, dtype=dtype, state=False)
+    a = {k: v if v is None else place(v) for k, v in a.items()}
+    cuts = [0, 7, 8, 30, 45]
+    keep = torch.ones(1, 45, device=DEV)
+    keep[0, cuts[:-1]] = 0
+    out, last = selective_scan(**a, keep=keep)
+    parts = [selective_scan(**{k: (v[:, :, lo:hi] if v is not None and v.dim() == 4 else v) for k, v in a.items()})
+             for lo, hi in zip(cuts, cuts[1:])]
+    want = torch.cat([p[0] for p in parts], 2).cpu().double()
+    check(out, want, "out")
+    check(last, parts[-1][1].cpu().double(), "last")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_scan_step(shape, dtype):
+    N, H, _, E, S, G = shape
+    a, m, _, _ = scan_case(N, H, 3, E, S, G, dtype=dtype, keep=True)
+    m["keep"][0, 1] = 0
+    out, last = selective.scan(**{k: v if v is None else v.double() for k, v in a.items()}, **m)
+    d = {k: v if v is None else place(v) for k, v in a.items()}
+    state, kd = d["state"], m["keep"].to(DEV)
+    for t in range(3):
+        o = selective_scan_step(d["u"][:, :, t], d["delta"][:, :, t], state, d["A"], d["B"][:, :, t], d["C"][:, :, t], d["D"],
+                                d["z"][:, :, t], d["delta_bias"], kd[:, t])
+        check(o, out[:, :, t], f"out {t}")
+    check(state, last, "state")
+
+
+def test_step_overwrites_a_strided_state():
+    a, _, _, _ = scan_case(2, 1, 1, 8, 16, 1)
+    d = {k: place(v) for k, v in a.items()}
+    pool = torch.zeros(2, 1, 8, 2, 16, device=DEV)
+    pool[:, :, :, 1] = d["state"]
+    one = {k: v[:, :, 0] if v.dim() == 4 and k != "state" else v for k, v in d.items()}
+    ref = d["state"].clone()
+    o1 = selective_scan_step(**{**one, "state": ref})
+    o2 = selective_scan_step(**{**one, "state": pool[:, :, :, 1]})
+    assert torch.equal(o1, o2) and torch.equal(pool[:, :, :, 1], ref) and not pool[:, :, :, 0].any()
+
+
+# ---- convolution
+def conv_case(N, H, L, E, W, dtype=torch.float32, order="steps", bias=True, state=True, keep=False, lengths=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    a = dict(x=rows(g, N, H, L, E, dtype, order), weight=torch.randn(H, E, W, generator=g),
+             bias=torch.randn(H, E, generator=g) if bias else None,
+             state=torch.randn(N, H, W - 1, E, generator=g).to(dtype) if state else None)
+    m = dict(keep=(torch.rand(N, L, generator=g) > 0.25).float() if keep else None,
+             lengths=torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None)
+    return a, m, rows(g, N, H, L, E, dtype, order), torch.randn(N, H, W - 1, E, generator=g).to(dtype)
+
+
+def run_conv(a, m, go, gl, silu=True):
+    w = {k: None if v is None else v.double().requires_grad_() for k, v in a.items()}
+    out, last = selective.conv(**w, **m, silu=silu)
+    leaves = [k for k in a if a[k] is not None]
+    grads = torch.autograd.grad((out * go.double()).sum() + (last * gl.double()).sum(), [w[k] for k in leaves], allow_unused=True)
+    want = dict(out=out, last=last, **{"g_" + k: torch.zeros_like(w[k]) if v is None else v for k, v in zip(leaves, grads)})
+    d = {k: None if v is None else place(v).requires_grad_() for k, v in a.items()}
+    md = {k: None if v is None else v.to(DEV) for k, v in m.items()}
+    out, last = causal_conv(**d, **md, silu=silu)
+    grads = torch.autograd.grad((out, last), [d[k] for k in leaves], (place(go), gl.to(DEV)))
+    got = dict(out=out, last=last, **{"g_" + k: v for k, v in zip(leaves, grads)})
+    for k in want:
+        check(got[k], want[k], k)
+
+
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1), (2, 3, 2, 5), (1, 2, 17, 16), (2, 1, 150, 40), (3, 2, 33, 7), (1, 4, 15, 64)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_conv_and_gradients(shape, W, dtype):
+    run_conv(*conv_case(*shape, W, dtype=dtype))
+
+
+@pytest.mark.parametrize("options", [
+    dict(bias=False), dict(state=False), dict(keep=True), dict(lengths=[37, 0, 1]), dict(keep=True, lengths=[37, 16, 18]),
+    dict(lengths=[99, -1, 33]), dict(order="dense"), dict(order="offset"), dict(silu=False), dict(keep=True, lengths=[2, 3, 17])], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_conv_options(options, dtype):
+    silu = options.pop("silu", True) if "silu" in options else True
+    run_conv(*conv_case(3, 2, 37, 24, 4, dtype=dtype, **options), silu=silu)
+
+
+def test_conv_masked_places_may_hold_anything():
+    a, m, go, gl = conv_case(2, 1, 20, 8, 4, lengths=[20, 6])
+    m["keep"] = torch.ones(2, 20)
+    m["keep"][:, 0] = 0
+    d = {k: place(v).requires_grad_() for k, v in a.items()}
+    md = {k: v.to(DEV) for k, v in m.items()}
+    out, last = causal_conv(**d, **md)
+    grads = torch.autograd.grad((out, last), list(d.values()), (place(go), gl.to(DEV)))
+    bad = {k: place(v) for k, v in a.items()}
+    bad["x"][1, :, 6:] = float("nan")
+    bad["state"][:] = float("nan")
+    gob = place(go)
+    gob[1, :, 6:] = float("nan")
+    bad = {k: v.requires_grad_() for k, v in bad.items()}
+    out2, last2 = causal_conv(**bad, **md)
+    grads2 = torch.autograd.grad((out2, last2), list(bad.values()), (gob, gl.to(DEV)))
+    assert torch.equal(out, out2) and torch.equal(last, last2)
+    for x, y in zip(grads, grads2):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("E", [1, 7, 24])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_conv_step(E, W, dtype):
+    a, m, _, _ = conv_case(3, 2, 5, E, W, dtype=dtype, keep=True)
+    m["keep"][1, 2] = 0
+    out, last = selective.conv(**{k: v.double() for k, v in a.items()}, **m)
+    d = {k: place(v) for k, v in a.items()}
+    kd = m["keep"].to(DEV)
+    for t in range(5):
+        check(causal_conv_step(d["x"][:, :, t], d["state"], d["weight"], d["bias"], kd[:, t]), out[:, :, t], f"out {t}")
+    check(d["state"], last, "state")
+
+
+# ---- together, and under a caller's conditions
+def _layer(d, h, state, keep=None, lengths=None):
+    """norm -> convolution -> scan on (N, H, L, E) rows, as a layer runs them."""
+    conv_state, scan_state = state
+    N, H, L, E = h.shape
+    y, _ = residual_rms_norm(h.permute(2, 0, 1, 3).reshape(L, N, H * E), None, d["norm"])
+    x, conv_state = causal_conv(y.reshape(L, N, H, E).permute(1, 2, 0, 3), d["weight"], d["bias"], conv_state, keep, lengths)
+    out, scan_state = selective_scan(x, x * 0.5, d["A"], d["B"][:, :, :L], d["C"][:, :, :L], d["D"], h, d["delta_bias"], scan_state,
+                                     keep, lengths)
+    return out, (conv_state, scan_state)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_prompt_then_tokens_equals_the_whole_sequence(dtype):
+    """A prompt of 13 steps and then 6 single tokens on the carried states, against all 19 steps at once."""
+    N, H, L, E, S = 2, 2, 19, 12, 16
+    a, _, _, _ = scan_case(N, H, L, E, S, 1, dtype=dtype, state=False)
+    g = torch.Generator().manual_seed(9)
+    d = {k: v if v is None else place(v) for k, v in a.items()}
+    d.update(weight=torch.randn(H, E, 4, generator=g).to(DEV), bias=torch.randn(H, E, generator=g).to(DEV),
+             norm=torch.rand(H * E, generator=g).to(DEV) + 0.5)
+    h = d["u"]
+    with torch.no_grad():
+        whole, (cs, ss) = _layer(d, h, (None, None))
+        out, (c, s) = _layer(d, h[:, :, :13], (None, None))
+        outs = [out]
+        for t in range(13, L):
+            y, _ = residual_rms_norm(h[:, :, t].reshape(N, H * E), None, d["norm"])
+            x = causal_conv_step(y.reshape(N, H, E), c, d["weight"], d["bias"])
+            outs.append(selective_scan_step(x, x * 0.5, s, d["A"], d["B"][:, :, t], d["C"][:, :, t], d["D"], h[:, :, t],
+                                            d["delta_bias"])[:, :, None])
+    check(torch.cat(outs, 2), whole.cpu().double(), "out")
+    check(c, cs.cpu().double(), "conv state")
+    check(s, ss.cpu().double(), "scan state")
+
+
+def test_another_stream_and_repeated_calls_give_the_same_bits():
+    a, m, go, gl = scan_case(3, 2, 70, 40, 16, 1, dtype=torch.bfloat16, keep=True, lengths=[70, 33, 5])
+    d = {k: place(v).requires_grad_() for k, v in a.items()}
+    md = {k: v.to(DEV) for k, v in m.items()}
+    gd = (place(go), gl.to(DEV))
+
+    def once():
+        out, last = selective_scan(**d, **md)
+        return [out, last, *torch.autograd.grad((out, last), list(d.values()), gd)]
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y, z in zip(first, second, once()):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_replays_from_a_captured_graph():
+    """Forward and backward of convolution and scan, captured once and replayed on new inputs in place."""
+    N, H, L, E, S = 2, 2, 50, 24, 16
+    a, m, go, gl = scan_case(N, H, L, E, S, 1, lengths=[50, 20])
+    ca, _, _, _ = conv_case(N, H, L, E, 4)
+    d = {k: place(v) for k, v in a.items()}
+    c = {k: place(v) for k, v in ca.items()}
+    ln, god, gld = m["lengths"].to(DEV), place(go), gl.to(DEV)
+
+    def step():
+        leaves = {k: v.detach().requires_grad_() for k, v in d.items() if k != "u"}
+        cl = {k: v.detach().requires_grad_() for k, v in c.items()}
+        x, _ = causal_conv(cl["x"], cl["weight"], cl["bias"], cl["state"], None, ln)
+        out, last = selective_scan(x, leaves["delta"], leaves["A"], leaves["B"], leaves["C"], leaves["D"], leaves["z"],
+                                   leaves["delta_bias"], leaves["state"], None, ln)
+        return [out, last, *torch.autograd.grad((out, last), [*leaves.values(), *cl.values()], (god, gld))]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    g = torch.Generator().manual_seed(11)
+    for k in range(3):
+        c["x"].copy_(torch.randn(c["x"].shape, generator=g))
+        d["state"].copy_(torch.randn(d["state"].shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in res]
+        for x, y in zip(got, step()):
+            assert torch.equal(x, y), k
+
+
+def test_offsets_past_32_bits():
+    """Rows whose elements lie further than 2^32 bytes (and 2^31 elements) apart."""
+    H, E, S, L = 1, 16, 16, 5
+    far = (1 << 31) // 4 + 64                                  # elements between two steps: 4 of them pass 2^31
+    store = torch.empty(far * (L - 1) + E, device=DEV, dtype=torch.bfloat16)
+    u = store.as_strided((1, H, L, E), (1, E, far, 1))
+    a, m, go, gl = scan_case(1, H, L, E, S, 1, dtype=torch.bfloat16)
+    u.copy_(a["u"])
+    d = {k: place(v) for k, v in a.items()}
+    near = selective_scan(**d)
+    wide = selective_scan(**{**d, "u": u})
+    assert torch.equal(near[0], wide[0]) and torch.equal(near[1], wide[1])
+    ca, _, _, _ = conv_case(1, H, L, E, 4, dtype=torch.bfloat16)
+    c = {k: place(v) for k, v in ca.items()}
+    u.copy_(c["x"])
+    assert torch.equal(causal_conv(**c)[0], causal_conv(**{**c, "x": u})[0])
+
+
+def test_empty_calls():
+    z = lambda *s: torch.zeros(*s, device=DEV)
+    state = torch.randn(2, 1, 4, 16, device=DEV)
+    out, last = selective_scan(z(2, 1, 0, 4), z(2, 1, 0, 4), z(1, 4, 16), z(2, 1, 0, 16), z(2, 1, 0, 16), state=state)
+    assert out.shape == (2, 1, 0, 4) and torch.equal(last, state)
+    leaf = state.clone().requires_grad_()
+    _, last = selective_scan(z(2, 1, 0, 4), z(2, 1, 0, 4), z(1, 4, 16), z(2, 1, 0, 16), z(2, 1, 0, 16), state=leaf)
+    g = torch.randn_like(state)
+    assert torch.equal(torch.autograd.grad(last, leaf, g)[0], g)
+    cs = torch.randn(2, 1, 3, 4, device=DEV)
+    out, last = causal_conv(z(2, 1, 0, 4), z(1, 4, 4), state=cs)
+    assert out.shape == (2, 1, 0, 4) and torch.equal(last, cs)
+    assert selective_scan(z(0, 1, 3, 4), z(0, 1, 3, 4), z(1, 4, 16), z(0, 1, 3, 16), z(0, 1, 3, 16))[0].shape == (0, 1, 3, 4)
