@@ -535,6 +535,8 @@ SRWM_API int delta_layer_prologue_grad_bf16(const uint16_t *gq, const int64_t gq
  *   lengths            [N] or NULL: steps of each row (values outside 0..L are taken as the nearer bound).  Steps behind
  *                      are not read, their rows of out are written as zeros, and last is the state after the row's end
  *   saved              dense [N, ceil(L/16), H*E, S]: states for the backward, or NULL
+ *   workspace          selective_scan_workspace(.., backward = 0) floats, contents ignored (NULL where that is 0).  Two
+ *                      calls that may overlap need one each; a captured graph keeps its own
  * S up to 64 (SRWM_ESIZE beyond).  A, state, last, saved, workspace and their gradients start at multiples of 16 bytes.
  * Arithmetic, states and the sums are fp32.
  */
@@ -543,21 +545,21 @@ SRWM_API int selective_scan_forward_f32(const float *u, const int64_t u_strides[
                              const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
                              const float *A, const float *D, const float *delta_bias, const float *state,
                              const float *keep, const int *lengths, float *out, const int64_t out_strides[3],
-                             float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags,
+                             float *last, float *saved, float *workspace, int N, int H, int L, int E, int S, int G, unsigned flags,
                              void *stream);
 SRWM_API int selective_scan_forward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
                              const int64_t delta_strides[3], const uint16_t *z, const int64_t z_strides[3],
                              const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
                              const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
                              const float *state, const float *keep, const int *lengths, uint16_t *out,
-                             const int64_t out_strides[3], float *last, float *saved, int N, int H, int L, int E,
+                             const int64_t out_strides[3], float *last, float *saved, float *workspace, int N, int H, int L, int E,
                              int S, int G, unsigned flags, void *stream);
 
 /*
  * Backward of the scan.  saved as the forward left it; grad_out strided [N,H,L,E]; grad_last dense [N,H,E,S] or NULL.
  * grad_u, grad_delta, grad_z strided [N,H,L,E] and grad_B, grad_C strided [N,G,L,S] in the type of the inputs (rows
  * behind a row's length are written as zeros); grad_A [H,E,S], grad_D and grad_bias [H,E], grad_state [N,H,E,S] fp32, the
- * last three may be NULL.  workspace: selective_scan_workspace() floats, contents ignored.  Sums over channels and over
+ * last three may be NULL.  workspace: selective_scan_workspace(.., backward = 1) floats, contents ignored.  Sums over channels and over
  * the batch are formed in a fixed order (the same call gives the same bits).
  */
 SRWM_API int selective_scan_backward_f32(const float *u, const int64_t u_strides[3], const float *delta,
@@ -583,7 +585,7 @@ SRWM_API int selective_scan_backward_bf16(const uint16_t *u, const int64_t u_str
                              const int64_t grad_c_strides[3], float *grad_A, float *grad_D, float *grad_bias,
                              float *grad_state, float *workspace, int N, int H, int L, int E, int S, int G,
                              unsigned flags, void *stream);
-SRWM_API int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G);
+SRWM_API int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G, int backward);
 
 /* One token: u, delta, z, out strided as above with L = 1 (the third stride is not used); keep [N] or NULL; state dense
  * [N,H,E,S], overwritten in place. */

@@ -117,7 +117,10 @@ bool refuses_fallback(unsigned flags) {
 Strided3 s3(const int64_t s[3]) { return s ? Strided3{s[0], s[1], s[2]} : Strided3{0, 0, 0}; }
 bool al16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int64_t kMaxGrid = 1 << 23;   // workgroups along x: 256 threads each must stay below 2^32
-int64_t scan_part_a_floats(int N, int H, int E, int S) { return N * scan_part_a_row((int64_t)H * E, S); }
+// floats of ScanParams::seg_decay (or seg_state), a multiple of four so that the next array starts aligned
+int64_t scan_segment_floats(int N, int H, int E, int S, int segments) {
+    return segments > 1 ? ((int64_t)N * segments * H * E * S + 3) / 4 * 4 : 0;
+}
 int64_t scan_tiles(int H, int E, int G) { return ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile; }
 
 int scan_dims(int N, int H, int L, int E, int S, int G) {
@@ -140,17 +143,23 @@ int norm_dims(int rows, int D) {
 int scan_forward(const void *u, const int64_t *us, const void *delta, const int64_t *ds, const void *z, const int64_t *zs,
                  const void *B, const int64_t *Bs, const void *C, const int64_t *Cs, const float *A, const float *D,
                  const float *bias, const float *state, const float *keep, const int *lengths, void *out, const int64_t *os,
-                 float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags, void *stream,
-                 bool bf16, bool step) {
+                 float *last, float *saved, float *workspace, int N, int H, int L, int E, int S, int G, unsigned flags,
+                 void *stream, bool bf16, bool step) {
     if (!u || !delta || !B || !C || !A || !out || !last || !us || !ds || !Bs || !Cs || !os || (z && !zs)) return SRWM_EINVAL;
     if (flags & ~SRWM_FLAG_SOFTPLUS) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
     if (!stride_ok(us, N, H, L, E) || !stride_ok(ds, N, H, L, E) || (z && !stride_ok(zs, N, H, L, E)) ||
         !stride_ok(Bs, N, G, L, S) || !stride_ok(Cs, N, G, L, S) || !out_stride_ok(os, N, H, L, E) || !al16(A) ||
-        !al16(state) || !al16(last) || !al16(saved))
+        !al16(state) || !al16(last) || !al16(saved) || !al16(workspace))
         return SRWM_ESTRIDE;
-    const ScanParams p{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, state, keep, lengths,
-                       out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS};
+    ScanParams p{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, state, keep, lengths,
+                 out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS, 1, L, nullptr, nullptr};
+    if (!step) {
+        p.segments = scan_segments(N, H, L, E, G, false, &p.seg_len);
+        if (p.segments > 1 && !workspace) return SRWM_EINVAL;
+        p.seg_decay = workspace;
+        p.seg_state = workspace + scan_segment_floats(N, H, E, S, p.segments);
+    }
     return step ? launch_scan_step(p, bf16, (hipStream_t)stream) : launch_scan_fwd(p, bf16, (hipStream_t)stream);
 }
 
@@ -175,13 +184,17 @@ int scan_backward(const void *u, const int64_t *us, const void *delta, const int
         return SRWM_ESTRIDE;
     ScanBwdParams b{};
     b.f = ScanParams{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, nullptr, keep, lengths,
-                     nullptr, {}, nullptr, const_cast<float *>(saved), N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS};
+                     nullptr, {}, nullptr, const_cast<float *>(saved), N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS,
+                     1, L, nullptr, nullptr};
+    b.f.segments = scan_segments(N, H, L, E, G, true, &b.f.seg_len);
     b.go = go, b.gos = s3(gos), b.glast = glast;
     b.gu = gu, b.gus = s3(gus), b.gdelta = gdelta, b.gds = s3(gds), b.gz = z ? gz : nullptr, b.gzs = s3(z ? gzs : nullptr);
     b.gB = gB, b.gBs = s3(gBs), b.gC = gC, b.gCs = s3(gCs);
     b.gA = gA, b.gD = gD, b.gbias = gbias, b.gstate = gstate;
-    b.part_a = workspace;                                                   // [N, H*E, S + 2]
-    b.part_bc = workspace + scan_part_a_floats(N, H, E, S);
+    b.f.seg_decay = workspace;
+    b.f.seg_state = b.f.seg_decay + scan_segment_floats(N, H, E, S, b.f.segments);
+    b.part_a = b.f.seg_state + scan_segment_floats(N, H, E, S, b.f.segments);
+    b.part_bc = b.part_a + (int64_t)N * b.f.segments * scan_part_a_row((int64_t)H * E, S);
     return launch_scan_bwd(b, bf16, (hipStream_t)stream);
 }
 
@@ -541,10 +554,10 @@ int selective_scan_forward_f32(const float *u, const int64_t u_strides[3], const
                                const float *B, const int64_t b_strides[3], const float *C, const int64_t c_strides[3],
                                const float *A, const float *D, const float *delta_bias, const float *state,
                                const float *keep, const int *lengths, float *out, const int64_t out_strides[3],
-                               float *last, float *saved, int N, int H, int L, int E, int S, int G, unsigned flags,
+                               float *last, float *saved, float *workspace, int N, int H, int L, int E, int S, int G, unsigned flags,
                                void *stream) {
     return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
-        state, keep, lengths, out, out_strides, last, saved, N, H, L, E, S, G, flags, stream, false, false);
+        state, keep, lengths, out, out_strides, last, saved, workspace, N, H, L, E, S, G, flags, stream, false, false);
 }
 
 int selective_scan_forward_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
@@ -552,10 +565,10 @@ int selective_scan_forward_bf16(const uint16_t *u, const int64_t u_strides[3], c
                                 const uint16_t *B, const int64_t b_strides[3], const uint16_t *C,
                                 const int64_t c_strides[3], const float *A, const float *D, const float *delta_bias,
                                 const float *state, const float *keep, const int *lengths, uint16_t *out,
-                                const int64_t out_strides[3], float *last, float *saved, int N, int H, int L, int E,
+                                const int64_t out_strides[3], float *last, float *saved, float *workspace, int N, int H, int L, int E,
                                 int S, int G, unsigned flags, void *stream) {
     return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
-        state, keep, lengths, out, out_strides, last, saved, N, H, L, E, S, G, flags, stream, true, false);
+        state, keep, lengths, out, out_strides, last, saved, workspace, N, H, L, E, S, G, flags, stream, true, false);
 }
 
 int selective_scan_backward_f32(const float *u, const int64_t u_strides[3], const float *delta,
@@ -601,7 +614,7 @@ int selective_scan_step_f32(const float *u, const int64_t u_strides[3], const fl
                             float *out, const int64_t out_strides[3], int N, int H, int E, int S, int G,
                             unsigned flags, void *stream) {
     return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
-        nullptr, keep, nullptr, out, out_strides, state, nullptr, N, H, 1, E, S, G, flags, stream, false, true);
+        nullptr, keep, nullptr, out, out_strides, state, nullptr, nullptr, N, H, 1, E, S, G, flags, stream, false, true);
 }
 
 int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides[3], const uint16_t *delta,
@@ -611,7 +624,7 @@ int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides[3], cons
                              const float *keep, float *state, uint16_t *out, const int64_t out_strides[3], int N,
                              int H, int E, int S, int G, unsigned flags, void *stream) {
     return scan_forward(u, u_strides, delta, delta_strides, z, z_strides, B, b_strides, C, c_strides, A, D, delta_bias,
-        nullptr, keep, nullptr, out, out_strides, state, nullptr, N, H, 1, E, S, G, flags, stream, true, true);
+        nullptr, keep, nullptr, out, out_strides, state, nullptr, nullptr, N, H, 1, E, S, G, flags, stream, true, true);
 }
 
 int causal_conv_forward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
@@ -699,10 +712,14 @@ int residual_rms_norm_backward_bf16(const void *sum, const float *weight, const 
         flags, stream, true);
 }
 
-int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G) {
+int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G, int backward) {
     if (!floats) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
-    floats[0] = scan_part_a_floats(N, H, E, S) + scan_tiles(H, E, G) * N * G * L * 2 * S;
+    int len;
+    const int segments = scan_segments(N, H, L, E, G, backward != 0, &len);
+    floats[0] = 2 * scan_segment_floats(N, H, E, S, segments);
+    if (backward)
+        floats[0] += (int64_t)N * segments * scan_part_a_row((int64_t)H * E, S) + scan_tiles(H, E, G) * N * G * L * 2 * S;
     return SRWM_OK;
 }
 int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E, int W) {

@@ -166,6 +166,8 @@ struct ScanParams {
     float *saved;                        // [N, ceil(L/16), H*E, S] states before each block of 16 steps, or null
     int N, H, L, E, S, G;
     unsigned softplus;
+    int segments, seg_len;               // steps are cut into `segments` runs of seg_len (a multiple of 16)
+    float *seg_decay, *seg_state;        // [N, segments, H*E, S]: a run's product of decays and its result from zero
 };
 
 struct ScanBwdParams {
@@ -179,7 +181,7 @@ struct ScanBwdParams {
     Strided3 gBs, gCs;
     float *gA, *gD, *gbias, *gstate;     // gD, gbias, gstate may be null
     float *part_bc;                      // [tiles of a group, N, G, L, 2, S]
-    float *part_a;                       // [N, scan_part_a_row]: gA [H*E, S], gD [H*E], gbias [H*E]
+    float *part_a;                       // [N * segments, scan_part_a_row]: gA [H*E, S], gD [H*E], gbias [H*E]
 };
 
 // Short causal convolution (causal_conv.hip)
@@ -318,6 +320,8 @@ int launch_delta_bwd_generic(const DeltaBwdParams &p, hipStream_t s);
 constexpr int kScanTile = 64;       // channels of a workgroup of the scan kernels
 // floats of a row of ScanBwdParams::part_a, a multiple of four so that every row can be written as float4
 inline __host__ __device__ int64_t scan_part_a_row(int64_t D, int S) { return (D * (S + 2) + 3) / 4 * 4; }
+// segments of the steps for a call (1: none) and their length, forward or backward
+int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len);
 int launch_scan_fwd(const ScanParams &p, bool bf16, hipStream_t s);
 int launch_scan_step(const ScanParams &p, bool bf16, hipStream_t s);   // u ... out: rows of one step; `last` is the state, in place
 int launch_scan_bwd(const ScanBwdParams &b, bool bf16, hipStream_t s);

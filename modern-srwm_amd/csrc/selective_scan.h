@@ -26,6 +26,8 @@ namespace fw {
 
 constexpr int kScanBlock = 16;      // steps between two saved states, and per stage of B and C in LDS
 constexpr int kScanThreads = 256;   // 4 waves
+constexpr int kScanWaves = 4096;        // a call is cut into segments until it has this many waves (4 on each SIMD)
+constexpr int kScanMinSegment = 64;     // shortest segment
 
 // From four values per lane to one: lane j of each quad ends up with the quad's sum of v[j].
 __device__ __forceinline__ float quad_sum_scatter(float v0, float v1, float v2, float v3, int lane) {
@@ -39,25 +41,102 @@ __device__ __forceinline__ float quad_lane(float v, int j) {
     return j == 0 ? quad_broadcast<0>(v) : j == 1 ? quad_broadcast<1>(v) : j == 2 ? quad_broadcast<2>(v) : quad_broadcast<3>(v);
 }
 
-// One lane's place: its channel, its states [q * SPL, q * SPL + SPL), and where they live.
+// A workgroup's place in the grid: x = batch row and tile of 64 channels, y = group, z = segment of the steps.
+// One lane's place in it: its channel and its states [q * SPL, q * SPL + SPL).
 struct ScanLane {
-    int h, e, d;        // head, channel of the head, channel of the tensor [H*E]
+    int n, tile, g, h0;   // of the workgroup; h0: head of its first channel
+    int h, e, d;          // head, channel of the head, channel of the tensor [H*E]
     int q, lane, wave;
-    bool on;            // false: a lane behind the group's last channel (reads the last one, writes nothing)
+    bool on;              // false: a lane behind the group's last channel (reads the last one, writes nothing)
 };
-__device__ __forceinline__ ScanLane scan_lane(int H, int E, int G, int tile, int g) {
+__device__ __forceinline__ ScanLane scan_lane(const ScanParams &p) {
     ScanLane r;
+    r.n = blockIdx.x % p.N, r.tile = blockIdx.x / p.N, r.g = blockIdx.y;
     r.lane = threadIdx.x & 63;
     r.wave = threadIdx.x >> 6;
     r.q = r.lane & 3;
-    const int Dg = (H / G) * E;
-    int c = tile * kScanTile + r.wave * 16 + (r.lane >> 2);
+    const int Dg = (p.H / p.G) * p.E;
+    int c = r.tile * kScanTile + r.wave * 16 + (r.lane >> 2);
     r.on = c < Dg;
     c = r.on ? c : Dg - 1;
-    r.d = g * Dg + c;
-    r.h = r.d / E;
-    r.e = r.d % E;
+    r.d = r.g * Dg + c;
+    r.h = r.d / p.E;
+    r.e = r.d % p.E;
+    r.h0 = (r.g * Dg + r.tile * kScanTile) / p.E;
     return r;
+}
+__device__ __forceinline__ int row_length(const ScanParams &p, int n) {
+    return p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
+}
+
+// Elements (t, channel) of a strided [N,H,L,E] tensor as one address per workgroup and step (scalar registers) plus one
+// offset per lane that never changes: a load is then one instruction without address arithmetic in the vector unit.
+// OFF: unsigned 32-bit byte offsets, or int64_t where a workgroup's channels and 16 steps span 2 GiB or more.
+template <typename T, typename OFF>
+struct ScanRows {
+    char *base;     // element (n, h0, t, 0) of the block's first step t; uniform
+    int64_t step;   // bytes between two steps; uniform
+    OFF off;        // of this lane's channel
+    __device__ __forceinline__ ScanRows(const void *p, const Strided3 &s, const ScanLane &w, int t)
+        : base((char *)p + (w.n * s.n + w.h0 * s.h + t * s.l) * (int64_t)sizeof(T)), step(s.l * (int64_t)sizeof(T)),
+          off((OFF)(((w.h - w.h0) * s.h + w.e) * (int64_t)sizeof(T))) {}
+    __device__ __forceinline__ void move(int steps) { base += steps * step; }
+    // the element of step 4i + k (i uniform; k >= 0: the lane's share)
+    __device__ __forceinline__ T *at(int i, int k) const { return (T *)(base + 4 * i * step + (OFF)(off + (OFF)(k * step))); }
+};
+
+// The elements of B and C that a thread stages in LDS: row r + R * k' of a block of 16, element s.
+template <typename T, int SPL>
+struct ScanBc {
+    static constexpr int SP = 4 * SPL, kRows = kScanThreads / SP;      // rows of B or C per pass of the workgroup
+    static constexpr int kEach = kRows >= kScanBlock ? 1 : kScanBlock / kRows;
+    static constexpr bool kSplit = kRows > kScanBlock;                 // half of the workgroup stages B, the other half C
+    const T *b, *c;
+    int64_t bs, cs;
+    int row, s;
+    bool pad;
+    __device__ __forceinline__ ScanBc(const ScanParams &p, const ScanLane &w, int t) {
+        const int i = threadIdx.x;
+        s = i % SP, row = i / SP % kScanBlock;
+        pad = s >= p.S;
+        const int sc = pad ? 0 : s;
+        b = (const T *)p.B + w.n * p.Bs.n + w.g * p.Bs.h + t * p.Bs.l + sc;
+        c = (const T *)p.C + w.n * p.Cs.n + w.g * p.Cs.h + t * p.Cs.l + sc;
+        bs = p.Bs.l, cs = p.Cs.l;
+        if (kSplit && i / SP >= kScanBlock) b = c, bs = cs;
+    }
+    __device__ __forceinline__ void move(int steps) { b += steps * bs, c += steps * cs; }
+    // n: steps from the block's first one to the sequence's end; rows behind it read the last one
+    __device__ __forceinline__ void fetch(T (&vb)[kEach], T (&vc)[kEach], int n, bool with_c) const {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int t = min(row + k * kRows, n - 1);
+            vb[k] = b[t * bs];
+            if (!kSplit && with_c) vc[k] = c[t * cs];
+        }
+    }
+    // dst: [2][16][SP]; rows behind the end are staged as zeros
+    __device__ __forceinline__ void stage(float *dst, const T (&vb)[kEach], const T (&vc)[kEach], int n, bool with_c) const {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const bool none = pad || row + k * kRows >= n;
+            const int i = threadIdx.x + k * kScanThreads;
+            dst[i] = none ? 0.f : (float)vb[k];
+            if (!kSplit && with_c) dst[kScanBlock * SP + i] = none ? 0.f : (float)vc[k];
+        }
+    }
+};
+
+// The product of decays of a segment with a reset in it: nothing of the state in front passes, not even NaN.  No power
+// of two has these bits.
+constexpr float kDropped = -0.f;
+__device__ __forceinline__ bool dropped(float pr) { return __float_as_uint(pr) == 0x80000000u; }
+
+// Whether a workgroup's lanes lie 2 GiB or more apart in rows of these strides (64 channels, 16 steps).
+inline bool scan_span(const ScanParams &p, const Strided3 &s, int64_t bytes) {
+    const auto mag = [](int64_t x) { return x < 0 ? -x : x; };
+    const int64_t heads = (kScanTile + p.E - 2) / p.E;   // heads that a tile reaches beyond its first
+    return (heads * mag(s.h) + kScanBlock * mag(s.l) + p.E) * bytes >= ((int64_t)1 << 31) || s.h < 0 || s.l < 0;
 }
 
 // SPL consecutive states of a row of S; those behind S read as zero and are not written

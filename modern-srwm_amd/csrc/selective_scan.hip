@@ -4,101 +4,182 @@
 namespace fw {
 namespace {
 
-// One workgroup carries 64 channels of one sequence through all its steps, 16 at a time.
-template <typename T, int SPL, bool KEEP>
+// Runs 64 channels of one sequence through one segment of its steps, 16 steps at a time.
+// LOCAL: from a zero state, for nothing but the segment's last state and its product of decays.  Otherwise the state
+// comes from the call's state and the segments in front of this one, and the outputs are formed.
+// The inputs of a block are fetched while the block before is computed.
+template <typename T, int SPL, bool KEEP, bool LOCAL, typename OFF>
 __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     constexpr int SP = 4 * SPL;
+    using Bc = ScanBc<T, SPL>;
     __shared__ float bc[2][2][kScanBlock][SP];   // [buffer][B | C][step][state]
-    const int n = blockIdx.x % p.N, tile = blockIdx.x / p.N, g = blockIdx.y;
-    const ScanLane w = scan_lane(p.H, p.E, p.G, tile, g);
-    const int S = p.S, D = p.H * p.E;
-    int Ln = p.L;
-    if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
+    const ScanLane w = scan_lane(p);
+    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
+    const int seg = blockIdx.z, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);
 
-    const T *u = (const T *)p.u + n * p.us.n + w.h * p.us.h + w.e;
-    const T *dl = (const T *)p.delta + n * p.ds.n + w.h * p.ds.h + w.e;
-    const T *z = p.z ? (const T *)p.z + n * p.zs.n + w.h * p.zs.h + w.e : nullptr;
-    T *out = (T *)p.out + n * p.os.n + w.h * p.os.h + w.e;
-    const T *Bp = (const T *)p.B + n * p.Bs.n + g * p.Bs.h;
-    const T *Cp = (const T *)p.C + n * p.Cs.n + g * p.Cs.h;
+    ScanRows<const T, OFF> u(p.u, p.us, w, tbeg), dl(p.delta, p.ds, w, tbeg), z(p.z, p.zs, w, tbeg);
+    ScanRows<T, OFF> out(p.out, p.os, w, tbeg);
+    Bc rows(p, w, tbeg);
+    const bool gate = !LOCAL && p.z != nullptr;
     const float bias = p.bias ? p.bias[w.d] : 0.f, Dc = p.D ? p.D[w.d] : 0.f;
+    const int64_t states = (int64_t)w.d * S;   // this channel's row in [H*E, S]
 
-    float A2[SPL], h[SPL];
-    load_states<SPL>(p.A + (int64_t)w.d * S, S, w.q, A2);
+    float A2[SPL], h[SPL], total = 0.f;
+    load_states<SPL>(p.A + states, S, w.q, A2);
 #pragma unroll
     for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, h[s] = 0.f;
-    if (p.state) load_states<SPL>(p.state + ((int64_t)n * D + w.d) * S, S, w.q, h);
+    bool alive = true;   // no reset in this segment so far
 
-    const int nblk = (Ln + kScanBlock - 1) / kScanBlock;
-    const int nsave = (p.L + kScanBlock - 1) / kScanBlock;
-    for (int blk = 0; blk < nblk; ++blk) {
-        const int t0 = blk * kScanBlock, buf = blk & 1;
-        for (int i = threadIdx.x; i < 2 * kScanBlock * SP; i += kScanThreads) {
-            const int s = i % SP, t = i / SP % kScanBlock, c = i / (SP * kScanBlock);
-            float v = 0.f;
-            if (s < S && t0 + t < Ln) v = c ? io_load(Cp + (t0 + t) * p.Cs.l + s) : io_load(Bp + (t0 + t) * p.Bs.l + s);
-            bc[buf][c][t][s] = v;
-        }
-        unsigned resets = 0;
-        if constexpr (KEEP) {
-            const int t = t0 + (w.lane & 15);
-            resets = (unsigned)__ballot(w.lane < 16 && t < Ln && is_reset(p.keep[(int64_t)n * p.L + min(t, p.L - 1)]));
-        }
-        __syncthreads();
-        if (p.saved && w.on)
-            store_states<SPL>(p.saved + (((int64_t)n * nsave + blk) * D + w.d) * S, S, w.q, h);
+    T ru[4], rd[4], rz[4], rb[Bc::kEach], rc[Bc::kEach];   // the next block as it lies in memory
+    float rk = 1.f;
+    // n: steps from the block's first one to the end (more than none); lanes behind it read the last one
+    auto fetch = [&](int t0, int n) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t t = t0 + 4 * i + w.q;
-            const bool in = t < Ln;
-            float uu = 0.f, dt = 0.f, zz = 0.f;
-            if (in) {
-                uu = io_load(u + t * p.us.l);
-                dt = io_load(dl + t * p.ds.l) + bias;
-                if (z) zz = io_load(z + t * p.zs.l);
-                float sig;
-                if (p.softplus) dt = softplus_sig(dt, sig);
-            }
-            const float du = dt * uu;
+            const bool full = n >= kScanBlock;
+            const int at = full ? i : 0, k = full ? w.q : min(4 * i + w.q, n - 1);
+            ru[i] = *u.at(at, k);
+            rd[i] = *dl.at(at, k);
+            if (gate) rz[i] = *z.at(at, k);
+        }
+        rows.fetch(rb, rc, n, !LOCAL);
+        if constexpr (KEEP) {
+            const int t = w.lane & 15;
+            rk = t < n ? p.keep[(int64_t)w.n * p.L + t0 + t] : 1.f;
+        }
+    };
+    if (tbeg < tend) fetch(tbeg, tend - tbeg);
+    if constexpr (!LOCAL) {
+        if (p.state) load_states<SPL>(p.state + w.n * (int64_t)D * S + states, S, w.q, h);
+        for (int k = 0; k < seg; ++k) {   // the segments in front, one after the other
+            const int64_t at = ((int64_t)w.n * p.segments + k) * D * S + states;
+            float pr[SPL], hl[SPL];
+            load_states<SPL>(p.seg_decay + at, S, w.q, pr);
+            load_states<SPL>(p.seg_state + at, S, w.q, hl);
+#pragma unroll
+            for (int s = 0; s < SPL; ++s) h[s] = dropped(pr[s]) ? hl[s] : fmaf(pr[s], h[s], hl[s]);
+        }
+    }
+    float *saved = nullptr;
+    if (!LOCAL && p.saved)
+        saved = p.saved + ((int64_t)w.n * ((p.L + kScanBlock - 1) / kScanBlock) + tbeg / kScanBlock) * D * S + states;
+
+    for (int t0 = tbeg, buf = 0; t0 < tend; t0 += kScanBlock, buf ^= 1) {
+        const int n = tend - t0;
+        float uu[4], dt[4], gg[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float sig;
+            uu[i] = (float)ru[i];
+            dt[i] = (float)rd[i] + bias;
+            if (p.softplus) dt[i] = softplus_sig(dt[i], sig);
+        }
+        if (n < kScanBlock) {   // behind the end: a decay of one, nothing added
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * i + w.q >= n) uu[i] = 0.f, dt[i] = 0.f;
+        }
+        if (gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gg[i] = (float)rz[i], gg[i] *= sigmoid(gg[i]);
+        }
+        rows.stage(&bc[buf][0][0][0], rb, rc, n, !LOCAL);
+        unsigned resets = 0;
+        if constexpr (KEEP) {
+            resets = (unsigned)__ballot(w.lane < 16 && is_reset(rk));
+            alive = alive && resets == 0;
+        }
+        __syncthreads();
+        if (n > kScanBlock) {
+            u.move(kScanBlock), dl.move(kScanBlock), z.move(kScanBlock), rows.move(kScanBlock);
+            fetch(t0 + kScanBlock, n - kScanBlock);
+        }
+        if (saved) {
+            if (w.on) store_states<SPL>(saved, S, w.q, h);
+            saved += (int64_t)D * S;
+        }
+        float o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float du = dt[i] * uu[i];
             float y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float dtj = quad_lane(dt, j), duj = quad_lane(du, j);
+                const float dtj = quad_lane(dt[i], j), duj = quad_lane(du, j);
                 const float *Bt = &bc[buf][0][4 * i + j][w.q * SPL], *Ct = &bc[buf][1][4 * i + j][w.q * SPL];
-                y[j] = 0.f;
                 const bool reset = KEEP && (resets >> (4 * i + j) & 1);
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
                     if constexpr (KEEP) h[s] = reset ? 0.f : h[s];
                     h[s] = fmaf(__builtin_amdgcn_exp2f(dtj * A2[s]), h[s], duj * Bt[s]);
-                    y[j] = fmaf(Ct[s], h[s], y[j]);
+                    if constexpr (!LOCAL) y[j] = s == 0 ? Ct[s] * h[s] : fmaf(Ct[s], h[s], y[j]);
                 }
             }
-            float o = quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane) + Dc * uu;
-            if (z) o *= zz * sigmoid(zz);
-            if (in && w.on) io_store(out + t * p.os.l, o);
+            if constexpr (LOCAL) total += dt[i];
+            else o[i] = fmaf(Dc, uu[i], quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane));
+        }
+        if constexpr (!LOCAL) {
+            if (gate) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] *= gg[i];
+            }
+            if (w.on) {
+                if (n >= kScanBlock) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) io_store(out.at(i, w.q), o[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * i + w.q < n) io_store(out.at(i, w.q), o[i]);
+                }
+            }
+            out.move(kScanBlock);
         }
     }
-    if (w.on) {
-        for (int64_t t = Ln + w.q; t < p.L; t += 4) io_store(out + t * p.os.l, 0.f);
-        store_states<SPL>(p.last + ((int64_t)n * D + w.d) * S, S, w.q, h);
+    if (!w.on) return;
+    if constexpr (LOCAL) {
+        total = group_sum<4>(total);
+        const int64_t at = ((int64_t)w.n * p.segments + seg) * D * S + states;
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) A2[s] = alive ? __builtin_amdgcn_exp2f(total * A2[s]) : kDropped;
+        store_states<SPL>(p.seg_decay + at, S, w.q, A2);
+        store_states<SPL>(p.seg_state + at, S, w.q, h);
+    } else {
+        // rows behind the sequence's end, and the last state from the last segment (those behind the end pass it on)
+        const int first = max(tbeg, Ln), behind = min(tbeg + p.seg_len, p.L);
+        ScanRows<T, OFF> rest(p.out, p.os, w, first);
+        for (int t = first; t < behind; t += 4, rest.move(4))
+            if (t + w.q < behind) io_store(rest.at(0, w.q), 0.f);
+        if (seg == p.segments - 1) store_states<SPL>(p.last + w.n * (int64_t)D * S + states, S, w.q, h);
     }
 }
 
+template <typename T, int SPL, typename OFF>
+int launch_fwd_as(const ScanParams &p, hipStream_t s) {
+    const unsigned tiles = (p.H / p.G * p.E + kScanTile - 1) / kScanTile;
+    const dim3 grid(tiles * p.N, p.G, p.segments), before(tiles * p.N, p.G, p.segments - 1);
+    if (p.segments > 1) {
+        if (p.keep) scan_fwd_kernel<T, SPL, true, true, OFF><<<before, kScanThreads, 0, s>>>(p);
+        else scan_fwd_kernel<T, SPL, false, true, OFF><<<before, kScanThreads, 0, s>>>(p);
+        const int r = (int)hipGetLastError();
+        if (r) return r;
+    }
+    if (p.keep) scan_fwd_kernel<T, SPL, true, false, OFF><<<grid, kScanThreads, 0, s>>>(p);
+    else scan_fwd_kernel<T, SPL, false, false, OFF><<<grid, kScanThreads, 0, s>>>(p);
+    return (int)hipGetLastError();
+}
 template <typename T, int SPL>
 int launch_fwd(const ScanParams &p, hipStream_t s) {
-    const int Dg = p.H / p.G * p.E;
-    const dim3 grid((Dg + kScanTile - 1) / kScanTile * p.N, p.G);
-    if (p.keep) scan_fwd_kernel<T, SPL, true><<<grid, kScanThreads, 0, s>>>(p);
-    else scan_fwd_kernel<T, SPL, false><<<grid, kScanThreads, 0, s>>>(p);
-    return (int)hipGetLastError();
+    const bool wide = scan_span(p, p.us, sizeof(T)) || scan_span(p, p.ds, sizeof(T)) || scan_span(p, p.zs, sizeof(T)) ||
+                      scan_span(p, p.os, sizeof(T));
+    return wide ? launch_fwd_as<T, SPL, int64_t>(p, s) : launch_fwd_as<T, SPL, uint32_t>(p, s);
 }
 
 // One token: every lane updates SPL states of a channel in place.
 template <typename T, int SPL>
 __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanParams p) {
-    const int n = blockIdx.x % p.N, tile = blockIdx.x / p.N, g = blockIdx.y;
-    const ScanLane w = scan_lane(p.H, p.E, p.G, tile, g);
+    const ScanLane w = scan_lane(p);
+    const int n = w.n, g = w.g;
     if (!w.on) return;
     const int S = p.S, D = p.H * p.E;
     const float uu = io_load((const T *)p.u + n * p.us.n + w.h * p.us.h + w.e);
@@ -144,6 +225,18 @@ int launch_step(const ScanParams &p, hipStream_t s) {
     if (p.S <= 16) return bf16 ? FN<__bf16, 4>(p, s) : FN<float, 4>(p, s);  \
     if (p.S <= 32) return bf16 ? FN<__bf16, 8>(p, s) : FN<float, 8>(p, s);  \
     return bf16 ? FN<__bf16, 16>(p, s) : FN<float, 16>(p, s);
+
+int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len) {
+    const int64_t waves = ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile * N * G * (kScanThreads / 64);
+    int64_t n = (kScanWaves + waves - 1) / waves;
+    const int64_t most = L / kScanMinSegment;
+    n = n < most ? n : most;
+    if (n < 2) n = 1;
+    int l = (int)((L + n - 1) / n);
+    l = (l + kScanBlock - 1) / kScanBlock * kScanBlock;
+    *len = l;
+    return (L + l - 1) / l;
+}
 
 int launch_scan_fwd(const ScanParams &p, bool bf16, hipStream_t s) { FW_BY_STATES(launch_fwd) }
 int launch_scan_step(const ScanParams &p, bool bf16, hipStream_t s) { FW_BY_STATES(launch_step) }

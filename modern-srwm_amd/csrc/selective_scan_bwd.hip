@@ -31,101 +31,215 @@ __device__ __forceinline__ void channels_sum_scatter(const float (&v)[R], float 
     for (int i = 0; i < R / 16; ++i) out[i] = (b2 ? c[i + R / 16] : c[i]) + xor4(b2 ? c[i] : c[i + R / 16]);
 }
 
-template <typename T, int SPL, bool KEEP>
+// Runs the state's gradient backwards through one segment from a zero gradient behind it, for nothing but the gradient
+// in front of the segment and its product of decays.
+template <typename T, int SPL, bool KEEP, typename OFF>
+__global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdParams b) {
+    constexpr int SP = 4 * SPL;
+    using Bc = ScanBc<T, SPL>;
+    __shared__ float bc[2][2][kScanBlock][SP];
+    const ScanParams &p = b.f;
+    const ScanLane w = scan_lane(p);
+    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
+    const int seg = blockIdx.z + 1, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);   // the first is never needed
+    const int64_t states = (int64_t)w.d * S;
+    const int last = tbeg + max(tend - tbeg - 1, 0) / kScanBlock * kScanBlock;   // first step of the last block
+    ScanRows<const T, OFF> dl(p.delta, p.ds, w, last), z(p.z, p.zs, w, last), go(b.go, b.gos, w, last);
+    Bc rows(p, w, last);
+    const bool gate = p.z != nullptr;
+    const float bias = p.bias ? p.bias[w.d] : 0.f;
+    float A2[SPL], gh[SPL], total = 0.f;
+    load_states<SPL>(p.A + states, S, w.q, A2);
+#pragma unroll
+    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, gh[s] = 0.f;
+    bool alive = true;
+
+    T rd[4], rz[4], rg[4], rb[Bc::kEach], rc[Bc::kEach];
+    float rk = 1.f;
+    auto fetch = [&](int t0, int n) {
+        const bool full = n >= kScanBlock;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = full ? i : 0, k = full ? w.q : min(4 * i + w.q, n - 1);
+            rd[i] = *dl.at(at, k);
+            rg[i] = *go.at(at, k);
+            if (gate) rz[i] = *z.at(at, k);
+        }
+        rows.fetch(rb, rc, n, true);
+        if constexpr (KEEP) {
+            const int t = w.lane & 15;
+            rk = t < n ? p.keep[(int64_t)w.n * p.L + t0 + t] : 1.f;
+        }
+    };
+    if (tbeg < tend) fetch(last, tend - last);
+    for (int t0 = last, buf = 0; t0 >= tbeg && tbeg < tend; t0 -= kScanBlock, buf ^= 1) {
+        const int n = tend - t0;
+        float dt[4], gy[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float sig;
+            dt[i] = (float)rd[i] + bias;
+            if (p.softplus) dt[i] = softplus_sig(dt[i], sig);
+            gy[i] = (float)rg[i];
+        }
+        if (gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float zz = (float)rz[i];
+                gy[i] *= zz * sigmoid(zz);
+            }
+        }
+        if (n < kScanBlock) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * i + w.q >= n) dt[i] = 0.f, gy[i] = 0.f;
+        }
+        rows.stage(&bc[buf][0][0][0], rb, rc, n, true);
+        unsigned resets = 0;
+        if constexpr (KEEP) {
+            resets = (unsigned)__ballot(w.lane < 16 && is_reset(rk));
+            alive = alive && resets == 0;
+        }
+        __syncthreads();
+        if (t0 > tbeg) {
+            dl.move(-kScanBlock), z.move(-kScanBlock), go.move(-kScanBlock), rows.move(-kScanBlock);
+            fetch(t0 - kScanBlock, kScanBlock);
+        }
+#pragma unroll
+        for (int t = kScanBlock - 1; t >= 0; --t) {
+            const int i = t / 4, j = t % 4;
+            const float dtj = quad_lane(dt[i], j), gyj = quad_lane(gy[i], j);
+            const bool reset = KEEP && (resets >> t & 1);
+#pragma unroll
+            for (int s = 0; s < SPL; ++s) {
+                gh[s] = fmaf(bc[buf][1][t][w.q * SPL + s], gyj, gh[s]) * __builtin_amdgcn_exp2f(dtj * A2[s]);
+                if constexpr (KEEP) gh[s] = reset ? 0.f : gh[s];
+            }
+        }
+        total += (dt[0] + dt[1]) + (dt[2] + dt[3]);
+    }
+    if (!w.on) return;
+    total = group_sum<4>(total);
+    const int64_t at = ((int64_t)w.n * p.segments + seg) * D * S + states;
+#pragma unroll
+    for (int s = 0; s < SPL; ++s) A2[s] = alive ? __builtin_amdgcn_exp2f(total * A2[s]) : kDropped;
+    store_states<SPL>(p.seg_decay + at, S, w.q, A2);
+    store_states<SPL>(p.seg_state + at, S, w.q, gh);
+}
+
+// Runs 64 channels of one sequence backwards through one segment of its steps, 16 at a time: the states of a block are
+// formed again from the saved one in front of it and held in registers with their decays, then the block is walked back.
+template <typename T, int SPL, bool KEEP, typename OFF>
 __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b) {
     constexpr int SP = 4 * SPL;
-    constexpr int TS = SPL <= 4 ? 16 : 64 / SPL;       // steps whose states are held in registers at once
+    constexpr int TS = SPL <= 4 ? 16 : 64 / SPL;       // steps whose states are held at once
     constexpr int TG = SPL >= 8 ? 1 : 8 / SPL;         // steps whose sums over channels travel together
     constexpr int R = 2 * SPL * TG;
+    using Bc = ScanBc<T, SPL>;
     __shared__ float bc[2][kScanBlock][SP];
     __shared__ float red[4][kScanBlock][2][SP];
     const ScanParams &p = b.f;
-    const int n = blockIdx.x % p.N, tile = blockIdx.x / p.N, g = blockIdx.y;
-    const ScanLane w = scan_lane(p.H, p.E, p.G, tile, g);
-    const int S = p.S, D = p.H * p.E;
-    int Ln = p.L;
-    if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
+    const ScanLane w = scan_lane(p);
+    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
+    const int seg = blockIdx.z, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);
+    const int64_t states = (int64_t)w.d * S;
+    const int last = tbeg + max(tend - tbeg - 1, 0) / kScanBlock * kScanBlock;   // first step of the last block
 
-    const T *u = (const T *)p.u + n * p.us.n + w.h * p.us.h + w.e;
-    const T *dl = (const T *)p.delta + n * p.ds.n + w.h * p.ds.h + w.e;
-    const T *z = p.z ? (const T *)p.z + n * p.zs.n + w.h * p.zs.h + w.e : nullptr;
-    const T *go = (const T *)b.go + n * b.gos.n + w.h * b.gos.h + w.e;
-    T *gu = (T *)b.gu + n * b.gus.n + w.h * b.gus.h + w.e;
-    T *gd = (T *)b.gdelta + n * b.gds.n + w.h * b.gds.h + w.e;
-    T *gz = z ? (T *)b.gz + n * b.gzs.n + w.h * b.gzs.h + w.e : nullptr;
-    const T *Bp = (const T *)p.B + n * p.Bs.n + g * p.Bs.h;
-    const T *Cp = (const T *)p.C + n * p.Cs.n + g * p.Cs.h;
+    ScanRows<const T, OFF> u(p.u, p.us, w, last), dl(p.delta, p.ds, w, last), z(p.z, p.zs, w, last), go(b.go, b.gos, w, last);
+    ScanRows<T, OFF> gu(b.gu, b.gus, w, last), gd(b.gdelta, b.gds, w, last), gz(b.gz, b.gzs, w, last);
+    Bc rows(p, w, last);
+    const bool gate = p.z != nullptr;
     const float bias = p.bias ? p.bias[w.d] : 0.f, Dc = p.D ? p.D[w.d] : 0.f;
+    const float *saved = p.saved + ((int64_t)w.n * ((p.L + kScanBlock - 1) / kScanBlock) + last / kScanBlock) * D * S + states;
+    float *part = b.part_bc + (((int64_t)w.tile * p.N + w.n) * p.G + w.g) * p.L * 2 * S;
 
     float A2[SPL], gh[SPL], gA[SPL];
-    load_states<SPL>(p.A + (int64_t)w.d * S, S, w.q, A2);
+    load_states<SPL>(p.A + states, S, w.q, A2);
 #pragma unroll
     for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, gh[s] = 0.f, gA[s] = 0.f;
-    if (b.glast) load_states<SPL>(b.glast + ((int64_t)n * D + w.d) * S, S, w.q, gh);
     float gDsum = 0.f, gbsum = 0.f;
 
-    if (w.on)
-        for (int64_t t = Ln + w.q; t < p.L; t += 4) {
-            io_store(gu + t * b.gus.l, 0.f);
-            io_store(gd + t * b.gds.l, 0.f);
-            if (z) io_store(gz + t * b.gzs.l, 0.f);
-        }
-
-    const int nblk = (Ln + kScanBlock - 1) / kScanBlock, nsave = (p.L + kScanBlock - 1) / kScanBlock;
-    float *part = b.part_bc + (((int64_t)tile * p.N + n) * p.G + g) * p.L * 2 * S;
-    for (int blk = nblk - 1; blk >= 0; --blk) {
-        const int t0 = blk * kScanBlock;
-        for (int i = threadIdx.x; i < 2 * kScanBlock * SP; i += kScanThreads) {
-            const int s = i % SP, t = i / SP % kScanBlock, c = i / (SP * kScanBlock);
-            float v = 0.f;
-            if (s < S && t0 + t < Ln) v = c ? io_load(Cp + (t0 + t) * p.Cs.l + s) : io_load(Bp + (t0 + t) * p.Bs.l + s);
-            bc[c][t][s] = v;
-        }
-        unsigned resets = 0;
-        if constexpr (KEEP) {
-            const int t = t0 + (w.lane & 15);
-            resets = (unsigned)__ballot(w.lane < 16 && t < Ln && is_reset(p.keep[(int64_t)n * p.L + min(t, p.L - 1)]));
-        }
-        __syncthreads();
-
-        // what a channel needs once per step: lane q holds the steps 4i + q
-        float uu[4], dt[4], du[4], sg[4], gg[4], zz[4], gy[4];
+    T ru[4], rd[4], rz[4], rg[4], rb[Bc::kEach], rc[Bc::kEach];   // the next block as it lies in memory
+    float rk = 1.f, h0[SPL];
+    auto fetch = [&](int t0, int n) {
+        const bool full = n >= kScanBlock;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int64_t t = t0 + 4 * i + w.q;
-            uu[i] = dt[i] = sg[i] = gg[i] = zz[i] = 0.f;
-            if (t < Ln) {
-                uu[i] = io_load(u + t * p.us.l);
-                gg[i] = w.on ? io_load(go + t * b.gos.l) : 0.f;   // a lane without a channel adds nothing to gB and gC
-                dt[i] = io_load(dl + t * p.ds.l) + bias;
-                if (z) zz[i] = io_load(z + t * p.zs.l);
-                sg[i] = 1.f;
-                if (p.softplus) dt[i] = softplus_sig(dt[i], sg[i]);
+            const int at = full ? i : 0, k = full ? w.q : min(4 * i + w.q, n - 1);
+            ru[i] = *u.at(at, k);
+            rd[i] = *dl.at(at, k);
+            rg[i] = *go.at(at, k);
+            if (gate) rz[i] = *z.at(at, k);
+        }
+        rows.fetch(rb, rc, n, true);
+        load_states<SPL>(saved, S, w.q, h0);
+        if constexpr (KEEP) {
+            const int t = w.lane & 15;
+            rk = t < n ? p.keep[(int64_t)w.n * p.L + t0 + t] : 1.f;
+        }
+    };
+    if (tbeg < tend) fetch(last, tend - last);
+    if (b.glast) load_states<SPL>(b.glast + w.n * (int64_t)D * S + states, S, w.q, gh);
+    for (int k = p.segments - 1; k > seg; --k) {   // the segments behind, one after the other
+        const int64_t at = ((int64_t)w.n * p.segments + k) * D * S + states;
+        float pr[SPL], gl[SPL];
+        load_states<SPL>(p.seg_decay + at, S, w.q, pr);
+        load_states<SPL>(p.seg_state + at, S, w.q, gl);
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) gh[s] = dropped(pr[s]) ? gl[s] : fmaf(pr[s], gh[s], gl[s]);
+    }
+    for (int t0 = last; t0 >= tbeg && tbeg < tend; t0 -= kScanBlock) {
+        const int n = tend - t0;   // steps of this block, 16 or more: all
+        // what a channel needs once per step: lane q holds the steps 4i + q
+        float uu[4], dt[4], sg[4], gy[4], gg[4], zz[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uu[i] = (float)ru[i];
+            dt[i] = (float)rd[i] + bias;
+            sg[i] = 1.f;
+            if (p.softplus) dt[i] = softplus_sig(dt[i], sg[i]);
+            gg[i] = w.on ? (float)rg[i] : 0.f;   // a lane without a channel adds nothing to gB and gC
+            zz[i] = gate ? (float)rz[i] : 0.f;
+        }
+        if (n < kScanBlock) {   // behind the end: a decay of one, nothing added, no gradient
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * i + w.q >= n) uu[i] = 0.f, dt[i] = 0.f, sg[i] = 0.f, gg[i] = 0.f, zz[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            gy[i] = gg[i];
+            if (gate) {   // gz = g y silu'(z): the factor of y takes the place of g
+                const float q = sigmoid(zz[i]);
+                gy[i] *= zz[i] * q;
+                gg[i] *= q * fmaf(zz[i], 1.f - q, 1.f);
             }
-            du[i] = dt[i] * uu[i];
-            gy[i] = z ? gg[i] * zz[i] * sigmoid(zz[i]) : gg[i];
             gDsum = fmaf(gy[i], uu[i], gDsum);
         }
+        rows.stage(&bc[0][0][0], rb, rc, n, true);
+        unsigned resets = 0;
+        if constexpr (KEEP) resets = (unsigned)__ballot(w.lane < 16 && is_reset(rk));
+        __syncthreads();
 
-        float h0[SPL];
-        load_states<SPL>(p.saved + (((int64_t)n * nsave + blk) * D + w.d) * S, S, w.q, h0);
+        float hb[SPL];   // the state in front of the block
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) hb[s] = h0[s];
 #pragma unroll
         for (int sub = kScanBlock / TS - 1; sub >= 0; --sub) {
             float h[SPL], a[TS][SPL], hs[TS + 1][SPL];
 #pragma unroll
-            for (int s = 0; s < SPL; ++s) h[s] = h0[s];
+            for (int s = 0; s < SPL; ++s) h[s] = hb[s];
             // forward again, keeping what the last TS steps need
             float y[4];
 #pragma unroll
             for (int t = 0; t < (sub + 1) * TS; ++t) {
                 const int i = t / 4, j = t % 4, k = t - sub * TS;
-                const float dtj = quad_lane(dt[i], j), duj = quad_lane(du[i], j);
+                const float dtj = quad_lane(dt[i], j), duj = quad_lane(dt[i] * uu[i], j);
                 const bool reset = KEEP && (resets >> t & 1);
                 if (k == 0) {
 #pragma unroll
                     for (int s = 0; s < SPL; ++s) hs[0][s] = h[s];
                 }
-                y[j] = 0.f;
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
                     float as = __builtin_amdgcn_exp2f(dtj * A2[s]);
@@ -134,15 +248,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
                     if (k >= 0) {
                         a[k < 0 ? 0 : k][s] = as;
                         hs[(k < 0 ? 0 : k) + 1][s] = h[s];
-                        y[j] = fmaf(bc[1][t][w.q * SPL + s], h[s], y[j]);
+                        const float c = bc[1][t][w.q * SPL + s];
+                        y[j] = s == 0 ? c * h[s] : fmaf(c, h[s], y[j]);
                     }
                 }
-                if (k >= 0 && j == 3 && z) {
-                    const float yy = quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane) + Dc * uu[i];
-                    const float q = sigmoid(zz[i]);
-                    const int64_t tt = t0 + 4 * i + w.q;
-                    if (tt < Ln && w.on) io_store(gz + tt * b.gzs.l, gg[i] * yy * q * (1.f + zz[i] * (1.f - q)));
+                if (k >= 0 && j == 3 && gate) {
+                    const float yy = fmaf(Dc, uu[i], quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane));
+                    if (4 * i + w.q < n && w.on) io_store(gz.at(i, w.q), gg[i] * yy);
                 }
+            }
+            if (sub == kScanBlock / TS - 1 && t0 > tbeg) {   // the next block's inputs come in while this one is walked back
+                u.move(-kScanBlock), dl.move(-kScanBlock), z.move(-kScanBlock), go.move(-kScanBlock), rows.move(-kScanBlock);
+                saved -= (int64_t)D * S;
+                fetch(t0 - kScanBlock, kScanBlock);
             }
             // and back
             float v[R];
@@ -150,29 +268,31 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
 #pragma unroll
             for (int k = TS - 1; k >= 0; --k) {
                 const int t = sub * TS + k, i = t / 4, j = t % 4;
-                const float dtj = quad_lane(dt[i], j), duj = quad_lane(du[i], j), gyj = quad_lane(gy[i], j);
+                const float dtj = quad_lane(dt[i], j), duj = quad_lane(dt[i] * uu[i], j), gyj = quad_lane(gy[i], j);
                 const bool reset = KEEP && (resets >> t & 1);
-                into[j] = ex[j] = 0.f;
                 const int o = (t % TG) * 2 * SPL;
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
+                    const float Bt = bc[0][t][w.q * SPL + s];
                     gh[s] = fmaf(bc[1][t][w.q * SPL + s], gyj, gh[s]);
-                    into[j] = fmaf(gh[s], bc[0][t][w.q * SPL + s], into[j]);
-                    v[o + s] = w.on ? gh[s] * duj : 0.f;
+                    into[j] = s == 0 ? gh[s] * Bt : fmaf(gh[s], Bt, into[j]);
+                    v[o + s] = gh[s] * duj;
                     v[o + SPL + s] = gyj * hs[k + 1][s];
                     const float ag = a[k][s] * gh[s];
                     const float before = KEEP && reset ? 0.f : hs[k][s];
                     const float e = ag * before;
-                    ex[j] = fmaf(e, A2[s], ex[j]);
+                    ex[j] = s == 0 ? e * A2[s] : fmaf(e, A2[s], ex[j]);
                     gA[s] = fmaf(e, dtj, gA[s]);
                     gh[s] = KEEP && reset ? 0.f : ag;
                 }
                 if (t % TG == 0) {
+                    if (!w.on) {
+#pragma unroll
+                        for (int x = 0; x < R; ++x) v[x] = 0.f;
+                    }
                     float r[R / 16];
                     channels_sum_scatter<R>(v, r, w.lane);
-                    const int first = (w.lane >> 2) % 16;
-                    // bits of the lane's place, most significant first: b5, b4, b3, b2
-                    const int at = ((first >> 3 & 1) * 8 + (first >> 2 & 1) * 4 + (first >> 1 & 1) * 2 + (first & 1)) * (R / 16);
+                    const int at = (w.lane >> 2) * (R / 16);
 #pragma unroll
                     for (int x = 0; x < R / 16; ++x) {
                         const int idx = at + x;
@@ -183,36 +303,45 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
                     const float in = quad_sum_scatter(into[0], into[1], into[2], into[3], w.lane);
                     const float xe = quad_sum_scatter(ex[0], ex[1], ex[2], ex[3], w.lane);
                     const float g1 = fmaf(xe, 0.693147180559945309f, in * uu[i]) * sg[i];
-                    const int64_t tt = t0 + 4 * i + w.q;
                     gbsum += g1;
-                    if (tt < Ln && w.on) {
-                        io_store(gu + tt * b.gus.l, fmaf(in, dt[i], Dc * gy[i]));
-                        io_store(gd + tt * b.gds.l, g1);
+                    if (4 * i + w.q < n && w.on) {
+                        io_store(gu.at(i, w.q), fmaf(in, dt[i], Dc * gy[i]));
+                        io_store(gd.at(i, w.q), g1);
                     }
                 }
             }
         }
+        gu.move(-kScanBlock), gd.move(-kScanBlock), gz.move(-kScanBlock);
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * kScanBlock * SP; i += kScanThreads) {
             const int s = i % SP, c = i / SP % 2, t = i / (2 * SP);
-            if (s < S && t0 + t < Ln)
+            if (s < S && t < n)
                 part[((int64_t)(t0 + t) * 2 + c) * S + s] = (red[0][t][c][s] + red[1][t][c][s]) + (red[2][t][c][s] + red[3][t][c][s]);
         }
     }
     gDsum = group_sum<4>(gDsum);
     gbsum = group_sum<4>(gbsum);
-    if (w.on) {
-        if (b.gstate) store_states<SPL>(b.gstate + ((int64_t)n * D + w.d) * S, S, w.q, gh);
-        float *pa = b.part_a + n * scan_part_a_row(D, S);
-        store_states<SPL>(pa + (int64_t)w.d * S, S, w.q, gA);
-        if (w.q == 0) {
-            pa[(int64_t)D * S + w.d] = gDsum;
-            pa[(int64_t)D * (S + 1) + w.d] = gbsum;
-        }
+    if (!w.on) return;
+    if (b.gstate && seg == 0) store_states<SPL>(b.gstate + w.n * (int64_t)D * S + states, S, w.q, gh);
+    float *pa = b.part_a + ((int64_t)w.n * p.segments + seg) * scan_part_a_row(D, S);
+    store_states<SPL>(pa + states, S, w.q, gA);
+    if (w.q == 0) {
+        pa[(int64_t)D * S + w.d] = gDsum;
+        pa[(int64_t)D * (S + 1) + w.d] = gbsum;
     }
+    // rows behind the sequence's end
+    const int first = max(tbeg, Ln), behind = min(tbeg + p.seg_len, p.L);
+    ScanRows<T, OFF> qu(b.gu, b.gus, w, first), qd(b.gdelta, b.gds, w, first), qz(b.gz, b.gzs, w, first);
+    for (int t = first; t < behind; t += 4, qu.move(4), qd.move(4), qz.move(4))
+        if (t + w.q < behind) {
+            io_store(qu.at(0, w.q), 0.f);
+            io_store(qd.at(0, w.q), 0.f);
+            if (gate) io_store(qz.at(0, w.q), 0.f);
+        }
 }
 
-// Joins the partial sums: those of gB and gC over the tiles of a group, those of gA, gD and gbias over the batch.
+// Joins the partial sums: those of gB and gC over the tiles of a group, those of gA, gD and gbias over batch and
+// segments.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bwd_join_kernel(ScanBwdParams b, int tiles, unsigned blocks_bc) {
     const ScanParams &p = b.f;
@@ -238,23 +367,36 @@ __global__ __launch_bounds__(256) void scan_bwd_join_kernel(ScanBwdParams b, int
                                                         : (b.gbias ? b.gbias + (i - D * (S + 1)) : nullptr);
     if (!dst) return;
     float v = 0.f;
-    for (int n = 0; n < p.N; ++n) v += b.part_a[n * row + i];
+    for (int n = 0; n < p.N * p.segments; ++n) v += b.part_a[n * row + i];
     *dst = v;
 }
 
+template <typename T, int SPL, typename OFF>
+int launch_bwd_as(const ScanBwdParams &b, hipStream_t s) {
+    const ScanParams &p = b.f;
+    const unsigned tiles = (p.H / p.G * p.E + kScanTile - 1) / kScanTile;
+    const dim3 grid(tiles * p.N, p.G, p.segments), behind(tiles * p.N, p.G, p.segments - 1);
+    int r = 0;
+    if (p.segments > 1) {
+        if (p.keep) scan_bwd_local_kernel<T, SPL, true, OFF><<<behind, kScanThreads, 0, s>>>(b);
+        else scan_bwd_local_kernel<T, SPL, false, OFF><<<behind, kScanThreads, 0, s>>>(b);
+        if ((r = (int)hipGetLastError())) return r;
+    }
+    if (p.keep) scan_bwd_kernel<T, SPL, true, OFF><<<grid, kScanThreads, 0, s>>>(b);
+    else scan_bwd_kernel<T, SPL, false, OFF><<<grid, kScanThreads, 0, s>>>(b);
+    if ((r = (int)hipGetLastError())) return r;
+    const int64_t nbc = ((int64_t)p.N * p.G * p.L * 2 * p.S + 255) / 256;
+    const int64_t na = ((int64_t)p.H * p.E * (p.S + 2) + 255) / 256;
+    scan_bwd_join_kernel<T><<<(unsigned)(nbc + na), 256, 0, s>>>(b, (int)tiles, (unsigned)nbc);
+    return (int)hipGetLastError();
+}
 template <typename T, int SPL>
 int launch_bwd(const ScanBwdParams &b, hipStream_t s) {
     const ScanParams &p = b.f;
-    const int Dg = p.H / p.G * p.E, tiles = (Dg + kScanTile - 1) / kScanTile;
-    const dim3 grid(tiles * p.N, p.G);
-    if (p.keep) scan_bwd_kernel<T, SPL, true><<<grid, kScanThreads, 0, s>>>(b);
-    else scan_bwd_kernel<T, SPL, false><<<grid, kScanThreads, 0, s>>>(b);
-    const int r = (int)hipGetLastError();
-    if (r) return r;
-    const int64_t nbc = ((int64_t)p.N * p.G * p.L * 2 * p.S + 255) / 256;
-    const int64_t na = ((int64_t)p.H * p.E * (p.S + 2) + 255) / 256;
-    scan_bwd_join_kernel<T><<<(unsigned)(nbc + na), 256, 0, s>>>(b, tiles, (unsigned)nbc);
-    return (int)hipGetLastError();
+    const bool wide = scan_span(p, p.us, sizeof(T)) || scan_span(p, p.ds, sizeof(T)) || scan_span(p, p.zs, sizeof(T)) ||
+                      scan_span(p, b.gos, sizeof(T)) || scan_span(p, b.gus, sizeof(T)) || scan_span(p, b.gds, sizeof(T)) ||
+                      scan_span(p, b.gzs, sizeof(T));
+    return wide ? launch_bwd_as<T, SPL, int64_t>(b, s) : launch_bwd_as<T, SPL, uint32_t>(b, s);
 }
 
 }  // namespace

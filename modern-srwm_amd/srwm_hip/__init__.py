@@ -14,6 +14,7 @@ PyTorch is used for device memory and streams only.  There is no CPU path: a mis
 library, a CPU tensor or a non-float32 tensor raises.
 """
 import ctypes
+import functools
 import os
 import subprocess
 
@@ -82,8 +83,8 @@ _SIGNATURES = {
     "delta_layer_prologue_grad_f32": [_F, _S] * 4 + [_F] * 5 + [_I] * 5 + [_U, ctypes.c_void_p],
     "delta_layer_prologue_bf16": [_F] * 6 + [_I] * 5 + [_U, ctypes.c_void_p],
     "delta_layer_prologue_grad_bf16": [_F, _S] * 4 + [_F] * 5 + [_I] * 5 + [_U, ctypes.c_void_p],
-    "selective_scan_forward_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_I] * 6 + [_U, ctypes.c_void_p],
-    "selective_scan_forward_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_forward_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 3 + [_I] * 6 + [_U, ctypes.c_void_p],
+    "selective_scan_forward_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 3 + [_I] * 6 + [_U, ctypes.c_void_p],
     "selective_scan_backward_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 5 + [_I] * 6 + [_U, ctypes.c_void_p],
     "selective_scan_backward_bf16": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 7 + [_S] + [_F] * 2 + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 5 + [_I] * 6 + [_U, ctypes.c_void_p],
     "selective_scan_step_f32": [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] + [_S] + [_F] * 6 + [_S] + [_I] * 5 + [_U, ctypes.c_void_p],
@@ -100,7 +101,7 @@ _SIGNATURES = {
     "residual_rms_norm_e4m3_bf16": [_F] * 7 + [_I] * 2 + [_U, ctypes.c_void_p],
     "residual_rms_norm_backward_f32": [_F] * 9 + [_I] * 2 + [_U, ctypes.c_void_p],
     "residual_rms_norm_backward_bf16": [_F] * 9 + [_I] * 2 + [_U, ctypes.c_void_p],
-    "selective_scan_workspace": [_S] + [_I] * 6,
+    "selective_scan_workspace": [_S] + [_I] * 7,
     "causal_conv_workspace": [_S] + [_I] * 5,
     "residual_rms_norm_workspace": [_S] + [_I] * 2,
 }
@@ -940,10 +941,17 @@ def rows_like(t):
     return out
 
 
-def _workspace(fn, device, *dims):
+@functools.lru_cache(maxsize=4096)
+def _workspace_floats(name, *dims):
     n = (ctypes.c_int64 * 1)()
-    _check(fn(n, *dims), fn.__name__)
-    return torch.empty(n[0], device=device, dtype=torch.float32)
+    _check(getattr(lib(), name)(n, *dims), name)
+    return n[0]
+
+
+def _workspace(name, device, *dims):
+    """What an entry point asks for at these sizes, or None."""
+    n = _workspace_floats(name, *dims)
+    return torch.empty(n, device=device, dtype=torch.float32) if n else None
 
 
 def _masks(keep, lengths, N, L, device):
@@ -986,11 +994,12 @@ def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, len
         out.zero_()
         last.zero_() if state is None else last.copy_(state)
         return out, last, saved
+    work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 0)
     fn = lib().selective_scan_forward_bf16 if io is torch.bfloat16 else lib().selective_scan_forward_f32
     with torch.cuda.device(dev):
         code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(state),
-                  _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]), _p(last), _p(saved), N, H, L, E, S, G,
-                  FLAG_SOFTPLUS if softplus else 0, _stream(dev))
+                  _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]), _p(last), _p(saved), _p(work), N, H, L, E,
+                  S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
     _check(code, fn.__name__)
     return out, last, saved
 
@@ -1027,7 +1036,7 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, 
             gstate.zero_() if glast is None else gstate.copy_(glast)
         return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
     fn = lib().selective_scan_backward_bf16 if io is torch.bfloat16 else lib().selective_scan_backward_f32
-    work = _workspace(lib().selective_scan_workspace, dev, N, H, L, E, S, G)
+    work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 1)
     st = lambda t: _I3(*t.stride()[:3])
     with torch.cuda.device(dev):
         code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(Dd), _p(bias), _p(keep),
@@ -1121,7 +1130,7 @@ def causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_l
             gstate.zero_() if glast is None else gstate.copy_(glast)
         return gx, gw, gb, gstate
     fn = lib().causal_conv_backward_bf16 if io is torch.bfloat16 else lib().causal_conv_backward_f32
-    work = _workspace(lib().causal_conv_workspace, dev, N, H, L, E, W)
+    work = _workspace("causal_conv_workspace", dev, N, H, L, E, W)
     with torch.cuda.device(dev):
         code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(gos), gostr, _p(glast), _p(gx),
                   _I3(*gx.stride()[:3]), _p(gw), _p(gb), _p(gstate), _p(work), N, H, L, E, W, FLAG_SILU if silu else 0,
@@ -1221,7 +1230,7 @@ def residual_rms_norm_backward(total, weight, rstd, grad_out, grad_total, with_r
     if not rows:
         return gx, gr, gw.zero_()
     fn = lib().residual_rms_norm_backward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_backward_f32
-    work = _workspace(lib().residual_rms_norm_workspace, dev, rows, D)
+    work = _workspace("residual_rms_norm_workspace", dev, rows, D)
     flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
     with torch.cuda.device(dev):
         code = fn(_p(total), _p(weight), _p(rstd), _p(go), _p(gt), _p(gx), _p(gr), _p(gw), _p(work), rows, D, flags,

@@ -22,7 +22,7 @@ def test_scan_argument_validation():
     def forward(u=fake(), us=ok, z=P(None), zs=None, A=fake(), os=ok, last=fake(), n=N, h=H, s=S, g=G, flags=0, fn=None):
         fn = fn or L.selective_scan_forward_f32
         return fn(u, us, fake(), ok, z, zs, fake(), okb, fake(), okb, A, fake(), fake(), fake(), P(None), P(None), fake(), os,
-                  last, P(None), n, h, T, E, s, g, flags, P(None))
+                  last, P(None), P(None), n, h, T, E, s, g, flags, P(None))
     for fn in (L.selective_scan_forward_f32, L.selective_scan_forward_bf16):
         assert forward(u=P(None), fn=fn) == -1
         assert forward(us=None, fn=fn) == -1
@@ -54,8 +54,8 @@ def test_scan_argument_validation():
                                                         P(None), P(None), P(None), state, fake(), ok, N, H, E, s, G, 0, P(None))
     assert step(P(None)) == -1 and step(P(0x1008)) == -3 and step(fake(), 65) == -2
     n = (ctypes.c_int64 * 1)()
-    assert L.selective_scan_workspace(n, N, H, T, E, S, G) == 0 and n[0] >= N * G * T * 2 * S
-    assert L.selective_scan_workspace(None, N, H, T, E, S, G) == -1 and L.selective_scan_workspace(n, N, H, T, E, 65, G) == -2
+    assert L.selective_scan_workspace(n, N, H, T, E, S, G, 1) == 0 and n[0] >= N * G * T * 2 * S
+    assert L.selective_scan_workspace(None, N, H, T, E, S, G, 1) == -1 and L.selective_scan_workspace(n, N, H, T, E, 65, G, 1) == -2
 
 
 def test_conv_and_norm_argument_validation():
