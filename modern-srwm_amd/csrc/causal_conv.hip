@@ -192,17 +192,27 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
     }
 }
 
+// Sums the runs' shares of gweight and gbias: 32 columns of one tap per workgroup, 8 threads over the runs of each.
 __global__ __launch_bounds__(256) void conv_join_kernel(const float *part, float *gweight, float *gbias, int64_t D, int W,
                                                         int parts) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= D * (W + 1)) return;
-    const int j = i / D;
-    const int64_t d = i % D;
+    __shared__ float sums[8][32];
+    const int c = threadIdx.x % 32, r = threadIdx.x / 32, j = blockIdx.y;
+    const int64_t d = (int64_t)blockIdx.x * 32 + c;
     if (j == W && !gbias) return;
     float v = 0.f;
-    for (int r = 0; r < parts; ++r) v += part[((int64_t)r * (W + 1) + j) * D + d];
-    if (j < W) gweight[d * W + j] = v;
-    else gbias[d] = v;
+    if (d < D) {
+#pragma unroll 8
+        for (int k = r; k < parts; k += 8) v += part[((int64_t)k * (W + 1) + j) * D + d];
+    }
+    sums[r][c] = v;
+    __syncthreads();
+    if (r == 0 && d < D) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += sums[k][c];
+        if (j < W) gweight[d * W + j] = v;
+        else gbias[d] = v;
+    }
 }
 
 template <typename T, int W, int V>
@@ -274,7 +284,7 @@ int bwd(const ConvBwdParams &b, hipStream_t s) {
     else conv_bwd_kernel<T, W, 1><<<grid(1), block, 0, s>>>(b, runs);
     const int r = (int)hipGetLastError();
     if (r) return r;
-    conv_join_kernel<<<(unsigned)((D * (W + 1) + 255) / 256), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);
+    conv_join_kernel<<<dim3((unsigned)((D + 31) / 32), W + 1), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);
     return (int)hipGetLastError();
 }
 template <typename T, int W>

@@ -210,12 +210,23 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormBwdParams p)
     }
 }
 
+// gweight[d] = sum of part[k][d]: 32 columns per workgroup, 8 threads over the rows of each, joined in a fixed order.
 __global__ __launch_bounds__(256) void norm_join_kernel(const float *part, float *gweight, int D, int blocks) {
-    const int d = blockIdx.x * 256 + threadIdx.x;
-    if (d >= D) return;
+    __shared__ float sums[8][32];
+    const int c = threadIdx.x % 32, r = threadIdx.x / 32, d = blockIdx.x * 32 + c;
     float v = 0.f;
-    for (int k = 0; k < blocks; ++k) v += part[(int64_t)k * D + d];
-    gweight[d] = v;
+    if (d < D) {
+#pragma unroll 8
+        for (int k = r; k < blocks; k += 8) v += part[(int64_t)k * D + d];
+    }
+    sums[r][c] = v;
+    __syncthreads();
+    if (r == 0 && d < D) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += sums[k][c];
+        gweight[d] = v;
+    }
 }
 
 template <typename TX, typename TR, int V, bool E4M3>
@@ -248,7 +259,7 @@ int bwd_by_size(const NormBwdParams &p, hipStream_t s) {
 #undef FW_NORM
     const int r = (int)hipGetLastError();
     if (r) return r;
-    norm_join_kernel<<<(unsigned)((p.D + 255) / 256), 256, 0, s>>>(p.part, p.gweight, p.D, p.blocks);
+    norm_join_kernel<<<(unsigned)((p.D + 31) / 32), 256, 0, s>>>(p.part, p.gweight, p.D, p.blocks);
     return (int)hipGetLastError();
 }
 

@@ -31,6 +31,9 @@ __device__ __forceinline__ void channels_sum_scatter(const float (&v)[R], float 
     for (int i = 0; i < R / 16; ++i) out[i] = (b2 ? c[i + R / 16] : c[i]) + xor4(b2 ? c[i] : c[i + R / 16]);
 }
 
+// v[i], i uniform: a constant after unrolling, else three selects
+__device__ __forceinline__ float pick4(const float (&v)[4], int i) { return i == 0 ? v[0] : i == 1 ? v[1] : i == 2 ? v[2] : v[3]; }
+
 // Runs the state's gradient backwards through one segment from a zero gradient behind it, for nothing but the gradient
 // in front of the segment and its product of decays.
 template <typename T, int SPL, bool KEEP, typename OFF>
@@ -130,9 +133,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
 // Runs 64 channels of one sequence backwards through one segment of its steps, 16 at a time: the states of a block are
 // formed again from the saved one in front of it and held in registers with their decays, then the block is walked back.
 template <typename T, int SPL, bool KEEP, typename OFF>
-__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b) {
+__global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kernel(ScanBwdParams b) {
     constexpr int SP = 4 * SPL;
     constexpr int TS = SPL <= 4 ? 16 : 64 / SPL;       // steps whose states are held at once
+    constexpr int kParts = kScanBlock / TS;
     constexpr int TG = SPL >= 8 ? 1 : 8 / SPL;         // steps whose sums over channels travel together
     constexpr int R = 2 * SPL * TG;
     using Bc = ScanBc<T, SPL>;
@@ -224,53 +228,72 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
         float hb[SPL];   // the state in front of the block
 #pragma unroll
         for (int s = 0; s < SPL; ++s) hb[s] = h0[s];
-#pragma unroll
-        for (int sub = kScanBlock / TS - 1; sub >= 0; --sub) {
+        // parts of TS steps, the last one first
+#pragma unroll 1
+        for (int sub = kParts - 1; sub >= 0; --sub) {
+            const int tsub = sub * TS;
             float h[SPL], a[TS][SPL], hs[TS + 1][SPL];
 #pragma unroll
             for (int s = 0; s < SPL; ++s) h[s] = hb[s];
-            // forward again, keeping what the last TS steps need
+            if constexpr (kParts > 1) {   // forward again up to the part
+#pragma unroll 1
+                for (int i = 0; i < sub * TS / 4; ++i) {
+                    const float d4 = pick4(dt, i), du4 = d4 * pick4(uu, i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float dtj = quad_lane(d4, j), duj = quad_lane(du4, j);
+                        const bool reset = KEEP && (resets >> (4 * i + j) & 1);
+#pragma unroll
+                        for (int s = 0; s < SPL; ++s) {
+                            if constexpr (KEEP) h[s] = reset ? 0.f : h[s];
+                            h[s] = fmaf(__builtin_amdgcn_exp2f(dtj * A2[s]), h[s], duj * bc[0][4 * i + j][w.q * SPL + s]);
+                        }
+                    }
+                }
+            }
+            // and through it, keeping its states and decays
             float y[4];
 #pragma unroll
-            for (int t = 0; t < (sub + 1) * TS; ++t) {
-                const int i = t / 4, j = t % 4, k = t - sub * TS;
-                const float dtj = quad_lane(dt[i], j), duj = quad_lane(dt[i] * uu[i], j);
-                const bool reset = KEEP && (resets >> t & 1);
-                if (k == 0) {
+            for (int s = 0; s < SPL; ++s) hs[0][s] = h[s];
 #pragma unroll
-                    for (int s = 0; s < SPL; ++s) hs[0][s] = h[s];
-                }
+            for (int k = 0; k < TS; ++k) {
+                const int t = tsub + k, i = k / 4, j = t % 4;
+                const float d4 = pick4(dt, tsub / 4 + i), u4 = pick4(uu, tsub / 4 + i);
+                const float dtj = quad_lane(d4, k % 4), duj = quad_lane(d4 * u4, k % 4);
+                const bool reset = KEEP && (resets >> t & 1);
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
                     float as = __builtin_amdgcn_exp2f(dtj * A2[s]);
                     if constexpr (KEEP) as = reset ? 0.f : as, h[s] = reset ? 0.f : h[s];
                     h[s] = fmaf(as, h[s], duj * bc[0][t][w.q * SPL + s]);
-                    if (k >= 0) {
-                        a[k < 0 ? 0 : k][s] = as;
-                        hs[(k < 0 ? 0 : k) + 1][s] = h[s];
-                        const float c = bc[1][t][w.q * SPL + s];
-                        y[j] = s == 0 ? c * h[s] : fmaf(c, h[s], y[j]);
-                    }
+                    a[k][s] = as;
+                    hs[k + 1][s] = h[s];
+                    const float c = bc[1][t][w.q * SPL + s];
+                    y[k % 4] = s == 0 ? c * h[s] : fmaf(c, h[s], y[k % 4]);
                 }
-                if (k >= 0 && j == 3 && gate) {
-                    const float yy = fmaf(Dc, uu[i], quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane));
-                    if (4 * i + w.q < n && w.on) io_store(gz.at(i, w.q), gg[i] * yy);
+                if (k % 4 == 3 && gate) {
+                    const float yy = fmaf(Dc, u4, quad_sum_scatter(y[0], y[1], y[2], y[3], w.lane));
+                    if (tsub + 4 * i + w.q < n && w.on) io_store(gz.at(tsub / 4 + i, w.q), pick4(gg, tsub / 4 + i) * yy);
                 }
             }
-            if (sub == kScanBlock / TS - 1 && t0 > tbeg) {   // the next block's inputs come in while this one is walked back
-                u.move(-kScanBlock), dl.move(-kScanBlock), z.move(-kScanBlock), go.move(-kScanBlock), rows.move(-kScanBlock);
-                saved -= (int64_t)D * S;
-                fetch(t0 - kScanBlock, kScanBlock);
-            }
+            if constexpr (KEEP) asm volatile("" : "+s"(resets));   // its bits are tested anew, not kept as 16 masks
             // and back
             float v[R];
             float into[4], ex[4];
 #pragma unroll
             for (int k = TS - 1; k >= 0; --k) {
-                const int t = sub * TS + k, i = t / 4, j = t % 4;
-                const float dtj = quad_lane(dt[i], j), duj = quad_lane(dt[i] * uu[i], j), gyj = quad_lane(gy[i], j);
+                // the next block's inputs come in while the second half of this one's first steps is walked back, when
+                // half of the registers of the states are free
+                if (k == TS / 2 - 1 && sub == 0 && t0 > tbeg) {
+                    u.move(-kScanBlock), dl.move(-kScanBlock), z.move(-kScanBlock), go.move(-kScanBlock), rows.move(-kScanBlock);
+                    saved -= (int64_t)D * S;
+                    fetch(t0 - kScanBlock, kScanBlock);
+                }
+                const int t = tsub + k, i = k / 4, j = k % 4;
+                const float d4 = pick4(dt, tsub / 4 + i), u4 = pick4(uu, tsub / 4 + i), g4 = pick4(gy, tsub / 4 + i);
+                const float dtj = quad_lane(d4, j), duj = quad_lane(d4 * u4, j), gyj = quad_lane(g4, j);
                 const bool reset = KEEP && (resets >> t & 1);
-                const int o = (t % TG) * 2 * SPL;
+                const int o = (k % TG) * 2 * SPL;
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
                     const float Bt = bc[0][t][w.q * SPL + s];
@@ -285,7 +308,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
                     gA[s] = fmaf(e, dtj, gA[s]);
                     gh[s] = KEEP && reset ? 0.f : ag;
                 }
-                if (t % TG == 0) {
+                if (k % TG == 0) {
                     if (!w.on) {
 #pragma unroll
                         for (int x = 0; x < R; ++x) v[x] = 0.f;
@@ -302,11 +325,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanBwdParams b)
                 if (j == 0) {
                     const float in = quad_sum_scatter(into[0], into[1], into[2], into[3], w.lane);
                     const float xe = quad_sum_scatter(ex[0], ex[1], ex[2], ex[3], w.lane);
-                    const float g1 = fmaf(xe, 0.693147180559945309f, in * uu[i]) * sg[i];
+                    const float g1 = fmaf(xe, 0.693147180559945309f, in * u4) * pick4(sg, tsub / 4 + i);
                     gbsum += g1;
-                    if (4 * i + w.q < n && w.on) {
-                        io_store(gu.at(i, w.q), fmaf(in, dt[i], Dc * gy[i]));
-                        io_store(gd.at(i, w.q), g1);
+                    if (tsub + 4 * i + w.q < n && w.on) {
+                        io_store(gu.at(tsub / 4 + i, w.q), fmaf(in, d4, Dc * g4));
+                        io_store(gd.at(tsub / 4 + i, w.q), g1);
                     }
                 }
             }

@@ -883,11 +883,21 @@ def _io_dtype(t, name):
     return t.dtype
 
 
+def _gpu(t, name):
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
+    return t.device
+
+
 def _on(t, name, shape, dtype, device):
-    """_require, and on the device of the call's other tensors."""
+    """_require, and on the device of the call's other tensors.  `device` is a GPU's (_gpu has seen to that).  The success path is three comparisons: single-token calls are bound by this side."""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.device == device:
+            return
+    except AttributeError:
+        pass
     _require(t, name, shape, dtype)
-    if t.device != device:
-        raise RuntimeError(f"{name} lives on {t.device}, the call's other tensors on {device}")
+    raise RuntimeError(f"{name} lives on {t.device}, the call's other tensors on {device}")
 
 
 def _rows_in(t, name, shape, dtype, device):
@@ -898,7 +908,7 @@ def _rows_in(t, name, shape, dtype, device):
     if st[-1] != 1 and shape[-1] != 1:
         t = t.contiguous()
         st = t.stride()
-    return t, _I3(st[0], st[1], st[2] if len(shape) == 4 else 0)
+    return t, _I3(st[0], st[1], st[2] if len(st) == 4 else 0)
 
 
 def _dense_in(t, name, shape, dtype, device):
@@ -908,25 +918,37 @@ def _dense_in(t, name, shape, dtype, device):
     _on(t, name, shape, dtype, device)
     if not t.is_contiguous():
         t = t.contiguous()
-    if t.data_ptr() % 16:
+    if t.data_ptr() & 15:
         t = t.clone()
     return t
 
 
-class _InPlace:
-    """A dense, 16-byte aligned stand-in for a tensor that a kernel overwrites; anything else is written back on exit."""
-
-    def __init__(self, t):
-        self.t = t
-        self.work = t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+class _Here:
+    """Stands for torch.cuda.device() where the tensors' device is the current one already (the context itself costs
+    more than a microsecond)."""
 
     def __enter__(self):
-        return self.work
+        return None
 
     def __exit__(self, *exc):
-        if self.work is not self.t and exc[0] is None:
-            self.t.copy_(self.work)
         return False
+
+
+_HERE_ALREADY = _Here()
+
+
+def _device(device):
+    return _HERE_ALREADY if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def _strides3(t):
+    a, b, c, _ = t.stride()
+    return _I3(a, b, c)
+
+
+def _overwritten(t):
+    """A tensor that a kernel overwrites: itself where it is dense and 16-byte aligned, else a copy to write back from."""
+    return t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _p(t):
@@ -976,7 +998,7 @@ def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, len
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{nm} must be a torch.Tensor")
     N, H, L, E, S, G = _scan_sizes(u, A, B)
-    dev = u.device
+    dev = _gpu(u, "u")
     us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
     ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
     zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
@@ -996,9 +1018,9 @@ def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, len
         return out, last, saved
     work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 0)
     fn = lib().selective_scan_forward_bf16 if io is torch.bfloat16 else lib().selective_scan_forward_f32
-    with torch.cuda.device(dev):
+    with _device(dev):
         code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(state),
-                  _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]), _p(last), _p(saved), _p(work), N, H, L, E,
+                  _p(keep), _p(lengths), _p(out), _strides3(out), _p(last), _p(saved), _p(work), N, H, L, E,
                   S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
     _check(code, fn.__name__)
     return out, last, saved
@@ -1010,7 +1032,7 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, 
     A, B, C, D, z, delta_bias and (with `with_state`) state; None for what was None."""
     io = _io_dtype(u, "u")
     N, H, L, E, S, G = _scan_sizes(u, A, B)
-    dev = u.device
+    dev = _gpu(u, "u")
     us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
     ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
     zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
@@ -1037,8 +1059,8 @@ def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, 
         return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
     fn = lib().selective_scan_backward_bf16 if io is torch.bfloat16 else lib().selective_scan_backward_f32
     work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 1)
-    st = lambda t: _I3(*t.stride()[:3])
-    with torch.cuda.device(dev):
+    st = _strides3
+    with _device(dev):
         code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(Dd), _p(bias), _p(keep),
                   _p(lengths), _p(saved), _p(gos), gostr, _p(glast), _p(gu), st(gu), _p(gdelta), st(gdelta), _p(gz),
                   None if gz is None else st(gz), _p(gB), st(gB), _p(gC), st(gC), _p(gA), _p(gD), _p(gbias), _p(gstate),
@@ -1056,7 +1078,7 @@ def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softpl
     G, S = B.shape[1], A.shape[-1]
     if G == 0 or H % G:
         raise ValueError(f"the {H} heads must divide into the {G} groups of B and C")
-    dev = u.device
+    dev = _gpu(u, "u")
     us, ustr = _rows_in(u, "u", (N, H, E), io, dev)
     ds, dstr = _rows_in(delta, "delta", (N, H, E), io, dev)
     zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, E), io, dev)
@@ -1067,14 +1089,17 @@ def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softpl
     bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
     keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
     _on(state, "state", (N, H, E, S), torch.float32, dev)
-    out = torch.empty((N, H, E), device=dev, dtype=io)
+    out = u.new_empty((N, H, E))
     if u.numel() == 0 or S == 0:
         return out.zero_()
     fn = lib().selective_scan_step_bf16 if io is torch.bfloat16 else lib().selective_scan_step_f32
-    with torch.cuda.device(dev), _InPlace(state) as h:
+    h = _overwritten(state)
+    with _device(dev):
         code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(keep),
                   _p(h), _p(out), _I3(H * E, E, 0), N, H, E, S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
     _check(code, fn.__name__)
+    if h is not state:
+        state.copy_(h)
     return out
 
 
@@ -1085,7 +1110,7 @@ def causal_conv_forward(x, weight, bias, state, keep, lengths, silu):
         raise ValueError("x must be (N, H, L, E), weight (H, E, W)")
     N, H, L, E = x.shape
     W = weight.shape[-1]
-    dev = x.device
+    dev = _gpu(x, "x")
     xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
     weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
     bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
@@ -1099,8 +1124,8 @@ def causal_conv_forward(x, weight, bias, state, keep, lengths, silu):
         last.zero_() if state is None else last.copy_(state)
         return out, last
     fn = lib().causal_conv_forward_bf16 if io is torch.bfloat16 else lib().causal_conv_forward_f32
-    with torch.cuda.device(dev):
-        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(out), _I3(*out.stride()[:3]),
+    with _device(dev):
+        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(out), _strides3(out),
                   _p(last), N, H, L, E, W, FLAG_SILU if silu else 0, _stream(dev))
     _check(code, fn.__name__)
     return out, last
@@ -1111,7 +1136,7 @@ def causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_l
     io = _io_dtype(x, "x")
     N, H, L, E = x.shape
     W = weight.shape[-1]
-    dev = x.device
+    dev = _gpu(x, "x")
     xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
     weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
     bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
@@ -1131,9 +1156,9 @@ def causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_l
         return gx, gw, gb, gstate
     fn = lib().causal_conv_backward_bf16 if io is torch.bfloat16 else lib().causal_conv_backward_f32
     work = _workspace("causal_conv_workspace", dev, N, H, L, E, W)
-    with torch.cuda.device(dev):
+    with _device(dev):
         code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(gos), gostr, _p(glast), _p(gx),
-                  _I3(*gx.stride()[:3]), _p(gw), _p(gb), _p(gstate), _p(work), N, H, L, E, W, FLAG_SILU if silu else 0,
+                  _strides3(gx), _p(gw), _p(gb), _p(gstate), _p(work), N, H, L, E, W, FLAG_SILU if silu else 0,
                   _stream(dev))
     _check(code, fn.__name__)
     return gx, gw, gb, gstate
@@ -1146,7 +1171,7 @@ def causal_conv_step(x, state, weight, bias, keep, silu):
         raise ValueError("x must be (N, H, E), weight (H, E, W)")
     N, H, E = x.shape
     W = weight.shape[-1]
-    dev = x.device
+    dev = _gpu(x, "x")
     xs, xstr = _rows_in(x, "x", (N, H, E), io, dev)
     weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
     bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
@@ -1154,14 +1179,17 @@ def causal_conv_step(x, state, weight, bias, keep, silu):
         raise ValueError(f"the convolution has 2 to 4 taps (got {W})")
     keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
     _on(state, "state", (N, H, W - 1, E), io, dev)
-    out = torch.empty((N, H, E), device=dev, dtype=io)
+    out = x.new_empty((N, H, E))
     if x.numel() == 0:
         return out
     fn = lib().causal_conv_step_bf16 if io is torch.bfloat16 else lib().causal_conv_step_f32
-    with torch.cuda.device(dev), _InPlace(state) as h:
+    h = _overwritten(state)
+    with _device(dev):
         code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(keep), _p(h), _p(out), _I3(H * E, E, 0), N, H, E, W,
                   FLAG_SILU if silu else 0, _stream(dev))
     _check(code, fn.__name__)
+    if h is not state:
+        state.copy_(h)
     return out
 
 
@@ -1169,14 +1197,14 @@ def _norm_rows(x, residual, weight):
     io = _io_dtype(x, "x")
     if x.dim() < 1:
         raise ValueError("x must have a last axis to normalise over")
-    D, dev = x.shape[-1], x.device
-    xs = _dense_in(x, "x", None, io, dev)
+    D, dev = x.shape[-1], _gpu(x, "x")
+    xs = _dense_in(x, "x", x.shape, io, dev)
     rdt = io
     if residual is not None:
         rdt = _io_dtype(residual, "residual")
         if io is torch.float32 and rdt is not torch.float32:
             raise TypeError("a float32 x takes a float32 residual")
-        residual = _dense_in(residual, "residual", tuple(x.shape), rdt, dev)
+        residual = _dense_in(residual, "residual", x.shape, rdt, dev)
     weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
     if D == 0:
         raise ValueError("the norm's rows are empty")
@@ -1193,7 +1221,7 @@ def residual_rms_norm_forward(x, residual, weight, eps, save):
     rstd = torch.empty(rows, device=dev, dtype=torch.float32) if save else None
     if rows:
         fn = lib().residual_rms_norm_forward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_forward_f32
-        with torch.cuda.device(dev):
+        with _device(dev):
             code = fn(_p(xs), _p(residual), _p(weight), _p(out), None if residual is None else _p(total), _p(rstd),
                       (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
         _check(code, fn.__name__)
@@ -1208,7 +1236,7 @@ def residual_rms_norm_e4m3(x, residual, weight, eps):
     total = xs if residual is None else torch.empty(x.shape, device=dev, dtype=rdt)
     if rows:
         fn = lib().residual_rms_norm_e4m3_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_e4m3_f32
-        with torch.cuda.device(dev):
+        with _device(dev):
             code = fn(_p(xs), _p(residual), _p(weight), _p(out), _p(scale), None if residual is None else _p(total),
                       (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
         _check(code, fn.__name__)
@@ -1218,11 +1246,11 @@ def residual_rms_norm_e4m3(x, residual, weight, eps):
 def residual_rms_norm_backward(total, weight, rstd, grad_out, grad_total, with_residual):
     """Gradients of residual_rms_norm_forward from the sum it returned: x (like grad_out), residual (like the sum; None
     without `with_residual`), weight.  grad_total may be None."""
-    io, rdt, D, dev = _io_dtype(grad_out, "grad_out"), _io_dtype(total, "total"), total.shape[-1], total.device
-    total = _dense_in(total, "total", None, rdt, dev)
+    io, rdt, D, dev = _io_dtype(grad_out, "grad_out"), _io_dtype(total, "total"), total.shape[-1], _gpu(total, "total")
+    total = _dense_in(total, "total", total.shape, rdt, dev)
     weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
-    go = _dense_in(grad_out, "grad_out", tuple(total.shape), io, dev)
-    gt = _dense_in(grad_total, "grad_total", tuple(total.shape), rdt, dev)
+    go = _dense_in(grad_out, "grad_out", total.shape, io, dev)
+    gt = _dense_in(grad_total, "grad_total", total.shape, rdt, dev)
     rows = total.numel() // D
     gx = torch.empty(total.shape, device=dev, dtype=io)
     gr = torch.empty(total.shape, device=dev, dtype=rdt) if with_residual else None
@@ -1232,7 +1260,7 @@ def residual_rms_norm_backward(total, weight, rstd, grad_out, grad_total, with_r
     fn = lib().residual_rms_norm_backward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_backward_f32
     work = _workspace("residual_rms_norm_workspace", dev, rows, D)
     flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
-    with torch.cuda.device(dev):
+    with _device(dev):
         code = fn(_p(total), _p(weight), _p(rstd), _p(go), _p(gt), _p(gx), _p(gr), _p(gw), _p(work), rows, D, flags,
                   _stream(dev))
     _check(code, fn.__name__)
