@@ -15,164 +15,212 @@ __device__ __forceinline__ void zero(float (&v)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.f;
 }
-
-// x at step t of a row: before the first step the carried rows (t = -1 the newest), zero without them.
-template <typename T, int W, int V>
-__device__ __forceinline__ void load_input(const T *x, int64_t stride, const T *state, int E, int64_t t, float (&v)[V]) {
-    if (t >= 0) load_vec<V>(x + t * stride, v);
-    else if (state) load_vec<V>(state + (W - 1 + t) * E, v);
-    else zero<V>(v);
+template <typename T, int V>
+__device__ __forceinline__ void widen(const Pack<T, V> &r, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)r.v[i];
 }
 
-template <typename T, int W, int V>
-__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs) {
-    const int64_t D = (int64_t)p.H * p.E;
-    const int64_t d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
-    const int n = blockIdx.x / runs;
-    const int64_t t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
-    if (d >= D || (t0 >= p.L && t0 > 0)) return;
-    const int h = d / p.E, e = d % p.E;
-    int Ln = p.L;
-    if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
-    const T *x = (const T *)p.x + n * p.xs.n + h * p.xs.h + e;
-    const T *state = p.state ? (const T *)p.state + ((int64_t)n * p.H + h) * (W - 1) * p.E + e : nullptr;
-    T *out = (T *)p.out + n * p.os.n + h * p.os.h + e;
-    const float *keep = p.keep ? p.keep + (int64_t)n * p.L : nullptr;
+// A thread's run: 16 steps of V channels of one sequence.
+struct ConvPlace {
+    int64_t d, t0;
+    int n, h, e, Ln;
+};
+template <int V>
+__device__ __forceinline__ ConvPlace conv_place(const ConvParams &p, int runs) {
+    ConvPlace c;
+    c.d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
+    c.n = blockIdx.x / runs;
+    c.t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
+    c.h = c.d / p.E, c.e = c.d % p.E;
+    c.Ln = p.lengths ? min(max(p.lengths[c.n], 0), p.L) : p.L;
+    return c;
+}
 
+// Rows t, t + 1, ... of a run as they lie in memory, all loads in flight at once.  Rows in front of the first step are
+// the carried ones (zeros without them), rows behind the sequence's end zeros.
+template <typename T, int W, int V, int R>
+__device__ __forceinline__ void load_rows(const T *x, int64_t stride, const T *state, int E, int64_t t, int Ln, Pack<T, V> (&r)[R]) {
+    if (t >= 0 && t + R <= Ln) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) r[j] = *reinterpret_cast<const Pack<T, V> *>(x + (t + j) * stride);
+    } else {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            r[j] = Pack<T, V>{};
+            if (t + j >= 0) {
+                if (t + j < Ln) r[j] = *reinterpret_cast<const Pack<T, V> *>(x + (t + j) * stride);
+            } else if (state && t + j >= -(W - 1)) {
+                r[j] = *reinterpret_cast<const Pack<T, V> *>(state + (W - 1 + t + j) * E);
+            }
+        }
+    }
+}
+// bit j: a reset in front of step t + j
+template <int R>
+__device__ __forceinline__ uint32_t load_resets(const float *keep, int64_t t, int Ln) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+        if (t + j >= 0 && t + j < Ln && is_reset(keep[t + j])) m |= 1u << j;
+    return m;
+}
+
+// Memory-bound: every input and output once, plus W - 1 rows of the run in front (from the caches).  All of a run's rows
+// are asked for before the first is used.
+template <typename T, int W, int V, bool KEEP>
+__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs) {
+    constexpr int R = kConvSteps + W - 1;
+    const ConvPlace c = conv_place<V>(p, runs);
+    if (c.d >= (int64_t)p.H * p.E || (c.t0 >= p.L && c.t0 > 0)) return;
+    const T *x = (const T *)p.x + c.n * p.xs.n + c.h * p.xs.h + c.e;
+    const int64_t srow = ((int64_t)c.n * p.H + c.h) * (W - 1) * p.E + c.e;
+    T *out = (T *)p.out + c.n * p.os.n + c.h * p.os.h + c.e + c.t0 * p.os.l;
+    const int Ln = c.Ln;
+
+    Pack<T, V> raw[R];
+    load_rows<T, W, V, R>(x, p.xs.l, p.state ? (const T *)p.state + srow : nullptr, p.E, c.t0 - (W - 1), Ln, raw);
+    uint32_t resets = 0;
+    if constexpr (KEEP) resets = load_resets<R>(p.keep + (int64_t)c.n * p.L, c.t0 - (W - 1), Ln);
     float w[W][V], bias[V], win[W][V];   // win: the last W inputs, the newest last
 #pragma unroll
     for (int i = 0; i < V; ++i) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[j][i] = p.weight[(d + i) * W + j];
-        bias[i] = p.bias ? p.bias[d + i] : 0.f;
+        for (int j = 0; j < W; ++j) w[j][i] = p.weight[(c.d + i) * W + j];
+        bias[i] = p.bias ? p.bias[c.d + i] : 0.f;
     }
+    // the row's last step is in this run (or the row is empty and this is its first run): it hands the carried rows on
+    const bool ends = Ln > 0 ? (c.t0 < Ln && Ln <= c.t0 + kConvSteps) : c.t0 == 0;
+    const int at_end = (int)(Ln - c.t0);
+    T *last = (T *)p.last + srow;
 #pragma unroll
     for (int j = 0; j < W; ++j) zero<V>(win[j]);
-    auto push = [&](int64_t t) {
-        const bool reset = keep && t >= 0 && is_reset(keep[t]);
+#pragma unroll
+    for (int k = 0; k <= R; ++k) {
+        // k rows are in the window, step t0 + k - W the newest of them
+        if (k >= W - 1 && ends && k - (W - 1) == at_end) {
+#pragma unroll
+            for (int j = 0; j + 1 < W; ++j) store_vec<V>(last + (int64_t)j * p.E, win[j + 1]);
+        }
+        if (k == R) break;
+        const bool reset = KEEP && (resets >> k & 1);
 #pragma unroll
         for (int j = 0; j + 1 < W; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) win[j][i] = reset ? 0.f : win[j + 1][i];
-        load_input<T, W, V>(x, p.xs.l, state, p.E, t, win[W - 1]);
-    };
-    const int64_t end = min(t0 + kConvSteps, (int64_t)Ln);
-    if (t0 < Ln || t0 == 0)
+        widen<T, V>(raw[k], win[W - 1]);
+        if (k >= W - 1) {
+            const int s = k - (W - 1);
+            float o[V];
 #pragma unroll
-        for (int j = 0; j + 1 < W; ++j) push(t0 - (W - 1) + j);
-    for (int64_t t = t0; t < end; ++t) {
-        push(t);
-        float o[V];
+            for (int i = 0; i < V; ++i) {
+                o[i] = bias[i];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            o[i] = bias[i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) o[i] = fmaf(w[j][i], win[j][i], o[i]);
-            if (p.silu) o[i] *= sigmoid(o[i]);
+                for (int j = 0; j < W; ++j) o[i] = fmaf(w[j][i], win[j][i], o[i]);
+                if (p.silu) o[i] *= sigmoid(o[i]);
+                if (s >= at_end) o[i] = 0.f;
+            }
+            if (c.t0 + s < p.L) store_vec<V>(out + s * p.os.l, o);
         }
-        store_vec<V>(out + t * p.os.l, o);
-    }
-    float none[V];
-    zero<V>(none);
-    for (int64_t t = max(t0, (int64_t)Ln); t < min(t0 + kConvSteps, (int64_t)p.L); ++t) store_vec<V>(out + t * p.os.l, none);
-    // the run with the row's last step hands the carried rows on
-    if (Ln > 0 ? (t0 < Ln && Ln <= t0 + kConvSteps) : t0 == 0) {
-        T *last = (T *)p.last + ((int64_t)n * p.H + h) * (W - 1) * p.E + e;
-#pragma unroll
-        for (int j = 0; j + 1 < W; ++j) store_vec<V>(last + (int64_t)j * p.E, win[j + 1]);
     }
 }
 
-// gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre); a run walks its steps and the W - 1 behind them, carrying the
+// gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre): a run walks its steps and the W - 1 behind them, carrying the
 // gradients of the last W inputs, each complete when the window leaves it.
-template <typename T, int W, int V>
+template <typename T, int W, int V, bool KEEP>
 __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs) {
+    constexpr int RX = kConvSteps + 2 * (W - 1), RG = kConvSteps + W - 1;
     const ConvParams &p = b.f;
     const int64_t D = (int64_t)p.H * p.E;
-    const int64_t d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
-    const int n = blockIdx.x / runs;
-    const int64_t t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
     __shared__ float red[kConvRuns][kConvLanes][V];
+    const ConvPlace c = conv_place<V>(p, runs);
     float gw[W + 1][V];
 #pragma unroll
     for (int j = 0; j <= W; ++j) zero<V>(gw[j]);
-    if (d < D && t0 < p.L) {
-        const int h = d / p.E, e = d % p.E;
-        int Ln = p.L;
-        if (p.lengths) Ln = min(max(p.lengths[n], 0), p.L);
-        const T *x = (const T *)p.x + n * p.xs.n + h * p.xs.h + e;
-        const T *go = (const T *)b.go + n * b.gos.n + h * b.gos.h + e;
-        T *gx = (T *)b.gx + n * b.gxs.n + h * b.gxs.h + e;
-        const int64_t srow = ((int64_t)n * p.H + h) * (W - 1) * p.E + e;
-        const T *state = p.state ? (const T *)p.state + srow : nullptr;
+    if (c.d < D && c.t0 < p.L) {
+        const int Ln = c.Ln;
+        const T *x = (const T *)p.x + c.n * p.xs.n + c.h * p.xs.h + c.e;
+        const T *go = (const T *)b.go + c.n * b.gos.n + c.h * b.gos.h + c.e;
+        T *gx = (T *)b.gx + c.n * b.gxs.n + c.h * b.gxs.h + c.e;
+        const int64_t srow = ((int64_t)c.n * p.H + c.h) * (W - 1) * p.E + c.e;
         const T *glast = b.glast ? (const T *)b.glast + srow : nullptr;
-        T *gstate = b.gstate ? (T *)b.gstate + srow : nullptr;
-        const float *keep = p.keep ? p.keep + (int64_t)n * p.L : nullptr;
+        T *gstate = b.gstate && c.t0 == 0 ? (T *)b.gstate + srow : nullptr;
 
+        Pack<T, V> rx[RX], rg[RG];
+        load_rows<T, W, V, RX>(x, p.xs.l, p.state ? (const T *)p.state + srow : nullptr, p.E, c.t0 - (W - 1), Ln, rx);
+        load_rows<T, W, V, RG>(go, b.gos.l, nullptr, p.E, c.t0, Ln, rg);
+        uint32_t resets = 0;
+        if constexpr (KEEP) resets = load_resets<RX>(p.keep + (int64_t)c.n * p.L, c.t0 - (W - 1), Ln);
         float w[W][V], bias[V], win[W][V], acc[W][V];   // acc[j]: gradient of the input j steps back
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) w[j][i] = p.weight[(d + i) * W + j];
-            bias[i] = p.bias ? p.bias[d + i] : 0.f;
+            for (int j = 0; j < W; ++j) w[j][i] = p.weight[(c.d + i) * W + j];
+            bias[i] = p.bias ? p.bias[c.d + i] : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < W; ++j) zero<V>(win[j]), zero<V>(acc[j]);
         int since = W;   // steps since the last reset, at most W
-        for (int64_t t = t0 - (W - 1); t < t0 + kConvSteps + W - 1; ++t) {
-            const bool reset = keep && t >= 0 && t < Ln && is_reset(keep[t]);
-            since = reset ? 0 : min(since + 1, W);
+#pragma unroll
+        for (int k = 0; k < RX; ++k) {
+            const int s = k - (W - 1);              // step t0 + s
+            const int64_t t = c.t0 + s;
+            const bool reset = KEEP && (resets >> k & 1);
+            if constexpr (KEEP) since = reset ? 0 : min(since + 1, W);
 #pragma unroll
             for (int j = 0; j + 1 < W; ++j)
 #pragma unroll
                 for (int i = 0; i < V; ++i) win[j][i] = reset ? 0.f : win[j + 1][i];
-            zero<V>(win[W - 1]);
-            if (t < Ln) load_input<T, W, V>(x, p.xs.l, state, p.E, t, win[W - 1]);
+            widen<T, V>(rx[k], win[W - 1]);
+            if (s < 0) continue;
 #pragma unroll
             for (int j = W - 1; j > 0; --j)
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[j][i] = acc[j - 1][i];
             zero<V>(acc[0]);
-            if (t >= t0 && t < Ln) {
-                float g[V];
-                load_vec<V>(go + t * b.gos.l, g);
-                if (p.silu) {
+            // rows behind the end are zeros in rg, so that nothing of them is added
+            float g[V];
+            widen<T, V>(rg[s < 0 ? 0 : s], g);
+            if (p.silu) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        float o = bias[i];
+                for (int i = 0; i < V; ++i) {
+                    float o = bias[i];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) o = fmaf(w[j][i], win[j][i], o);
-                        const float q = sigmoid(o);
-                        g[i] *= q * fmaf(o, 1.f - q, 1.f);
-                    }
+                    for (int j = 0; j < W; ++j) o = fmaf(w[j][i], win[j][i], o);
+                    const float q = sigmoid(o);
+                    g[i] *= q * fmaf(o, 1.f - q, 1.f);
+                    if (t >= Ln) g[i] = 0.f;
                 }
+            }
 #pragma unroll
-                for (int j = 0; j < W; ++j)
-                    if (j <= since)
+            for (int j = 0; j < W; ++j)
+                if (!KEEP || j <= since)
 #pragma unroll
-                        for (int i = 0; i < V; ++i) acc[j][i] = fmaf(w[W - 1 - j][i], g[i], acc[j][i]);
-                if (t < t0 + kConvSteps) {
+                    for (int i = 0; i < V; ++i) acc[j][i] = fmaf(w[W - 1 - j][i], g[i], acc[j][i]);
+            if (s < kConvSteps) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
+                for (int i = 0; i < V; ++i) {
 #pragma unroll
-                        for (int j = 0; j < W; ++j) gw[j][i] = fmaf(g[i], win[j][i], gw[j][i]);
-                        gw[W][i] += g[i];
-                    }
+                    for (int j = 0; j < W; ++j) gw[j][i] = fmaf(g[i], win[j][i], gw[j][i]);
+                    gw[W][i] += g[i];
                 }
-            } else if (t == Ln && glast) {
-                // one step behind the end: the carried rows are the inputs 1 .. W-1 steps back
+            }
+            if (t == Ln && glast) {   // one step behind the end: the carried rows are the inputs 1 .. W-1 steps back
 #pragma unroll
                 for (int j = 1; j < W; ++j)
-                    if (j <= since) {   // `since` already counts this step
-                        float g[V];
-                        load_vec<V>(glast + (int64_t)(W - 1 - j) * p.E, g);
+                    if (!KEEP || j <= since) {
+                        float gl[V];
+                        load_vec<V>(glast + (int64_t)(W - 1 - j) * p.E, gl);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) acc[j][i] += g[i];
+                        for (int i = 0; i < V; ++i) acc[j][i] += gl[i];
                     }
             }
-            const int64_t done = t - (W - 1);   // the input that leaves the window
-            if (done >= t0 && done < p.L) store_vec<V>(gx + done * b.gxs.l, acc[W - 1]);
-            if (done < 0 && t >= 0 && t0 == 0 && gstate) store_vec<V>(gstate + (W - 1 + done) * p.E, acc[W - 1]);
+            const int done = s - (W - 1);   // the input that leaves the window, t0 + done
+            if (done >= 0) {
+                if (c.t0 + done < p.L) store_vec<V>(gx + (c.t0 + done) * b.gxs.l, acc[W - 1]);
+            } else if (gstate) {
+                store_vec<V>(gstate + (int64_t)(W - 1 + done) * p.E, acc[W - 1]);
+            }
         }
     }
     float *part = b.part + (int64_t)blockIdx.x * (W + 1) * D;
@@ -266,8 +314,14 @@ int fwd(const ConvParams &p, hipStream_t s) {
     const dim3 block(kConvLanes, kConvRuns);
     const int runs = conv_runs(p.L);
     auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
-    if (conv_vec<T, V>(p)) conv_fwd_kernel<T, W, V><<<grid(V), block, 0, s>>>(p, runs);
-    else conv_fwd_kernel<T, W, 1><<<grid(1), block, 0, s>>>(p, runs);
+    const bool vec = conv_vec<T, V>(p);
+    if (p.keep) {
+        if (vec) conv_fwd_kernel<T, W, V, true><<<grid(V), block, 0, s>>>(p, runs);
+        else conv_fwd_kernel<T, W, 1, true><<<grid(1), block, 0, s>>>(p, runs);
+    } else {
+        if (vec) conv_fwd_kernel<T, W, V, false><<<grid(V), block, 0, s>>>(p, runs);
+        else conv_fwd_kernel<T, W, 1, false><<<grid(1), block, 0, s>>>(p, runs);
+    }
     return (int)hipGetLastError();
 }
 template <typename T, int W>
@@ -278,10 +332,15 @@ int bwd(const ConvBwdParams &b, hipStream_t s) {
     const dim3 block(kConvLanes, kConvRuns);
     const int runs = conv_runs(p.L);
     auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
-    if (p.E % V == 0 && rows_ok<T, V>(p.x, p.xs) && rows_ok<T, V>(b.go, b.gos) && rows_ok<T, V>(b.gx, b.gxs) &&
-        vec_ok(p.state, sizeof(T) * V) && vec_ok(b.glast, sizeof(T) * V) && vec_ok(b.gstate, sizeof(T) * V))
-        conv_bwd_kernel<T, W, V><<<grid(V), block, 0, s>>>(b, runs);
-    else conv_bwd_kernel<T, W, 1><<<grid(1), block, 0, s>>>(b, runs);
+    const bool vec = p.E % V == 0 && rows_ok<T, V>(p.x, p.xs) && rows_ok<T, V>(b.go, b.gos) && rows_ok<T, V>(b.gx, b.gxs) &&
+                     vec_ok(p.state, sizeof(T) * V) && vec_ok(b.glast, sizeof(T) * V) && vec_ok(b.gstate, sizeof(T) * V);
+    if (p.keep) {
+        if (vec) conv_bwd_kernel<T, W, V, true><<<grid(V), block, 0, s>>>(b, runs);
+        else conv_bwd_kernel<T, W, 1, true><<<grid(1), block, 0, s>>>(b, runs);
+    } else {
+        if (vec) conv_bwd_kernel<T, W, V, false><<<grid(V), block, 0, s>>>(b, runs);
+        else conv_bwd_kernel<T, W, 1, false><<<grid(1), block, 0, s>>>(b, runs);
+    }
     const int r = (int)hipGetLastError();
     if (r) return r;
     conv_join_kernel<<<dim3((unsigned)((D + 31) / 32), W + 1), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);

@@ -153,6 +153,16 @@ __device__ __forceinline__ void load_states(const float *row, int S, int q, floa
         for (int i = 0; i < SPL; ++i) v[i] = q * SPL + i < S ? row[q * SPL + i] : 0.f;
     }
 }
+// the same from a row of fp32 or bf16 elements that may start anywhere
+template <int SPL, typename T>
+__device__ __forceinline__ void load_io_states(const T *row, int S, int q, float (&v)[SPL]) {
+    if (S == 4 * SPL && ((uintptr_t)row & (sizeof(T) * SPL - 1)) == 0 && sizeof(T) * SPL <= 16) {
+        load_vec<SPL>(row + q * SPL, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < SPL; ++i) v[i] = q * SPL + i < S ? io_load(row + q * SPL + i) : 0.f;
+    }
+}
 template <int SPL>
 __device__ __forceinline__ void store_states(float *row, int S, int q, const float (&v)[SPL]) {
     if (S == 4 * SPL && SPL % 4 == 0) {

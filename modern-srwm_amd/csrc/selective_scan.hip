@@ -175,46 +175,61 @@ int launch_fwd(const ScanParams &p, hipStream_t s) {
     return wide ? launch_fwd_as<T, SPL, int64_t>(p, s) : launch_fwd_as<T, SPL, uint32_t>(p, s);
 }
 
-// One token: every lane updates SPL states of a channel in place.
-template <typename T, int SPL>
+// One token: a lane updates SPL states of a channel in place, for RN batch rows whose states are all asked for before the
+// first is used (A, D and the bias are read once for them).  Bound by the states' memory traffic for many rows, by
+// latency for few.
+template <typename T, int SPL, int RN>
 __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanParams p) {
-    const ScanLane w = scan_lane(p);
-    const int n = w.n, g = w.g;
+    ScanParams at = p;
+    at.N = (p.N + RN - 1) / RN;
+    const ScanLane w = scan_lane(at);
     if (!w.on) return;
-    const int S = p.S, D = p.H * p.E;
-    const float uu = io_load((const T *)p.u + n * p.us.n + w.h * p.us.h + w.e);
-    float dt = io_load((const T *)p.delta + n * p.ds.n + w.h * p.ds.h + w.e) + (p.bias ? p.bias[w.d] : 0.f), sig;
-    const T *Bp = (const T *)p.B + n * p.Bs.n + g * p.Bs.h, *Cp = (const T *)p.C + n * p.Cs.n + g * p.Cs.h;
-    if (p.softplus) dt = softplus_sig(dt, sig);
-    float *row = p.last + ((int64_t)n * D + w.d) * S;
-    float h[SPL], A[SPL];
-    load_states<SPL>(row, S, w.q, h);
-    load_states<SPL>(p.A + (int64_t)w.d * S, S, w.q, A);
-    const bool reset = p.keep && is_reset(p.keep[n]);
-    float y = 0.f;
+    const int S = p.S, n0 = w.n * RN;
+    const int64_t D = (int64_t)p.H * p.E, states = (int64_t)w.d * S;
+    float h[RN][SPL], A2[SPL], b[RN][SPL], c[RN][SPL], uu[RN], dt[RN], zz[RN];
+    bool reset[RN];
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) {
-        const int k = w.q * SPL + s;
-        const float b = k < S ? io_load(Bp + k) : 0.f, c = k < S ? io_load(Cp + k) : 0.f;
-        h[s] = fmaf(__builtin_amdgcn_exp2f(dt * (A[s] * kLog2e)), reset ? 0.f : h[s], dt * uu * b);
-        y = fmaf(c, h[s], y);
+    for (int r = 0; r < RN; ++r) {
+        const int n = min(n0 + r, p.N - 1);
+        load_states<SPL>(p.last + n * D * S + states, S, w.q, h[r]);
+        uu[r] = io_load((const T *)p.u + n * p.us.n + w.h * p.us.h + w.e);
+        dt[r] = io_load((const T *)p.delta + n * p.ds.n + w.h * p.ds.h + w.e);
+        zz[r] = p.z ? io_load((const T *)p.z + n * p.zs.n + w.h * p.zs.h + w.e) : 0.f;
+        load_io_states<SPL>((const T *)p.B + n * p.Bs.n + w.g * p.Bs.h, S, w.q, b[r]);
+        load_io_states<SPL>((const T *)p.C + n * p.Cs.n + w.g * p.Cs.h, S, w.q, c[r]);
+        reset[r] = p.keep && is_reset(p.keep[n]);
     }
-    store_states<SPL>(row, S, w.q, h);
-    y = group_sum<4>(y);
-    if (w.q == 0) {
-        y += (p.D ? p.D[w.d] : 0.f) * uu;
-        if (p.z) {
-            const float zz = io_load((const T *)p.z + n * p.zs.n + w.h * p.zs.h + w.e);
-            y *= zz * sigmoid(zz);
+    load_states<SPL>(p.A + states, S, w.q, A2);
+    const float bias = p.bias ? p.bias[w.d] : 0.f, Dc = p.D ? p.D[w.d] : 0.f;
+#pragma unroll
+    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e;
+#pragma unroll
+    for (int r = 0; r < RN; ++r) {
+        float d = dt[r] + bias, sig, y = 0.f;
+        if (p.softplus) d = softplus_sig(d, sig);
+#pragma unroll
+        for (int s = 0; s < SPL; ++s) {
+            h[r][s] = fmaf(__builtin_amdgcn_exp2f(d * A2[s]), reset[r] ? 0.f : h[r][s], d * uu[r] * b[r][s]);
+            y = fmaf(c[r][s], h[r][s], y);
         }
-        io_store((T *)p.out + n * p.os.n + w.h * p.os.h + w.e, y);
+        y = fmaf(Dc, uu[r], group_sum<4>(y));
+        if (p.z) y *= zz[r] * sigmoid(zz[r]);
+        const int n = n0 + r;
+        if (n < p.N) {
+            store_states<SPL>(p.last + n * D * S + states, S, w.q, h[r]);
+            if (w.q == 0) io_store((T *)p.out + n * p.os.n + w.h * p.os.h + w.e, y);
+        }
     }
 }
 
 template <typename T, int SPL>
 int launch_step(const ScanParams &p, hipStream_t s) {
-    const int Dg = p.H / p.G * p.E;
-    scan_step_kernel<T, SPL><<<dim3((Dg + kScanTile - 1) / kScanTile * p.N, p.G), kScanThreads, 0, s>>>(p);
+    constexpr int RN = SPL <= 4 ? 4 : SPL <= 8 ? 2 : 1;   // rows per thread where there are many
+    const unsigned tiles = (p.H / p.G * p.E + kScanTile - 1) / kScanTile;
+    if ((int64_t)tiles * p.G * p.N >= kScanWaves && RN > 1)
+        scan_step_kernel<T, SPL, RN><<<dim3(tiles * ((p.N + RN - 1) / RN), p.G), kScanThreads, 0, s>>>(p);
+    else
+        scan_step_kernel<T, SPL, 1><<<dim3(tiles * p.N, p.G), kScanThreads, 0, s>>>(p);
     return (int)hipGetLastError();
 }
 
