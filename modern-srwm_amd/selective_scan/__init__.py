@@ -28,86 +28,28 @@ are not read, their rows of out and of the gradients are zeros, and `last` is th
 
 Gradients go to every float tensor, through `last` and into `state` as well; keep and lengths get none.
 """
-import torch
-
 import srwm_hip
 
-
-def _wants_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-class SelectiveScan(torch.autograd.Function):
-    """selective_scan with its backward; the states of every 16th step are kept for it."""
-
-    @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus):
-        out, last, saved = srwm_hip.selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths,
-                                                           softplus, True)
-        ctx.set_materialize_grads(False)
-        ctx.softplus = softplus
-        ctx.has_state = state is not None
-        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, saved)
-        return out, last
-
-    @staticmethod
-    def backward(ctx, grad_out, grad_last):
-        u, delta, A, B, C, D, z, delta_bias, keep, lengths, saved = ctx.saved_tensors
-        if grad_out is None:
-            grad_out = torch.zeros_like(u)
-        gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate = srwm_hip.selective_scan_backward(
-            u, delta, A, B, C, D, z, delta_bias, keep, lengths, saved, grad_out, grad_last, ctx.softplus, ctx.has_state)
-        return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate, None, None, None
+_ops = srwm_hip.binding()
 
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, keep=None, lengths=None, softplus=True):
     """The scan over whole sequences: (out, last).  See the module's text.  softplus=False: dt = delta + delta_bias."""
-    if _wants_grad(u, delta, A, B, C, D, z, delta_bias, state):
-        return SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus)
-    return srwm_hip.selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus, False)[:2]
+    return _ops.selective_scan(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus)
 
 
 def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, keep=None, softplus=True):
     """One token: u, delta, z (N, H, E), B and C (N, G, S), keep (N,).  state is OVERWRITTEN; returns out (N, H, E).
     There is no backward: the call raises where a gradient would be asked of it."""
-    if _wants_grad(u, delta, A, B, C, D, z, delta_bias, state):
-        raise RuntimeError("selective_scan_step has no backward: call it under torch.no_grad(), or selective_scan with L = 1")
-    return srwm_hip.selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus)
-
-
-class CausalConv(torch.autograd.Function):
-    """causal_conv with its backward."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, state, keep, lengths, silu):
-        out, last = srwm_hip.causal_conv_forward(x, weight, bias, state, keep, lengths, silu)
-        ctx.set_materialize_grads(False)
-        ctx.silu = silu
-        ctx.save_for_backward(x, weight, bias, state, keep, lengths)
-        return out, last
-
-    @staticmethod
-    def backward(ctx, grad_out, grad_last):
-        x, weight, bias, state, keep, lengths = ctx.saved_tensors
-        if grad_out is None:
-            grad_out = torch.zeros_like(x)
-        gx, gw, gb, gstate = srwm_hip.causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_last, ctx.silu)
-        return gx, gw, gb, gstate, None, None, None
+    return _ops.selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus)
 
 
 def causal_conv(x, weight, bias=None, state=None, keep=None, lengths=None, silu=True):
     """Short causal depthwise convolution over whole sequences: (out, last).  silu=False: no activation behind it."""
-    if _wants_grad(x, weight, bias, state):
-        return CausalConv.apply(x, weight, bias, state, keep, lengths, silu)
-    return srwm_hip.causal_conv_forward(x, weight, bias, state, keep, lengths, silu)
+    return _ops.causal_conv(x, weight, bias, state, keep, lengths, silu)
 
 
 def causal_conv_step(x, state, weight, bias=None, keep=None, silu=True):
-    """One token: x (N, H, E), keep (N,).  state (N, H, W-1, E) is OVERWRITTEN; returns out (N, H, E).  No backward."""
-    if _wants_grad(x, weight, bias, state):
-        raise RuntimeError("causal_conv_step has no backward: call it under torch.no_grad(), or causal_conv with L = 1")
-    return srwm_hip.causal_conv_step(x, state, weight, bias, keep, silu)
+    """One token: x (N, H, E), keep (N,).  state (N, H, W-1, E) is OVERWRITTEN; returns out (N, H, E).  No backward: the
+    call raises where a gradient would be asked of it."""
+    return _ops.causal_conv_step(x, state, weight, bias, keep, silu)

@@ -14,7 +14,7 @@ PyTorch is used for device memory and streams only.  There is no CPU path: a mis
 library, a CPU tensor or a non-float32 tensor raises.
 """
 import ctypes
-import functools
+import importlib.util
 import os
 import subprocess
 
@@ -24,6 +24,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _PKG = os.path.dirname(_HERE)
 LIB_PATH = os.path.join(_PKG, "lib", "libsrwm_hip.so")
 CSRC = os.path.join(_PKG, "csrc")
+BINDING_PATH = os.path.join(_PKG, "lib", "srwm_torch.so")
 
 # flags of include/srwm_hip.h
 GRAD_STATE_ZERO = 0
@@ -50,6 +51,7 @@ ABI_VERSION = 18
 NO_FALLBACK = False
 
 _lib = None
+_binding = None
 
 _F = ctypes.c_void_p      # device float*
 _S = ctypes.POINTER(ctypes.c_int64)
@@ -108,7 +110,7 @@ _SIGNATURES = {
 
 
 def build(verbose=False):
-    """Compile libsrwm_hip.so for gfx950 with hipcc (always recompiles)."""
+    """Compile libsrwm_hip.so for gfx950 with hipcc, and the torch binding over it (always recompiles)."""
     out = None if verbose else subprocess.DEVNULL
     subprocess.check_call(["make", "-C", CSRC, "-B", "-j8"], stdout=out, stderr=out)
     return LIB_PATH
@@ -140,6 +142,23 @@ def lib():
         L.srwm_hip_fallback_calls.argtypes = []
         _lib = L
     return _lib
+
+
+def binding():
+    """The compiled host layer of the selective-scan, convolution and norm operators (csrc/torch_binding.cpp), over the
+    same library.  Raises if it has not been built -- there is no fallback."""
+    global _binding
+    if _binding is None:
+        if not os.path.exists(BINDING_PATH):
+            raise RuntimeError(f"{BINDING_PATH} is missing: build it with `make -C {CSRC}` (or __graft_entry__.build())")
+        lib()
+        spec = importlib.util.spec_from_file_location("srwm_torch", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.abi_version() != ABI_VERSION:
+            raise RuntimeError("srwm_torch.so was built for another ABI version; rebuild the library")
+        _binding = module
+    return _binding
 
 
 def fallback_calls():
@@ -867,401 +886,3 @@ def fast_weight_backward(q, k, v, beta, v_old, v_insert, grad_out, kv, grad_q, g
         for dst, src in zip(bf_outs, (grad_q, grad_k, grad_v, grad_beta)):
             if dst is not src:
                 dst.copy_(src)
-
-
-# ---- selective scan, short causal convolution, norm -------------------------------------------------------------------
-# These functions allocate what they return.  Optional tensors may be None.
-
-_I3 = ctypes.c_int64 * 3
-
-
-def _io_dtype(t, name):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype is not torch.float32 and t.dtype is not torch.bfloat16:
-        raise TypeError(f"{name} must be torch.float32 or torch.bfloat16 (got {t.dtype})")
-    return t.dtype
-
-
-def _gpu(t, name):
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must live on the GPU (got {t.device}); there is no CPU path")
-    return t.device
-
-
-def _on(t, name, shape, dtype, device):
-    """_require, and on the device of the call's other tensors.  `device` is a GPU's (_gpu has seen to that).  The success path is three comparisons: single-token calls are bound by this side."""
-    try:
-        if t.dtype is dtype and t.shape == shape and t.device == device:
-            return
-    except AttributeError:
-        pass
-    _require(t, name, shape, dtype)
-    raise RuntimeError(f"{name} lives on {t.device}, the call's other tensors on {device}")
-
-
-def _rows_in(t, name, shape, dtype, device):
-    """A (N, H, L, E) tensor, or the (N, H, E) rows of one step, as the kernels read it: any strides with a contiguous
-    last axis (other layouts are copied).  Returns the tensor, which the caller keeps until the launch, and its strides."""
-    _on(t, name, shape, dtype, device)
-    st = t.stride()
-    if st[-1] != 1 and shape[-1] != 1:
-        t = t.contiguous()
-        st = t.stride()
-    return t, _I3(st[0], st[1], st[2] if len(st) == 4 else 0)
-
-
-def _dense_in(t, name, shape, dtype, device):
-    """A dense tensor that starts at a multiple of 16 bytes (copied where it is not), or None."""
-    if t is None:
-        return None
-    _on(t, name, shape, dtype, device)
-    if not t.is_contiguous():
-        t = t.contiguous()
-    if t.data_ptr() & 15:
-        t = t.clone()
-    return t
-
-
-class _Here:
-    """Stands for torch.cuda.device() where the tensors' device is the current one already (the context itself costs
-    more than a microsecond)."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_ALREADY = _Here()
-
-
-def _device(device):
-    return _HERE_ALREADY if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
-
-
-def _strides3(t):
-    a, b, c, _ = t.stride()
-    return _I3(a, b, c)
-
-
-def _overwritten(t):
-    """A tensor that a kernel overwrites: itself where it is dense and 16-byte aligned, else a copy to write back from."""
-    return t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def rows_like(t):
-    """An empty tensor of t's shape and type in the memory order of t's rows, its last axis contiguous."""
-    out = torch.empty_like(t)
-    if out.stride(-1) != 1 and out.shape[-1] != 1:
-        out = torch.empty(t.shape, device=t.device, dtype=t.dtype)
-    return out
-
-
-@functools.lru_cache(maxsize=4096)
-def _workspace_floats(name, *dims):
-    n = (ctypes.c_int64 * 1)()
-    _check(getattr(lib(), name)(n, *dims), name)
-    return n[0]
-
-
-def _workspace(name, device, *dims):
-    """What an entry point asks for at these sizes, or None."""
-    n = _workspace_floats(name, *dims)
-    return torch.empty(n, device=device, dtype=torch.float32) if n else None
-
-
-def _masks(keep, lengths, N, L, device):
-    return _dense_in(keep, "keep", (N, L), torch.float32, device), _dense_in(lengths, "lengths", (N,), torch.int32, device)
-
-
-def _scan_sizes(u, A, B):
-    if u.dim() != 4 or A.dim() != 3 or B.dim() != 4:
-        raise ValueError("u must be (N, H, L, E), A (H, E, S), B and C (N, G, L, S)")
-    N, H, L, E = u.shape
-    G, S = B.shape[1], A.shape[-1]
-    if G == 0 or H % G:
-        raise ValueError(f"the {H} heads must divide into the {G} groups of B and C")
-    return N, H, L, E, S, G
-
-
-def selective_scan_forward(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus, save):
-    """The scan over whole sequences.  Returns out (in the memory order of u's rows), last (N, H, E, S) and, with `save`,
-    the states that selective_scan_backward starts from (else None)."""
-    io = _io_dtype(u, "u")
-    for t, nm in ((A, "A"), (B, "B")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{nm} must be a torch.Tensor")
-    N, H, L, E, S, G = _scan_sizes(u, A, B)
-    dev = _gpu(u, "u")
-    us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
-    ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
-    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
-    Bs, bstr = _rows_in(B, "B", (N, G, L, S), io, dev)
-    Cs, cstr = _rows_in(C, "C", (N, G, L, S), io, dev)
-    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
-    D = _dense_in(D, "D", (H, E), torch.float32, dev)
-    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
-    state = _dense_in(state, "state", (N, H, E, S), torch.float32, dev)
-    keep, lengths = _masks(keep, lengths, N, L, dev)
-    out = rows_like(u)
-    last = torch.empty((N, H, E, S), device=dev, dtype=torch.float32)
-    saved = torch.empty((N, (L + 15) // 16, H * E, S), device=dev, dtype=torch.float32) if save else None
-    if u.numel() == 0 or S == 0:
-        out.zero_()
-        last.zero_() if state is None else last.copy_(state)
-        return out, last, saved
-    work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 0)
-    fn = lib().selective_scan_forward_bf16 if io is torch.bfloat16 else lib().selective_scan_forward_f32
-    with _device(dev):
-        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(state),
-                  _p(keep), _p(lengths), _p(out), _strides3(out), _p(last), _p(saved), _p(work), N, H, L, E,
-                  S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
-    _check(code, fn.__name__)
-    return out, last, saved
-
-
-def selective_scan_backward(u, delta, A, B, C, D, z, delta_bias, keep, lengths, saved, grad_out, grad_last, softplus,
-                            with_state):
-    """Gradients of selective_scan_forward, from the states it saved.  grad_last may be None.  Returns those of u, delta,
-    A, B, C, D, z, delta_bias and (with `with_state`) state; None for what was None."""
-    io = _io_dtype(u, "u")
-    N, H, L, E, S, G = _scan_sizes(u, A, B)
-    dev = _gpu(u, "u")
-    us, ustr = _rows_in(u, "u", (N, H, L, E), io, dev)
-    ds, dstr = _rows_in(delta, "delta", (N, H, L, E), io, dev)
-    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, L, E), io, dev)
-    Bs, bstr = _rows_in(B, "B", (N, G, L, S), io, dev)
-    Cs, cstr = _rows_in(C, "C", (N, G, L, S), io, dev)
-    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
-    Dd = _dense_in(D, "D", (H, E), torch.float32, dev)
-    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
-    keep, lengths = _masks(keep, lengths, N, L, dev)
-    saved = _dense_in(saved, "saved", (N, (L + 15) // 16, H * E, S), torch.float32, dev)
-    gos, gostr = _rows_in(grad_out, "grad_out", (N, H, L, E), io, dev)
-    glast = _dense_in(grad_last, "grad_last", (N, H, E, S), torch.float32, dev)
-    gu, gdelta, gz = rows_like(u), rows_like(delta), None if z is None else rows_like(z)
-    gB, gC = rows_like(B), rows_like(C)
-    gA = torch.empty_like(A)
-    gD, gbias = None if D is None else torch.empty_like(Dd), None if bias is None else torch.empty_like(bias)
-    gstate = torch.empty((N, H, E, S), device=dev, dtype=torch.float32) if with_state else None
-    if u.numel() == 0 or S == 0:
-        for t in (gu, gdelta, gz, gB, gC, gA, gD, gbias):
-            if t is not None:
-                t.zero_()
-        if gstate is not None:
-            gstate.zero_() if glast is None else gstate.copy_(glast)
-        return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
-    fn = lib().selective_scan_backward_bf16 if io is torch.bfloat16 else lib().selective_scan_backward_f32
-    work = _workspace("selective_scan_workspace", dev, N, H, L, E, S, G, 1)
-    st = _strides3
-    with _device(dev):
-        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(Dd), _p(bias), _p(keep),
-                  _p(lengths), _p(saved), _p(gos), gostr, _p(glast), _p(gu), st(gu), _p(gdelta), st(gdelta), _p(gz),
-                  None if gz is None else st(gz), _p(gB), st(gB), _p(gC), st(gC), _p(gA), _p(gD), _p(gbias), _p(gstate),
-                  _p(work), N, H, L, E, S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
-    _check(code, fn.__name__)
-    return gu, gdelta, gA, gB, gC, gD, gz, gbias, gstate
-
-
-def selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus):
-    """One token: u, delta, z (N, H, E), B, C (N, G, S), keep (N,); state (N, H, E, S) is overwritten.  Returns out."""
-    io = _io_dtype(u, "u")
-    if u.dim() != 3 or not isinstance(A, torch.Tensor) or A.dim() != 3 or not isinstance(B, torch.Tensor) or B.dim() != 3:
-        raise ValueError("u must be (N, H, E), A (H, E, S), B and C (N, G, S)")
-    N, H, E = u.shape
-    G, S = B.shape[1], A.shape[-1]
-    if G == 0 or H % G:
-        raise ValueError(f"the {H} heads must divide into the {G} groups of B and C")
-    dev = _gpu(u, "u")
-    us, ustr = _rows_in(u, "u", (N, H, E), io, dev)
-    ds, dstr = _rows_in(delta, "delta", (N, H, E), io, dev)
-    zs, zstr = (None, None) if z is None else _rows_in(z, "z", (N, H, E), io, dev)
-    Bs, bstr = _rows_in(B, "B", (N, G, S), io, dev)
-    Cs, cstr = _rows_in(C, "C", (N, G, S), io, dev)
-    A = _dense_in(A, "A", (H, E, S), torch.float32, dev)
-    D = _dense_in(D, "D", (H, E), torch.float32, dev)
-    bias = _dense_in(delta_bias, "delta_bias", (H, E), torch.float32, dev)
-    keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
-    _on(state, "state", (N, H, E, S), torch.float32, dev)
-    out = u.new_empty((N, H, E))
-    if u.numel() == 0 or S == 0:
-        return out.zero_()
-    fn = lib().selective_scan_step_bf16 if io is torch.bfloat16 else lib().selective_scan_step_f32
-    h = _overwritten(state)
-    with _device(dev):
-        code = fn(_p(us), ustr, _p(ds), dstr, _p(zs), zstr, _p(Bs), bstr, _p(Cs), cstr, _p(A), _p(D), _p(bias), _p(keep),
-                  _p(h), _p(out), _I3(H * E, E, 0), N, H, E, S, G, FLAG_SOFTPLUS if softplus else 0, _stream(dev))
-    _check(code, fn.__name__)
-    if h is not state:
-        state.copy_(h)
-    return out
-
-
-def causal_conv_forward(x, weight, bias, state, keep, lengths, silu):
-    """Short causal depthwise convolution.  Returns out (in the memory order of x's rows) and last (N, H, W-1, E)."""
-    io = _io_dtype(x, "x")
-    if x.dim() != 4 or not isinstance(weight, torch.Tensor) or weight.dim() != 3:
-        raise ValueError("x must be (N, H, L, E), weight (H, E, W)")
-    N, H, L, E = x.shape
-    W = weight.shape[-1]
-    dev = _gpu(x, "x")
-    xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
-    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
-    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
-    if not 2 <= W <= 4:
-        raise ValueError(f"the convolution has 2 to 4 taps (got {W})")
-    state = _dense_in(state, "state", (N, H, W - 1, E), io, dev)
-    keep, lengths = _masks(keep, lengths, N, L, dev)
-    out = rows_like(x)
-    last = torch.empty((N, H, W - 1, E), device=dev, dtype=io)
-    if x.numel() == 0:
-        last.zero_() if state is None else last.copy_(state)
-        return out, last
-    fn = lib().causal_conv_forward_bf16 if io is torch.bfloat16 else lib().causal_conv_forward_f32
-    with _device(dev):
-        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(out), _strides3(out),
-                  _p(last), N, H, L, E, W, FLAG_SILU if silu else 0, _stream(dev))
-    _check(code, fn.__name__)
-    return out, last
-
-
-def causal_conv_backward(x, weight, bias, state, keep, lengths, grad_out, grad_last, silu):
-    """Gradients of causal_conv_forward: x, weight, bias, state (None for what was None).  grad_last may be None."""
-    io = _io_dtype(x, "x")
-    N, H, L, E = x.shape
-    W = weight.shape[-1]
-    dev = _gpu(x, "x")
-    xs, xstr = _rows_in(x, "x", (N, H, L, E), io, dev)
-    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
-    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
-    state = _dense_in(state, "state", (N, H, W - 1, E), io, dev)
-    keep, lengths = _masks(keep, lengths, N, L, dev)
-    gos, gostr = _rows_in(grad_out, "grad_out", (N, H, L, E), io, dev)
-    glast = _dense_in(grad_last, "grad_last", (N, H, W - 1, E), io, dev)
-    gx, gw = rows_like(x), torch.empty_like(weight)
-    gb = None if bias is None else torch.empty_like(bias)
-    gstate = None if state is None else torch.empty_like(state)
-    if x.numel() == 0:
-        gw.zero_()
-        if gb is not None:
-            gb.zero_()
-        if gstate is not None:
-            gstate.zero_() if glast is None else gstate.copy_(glast)
-        return gx, gw, gb, gstate
-    fn = lib().causal_conv_backward_bf16 if io is torch.bfloat16 else lib().causal_conv_backward_f32
-    work = _workspace("causal_conv_workspace", dev, N, H, L, E, W)
-    with _device(dev):
-        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(state), _p(keep), _p(lengths), _p(gos), gostr, _p(glast), _p(gx),
-                  _strides3(gx), _p(gw), _p(gb), _p(gstate), _p(work), N, H, L, E, W, FLAG_SILU if silu else 0,
-                  _stream(dev))
-    _check(code, fn.__name__)
-    return gx, gw, gb, gstate
-
-
-def causal_conv_step(x, state, weight, bias, keep, silu):
-    """One token: x (N, H, E), keep (N,); state (N, H, W-1, E) is overwritten.  Returns out."""
-    io = _io_dtype(x, "x")
-    if x.dim() != 3 or not isinstance(weight, torch.Tensor) or weight.dim() != 3:
-        raise ValueError("x must be (N, H, E), weight (H, E, W)")
-    N, H, E = x.shape
-    W = weight.shape[-1]
-    dev = _gpu(x, "x")
-    xs, xstr = _rows_in(x, "x", (N, H, E), io, dev)
-    weight = _dense_in(weight, "weight", (H, E, W), torch.float32, dev)
-    bias = _dense_in(bias, "bias", (H, E), torch.float32, dev)
-    if not 2 <= W <= 4:
-        raise ValueError(f"the convolution has 2 to 4 taps (got {W})")
-    keep = _dense_in(keep, "keep", (N,), torch.float32, dev)
-    _on(state, "state", (N, H, W - 1, E), io, dev)
-    out = x.new_empty((N, H, E))
-    if x.numel() == 0:
-        return out
-    fn = lib().causal_conv_step_bf16 if io is torch.bfloat16 else lib().causal_conv_step_f32
-    h = _overwritten(state)
-    with _device(dev):
-        code = fn(_p(xs), xstr, _p(weight), _p(bias), _p(keep), _p(h), _p(out), _I3(H * E, E, 0), N, H, E, W,
-                  FLAG_SILU if silu else 0, _stream(dev))
-    _check(code, fn.__name__)
-    if h is not state:
-        state.copy_(h)
-    return out
-
-
-def _norm_rows(x, residual, weight):
-    io = _io_dtype(x, "x")
-    if x.dim() < 1:
-        raise ValueError("x must have a last axis to normalise over")
-    D, dev = x.shape[-1], _gpu(x, "x")
-    xs = _dense_in(x, "x", x.shape, io, dev)
-    rdt = io
-    if residual is not None:
-        rdt = _io_dtype(residual, "residual")
-        if io is torch.float32 and rdt is not torch.float32:
-            raise TypeError("a float32 x takes a float32 residual")
-        residual = _dense_in(residual, "residual", x.shape, rdt, dev)
-    weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
-    if D == 0:
-        raise ValueError("the norm's rows are empty")
-    flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
-    return xs, residual, weight, io, rdt, x.numel() // D, D, dev, flags
-
-
-def residual_rms_norm_forward(x, residual, weight, eps, save):
-    """Root-mean-square norm of x + residual over the last axis.  Returns out (like x), the sum (like residual; x itself
-    without one) and, with `save`, the rows' reciprocal norms for the backward (else None)."""
-    xs, residual, weight, io, rdt, rows, D, dev, flags = _norm_rows(x, residual, weight)
-    out = torch.empty(x.shape, device=dev, dtype=io)
-    total = xs if residual is None else torch.empty(x.shape, device=dev, dtype=rdt)
-    rstd = torch.empty(rows, device=dev, dtype=torch.float32) if save else None
-    if rows:
-        fn = lib().residual_rms_norm_forward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_forward_f32
-        with _device(dev):
-            code = fn(_p(xs), _p(residual), _p(weight), _p(out), None if residual is None else _p(total), _p(rstd),
-                      (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
-        _check(code, fn.__name__)
-    return out, total, rstd
-
-
-def residual_rms_norm_e4m3(x, residual, weight, eps):
-    """The same with out in torch.float8_e4m3fn.  Returns out, scale (the rows' scales, last axis 1), sum."""
-    xs, residual, weight, io, rdt, rows, D, dev, flags = _norm_rows(x, residual, weight)
-    out = torch.empty(x.shape, device=dev, dtype=torch.float8_e4m3fn)
-    scale = torch.empty((*x.shape[:-1], 1), device=dev, dtype=torch.float32)
-    total = xs if residual is None else torch.empty(x.shape, device=dev, dtype=rdt)
-    if rows:
-        fn = lib().residual_rms_norm_e4m3_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_e4m3_f32
-        with _device(dev):
-            code = fn(_p(xs), _p(residual), _p(weight), _p(out), _p(scale), None if residual is None else _p(total),
-                      (ctypes.c_float * 1)(eps), rows, D, flags, _stream(dev))
-        _check(code, fn.__name__)
-    return out, scale, total
-
-
-def residual_rms_norm_backward(total, weight, rstd, grad_out, grad_total, with_residual):
-    """Gradients of residual_rms_norm_forward from the sum it returned: x (like grad_out), residual (like the sum; None
-    without `with_residual`), weight.  grad_total may be None."""
-    io, rdt, D, dev = _io_dtype(grad_out, "grad_out"), _io_dtype(total, "total"), total.shape[-1], _gpu(total, "total")
-    total = _dense_in(total, "total", total.shape, rdt, dev)
-    weight = _dense_in(weight, "weight", (D,), torch.float32, dev)
-    go = _dense_in(grad_out, "grad_out", total.shape, io, dev)
-    gt = _dense_in(grad_total, "grad_total", total.shape, rdt, dev)
-    rows = total.numel() // D
-    gx = torch.empty(total.shape, device=dev, dtype=io)
-    gr = torch.empty(total.shape, device=dev, dtype=rdt) if with_residual else None
-    gw = torch.empty_like(weight)
-    if not rows:
-        return gx, gr, gw.zero_()
-    fn = lib().residual_rms_norm_backward_bf16 if io is torch.bfloat16 else lib().residual_rms_norm_backward_f32
-    work = _workspace("residual_rms_norm_workspace", dev, rows, D)
-    flags = FLAG_RESIDUAL_F32 if io is torch.bfloat16 and rdt is torch.float32 else 0
-    with _device(dev):
-        code = fn(_p(total), _p(weight), _p(rstd), _p(go), _p(gt), _p(gx), _p(gr), _p(gw), _p(work), rows, D, flags,
-                  _stream(dev))
-    _check(code, fn.__name__)
-    return gx, gr, gw

@@ -119,6 +119,7 @@ def test_host_layer_refusals():
 
 def test_output_rows_follow_the_input():
     import srwm_hip
+    srwm_hip = srwm_hip.binding()
     x = torch.zeros(5, 3, 2 * 2 * 4).view(5, 3, 2, 2, 4)[:, :, 1].permute(1, 2, 0, 3)     # the second half of wider rows
     out = srwm_hip.rows_like(x)
     assert out.shape == (3, 2, 5, 4) and out.stride(-1) == 1
