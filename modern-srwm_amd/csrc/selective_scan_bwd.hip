@@ -9,26 +9,37 @@
 namespace fw {
 namespace {
 
-// Value of lane ^ 4 (within a row of 16: the even banks read four lanes up, the odd ones four lanes down).
-__device__ __forceinline__ float xor4(float v) {
-    const int x = __builtin_bit_cast(int, v);
-    int r = __builtin_amdgcn_update_dpp(0, x, 0x104, 0xF, 0x5, true);
-    r = __builtin_amdgcn_update_dpp(r, x, 0x114, 0xF, 0xA, false);
-    return __builtin_bit_cast(float, r);
+// One step of a reduce-scatter over lanes 8 apart, for two values: lanes 0-7 of each row of 16 end up with the sum of
+// lo over the pair (l, l ^ 8), lanes 8-15 with that of hi.  A DPP add writes the banks (groups of four lanes) that it is
+// told to, so the sum and the choice between the two are one instruction each.  Written as assembly because the compiler
+// forms it from a select, a move and an add; the s_nop covers the wait states between a vector write and a DPP read.
+__device__ __forceinline__ float scatter_add8(float lo, float hi) {
+    float r;
+    asm("s_nop 1\n\tv_add_f32_dpp %0, %1, %1 row_ror:8 row_mask:0xf bank_mask:0x3\n\t"
+        "v_add_f32_dpp %0, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xc"
+        : "=&v"(r) : "v"(lo), "v"(hi));
+    return r;
+}
+// The same over lanes 4 apart: even banks read four lanes up, odd ones four lanes down.
+__device__ __forceinline__ float scatter_add4(float lo, float hi) {
+    float r;
+    asm("s_nop 1\n\tv_add_f32_dpp %0, %1, %1 row_shl:4 row_mask:0xf bank_mask:0x5\n\t"
+        "v_add_f32_dpp %0, %2, %2 row_shr:4 row_mask:0xf bank_mask:0xa"
+        : "=&v"(r) : "v"(lo), "v"(hi));
+    return r;
 }
 
 // Sums R values over the 16 lanes with the same lane % 4 and leaves R / 16 of the sums on each of them: the lane with
 // bits (b5, b4, b3, b2) has those from index (8 b5 + 4 b4 + 2 b3 + b2) * R / 16 on.
 template <int R>
-__device__ __forceinline__ void channels_sum_scatter(const float (&v)[R], float (&out)[R / 16], int lane) {
+__device__ __forceinline__ void channels_sum_scatter(const float (&v)[R], float (&out)[R / 16]) {
     float a[R / 2], b[R / 4], c[R / 8];
     swap_halve<32, R>(v, a);
     swap_halve<16, R / 2>(a, b);
-    const bool b3 = lane & 8, b2 = lane & 4;
 #pragma unroll
-    for (int i = 0; i < R / 8; ++i) c[i] = (b3 ? b[i + R / 8] : b[i]) + dpp_mov<kDppRor8>(b3 ? b[i] : b[i + R / 8]);
+    for (int i = 0; i < R / 8; ++i) c[i] = scatter_add8(b[i], b[i + R / 8]);
 #pragma unroll
-    for (int i = 0; i < R / 16; ++i) out[i] = (b2 ? c[i + R / 16] : c[i]) + xor4(b2 ? c[i] : c[i + R / 16]);
+    for (int i = 0; i < R / 16; ++i) out[i] = scatter_add4(c[i], c[i + R / 16]);
 }
 
 // v[i], i uniform: a constant after unrolling, else three selects
@@ -202,13 +213,19 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
             dt[i] = (float)rd[i] + bias;
             sg[i] = 1.f;
             if (p.softplus) dt[i] = softplus_sig(dt[i], sg[i]);
-            gg[i] = w.on ? (float)rg[i] : 0.f;   // a lane without a channel adds nothing to gB and gC
+            gg[i] = (float)rg[i];
             zz[i] = gate ? (float)rz[i] : 0.f;
         }
         if (n < kScanBlock) {   // behind the end: a decay of one, nothing added, no gradient
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (4 * i + w.q >= n) uu[i] = 0.f, dt[i] = 0.f, sg[i] = 0.f, gg[i] = 0.f, zz[i] = 0.f;
+        }
+        if (!w.on) {   // a lane without a channel: zeros throughout, so that it adds nothing to gB and gC
+#pragma unroll
+            for (int i = 0; i < 4; ++i) uu[i] = 0.f, dt[i] = 0.f, gg[i] = 0.f, zz[i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < SPL; ++s) h0[s] = 0.f, gh[s] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -309,12 +326,8 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
                     gh[s] = KEEP && reset ? 0.f : ag;
                 }
                 if (k % TG == 0) {
-                    if (!w.on) {
-#pragma unroll
-                        for (int x = 0; x < R; ++x) v[x] = 0.f;
-                    }
                     float r[R / 16];
-                    channels_sum_scatter<R>(v, r, w.lane);
+                    channels_sum_scatter<R>(v, r);
                     const int at = (w.lane >> 2) * (R / 16);
 #pragma unroll
                     for (int x = 0; x < R / 16; ++x) {
