@@ -175,7 +175,7 @@ int scan_backward(const void *u, const int64_t *us, const void *delta, const int
         return SRWM_EINVAL;
     if (flags & ~SRWM_FLAG_SOFTPLUS) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
-    if ((int64_t)N * G * L * 2 * S + (int64_t)H * E * (S + 2) > kMaxGrid * 256) return SRWM_ESIZE;
+    if ((int64_t)N * G * L * 2 * S / 256 + (int64_t)H * E * (S + 2) / 32 + 2 > kMaxGrid) return SRWM_ESIZE;   // the join's workgroups
     if (!stride_ok(us, N, H, L, E) || !stride_ok(ds, N, H, L, E) || (z && !stride_ok(zs, N, H, L, E)) ||
         !stride_ok(Bs, N, G, L, S) || !stride_ok(Cs, N, G, L, S) || !stride_ok(gos, N, H, L, E) ||
         !out_stride_ok(gus, N, H, L, E) || !out_stride_ok(gds, N, H, L, E) || (z && !out_stride_ok(gzs, N, H, L, E)) ||

@@ -10,6 +10,7 @@ namespace fw {
 namespace {
 
 constexpr int kNormThreads = 256;
+constexpr int kNormBlocks = 1024;   // workgroups of the backward, each with a share of the weight's gradient
 constexpr float kE4m3Max = 448.f;
 
 // Sum (or maximum) over the TPR lanes of a row.
@@ -155,7 +156,14 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormBwdParams p)
     for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR; row < p.rows; row += (int64_t)p.blocks * RPB) {
         const int64_t base = row * p.D;
         const float rstd = p.rstd[row];
-        float hat[NV][V], g[NV][V], m = 0.f;
+        float hat[NV][V], g[NV][V], s[NV][V], m = 0.f;
+        if (p.gsum) {   // asked for in front of the row's reduction, used behind it
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int d = (k * TPR + lane) * V;
+                if (d < p.D) load_vec<V>((const TR *)p.gsum + base + d, s[k]);
+            }
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int d = (k * TPR + lane) * V;
@@ -178,13 +186,11 @@ __global__ __launch_bounds__(kNormThreads) void norm_bwd_kernel(NormBwdParams p)
         for (int k = 0; k < NV; ++k) {
             const int d = (k * TPR + lane) * V;
             if (d < p.D) {
-                float v[V], s[V];
+                float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = rstd * fmaf(-hat[k][i], m, g[k][i]);
-                if (p.gsum) {
-                    load_vec<V>((const TR *)p.gsum + base + d, s);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) v[i] += s[i];
+                for (int i = 0; i < V; ++i) {
+                    v[i] = rstd * fmaf(-hat[k][i], m, g[k][i]);
+                    if (p.gsum) v[i] += s[k][i];
                 }
                 store_vec<V>((TX *)p.gx + base + d, v);
                 if (p.gres) store_vec<V>((TR *)p.gres + base + d, v);
@@ -252,7 +258,9 @@ int bwd_by_size(const NormBwdParams &p, hipStream_t s) {
     constexpr int M = 32 / V;
 #define FW_NORM(TPR, NV) norm_bwd_kernel<TX, TR, V, TPR, NV><<<(unsigned)p.blocks, kNormThreads, 0, s>>>(p)
     if (per <= M / 4) FW_NORM(64, M / 4);
+    else if (per <= M / 2) FW_NORM(64, M / 2);
     else if (per <= M) FW_NORM(64, M);
+    else if (per <= 2 * M) FW_NORM(256, M / 2);
     else if (per <= 4 * M) FW_NORM(256, M);
     else if (per <= 8 * M) FW_NORM(256, 2 * M);
     else return -1;
@@ -281,7 +289,7 @@ int bwd_types(const NormBwdParams &p, hipStream_t s) {
 
 int norm_bwd_blocks(int64_t rows, int D) {
     const int64_t groups = D <= 2048 ? (rows + 3) / 4 : rows;
-    return (int)(groups < 512 ? groups : 512);
+    return (int)(groups < kNormBlocks ? groups : kNormBlocks);
 }
 
 int launch_norm_fwd(const NormParams &p, bool x_bf16, bool r_bf16, bool e4m3, hipStream_t s) {

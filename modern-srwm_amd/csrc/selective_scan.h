@@ -27,7 +27,7 @@ namespace fw {
 constexpr int kScanBlock = 16;      // steps between two saved states, and per stage of B and C in LDS
 constexpr int kScanThreads = 256;   // 4 waves
 constexpr int kScanWaves = 4096;        // a call is cut into segments until it has this many waves (4 on each SIMD)
-constexpr int kScanMinSegment = 64;     // shortest segment
+constexpr int kScanMinSegment = 32;     // shortest segment
 
 // From four values per lane to one: lane j of each quad ends up with the quad's sum of v[j].
 __device__ __forceinline__ float quad_sum_scatter(float v0, float v1, float v2, float v3, int lane) {
@@ -173,6 +173,28 @@ __device__ __forceinline__ void store_states(float *row, int S, int q, const flo
 #pragma unroll
         for (int i = 0; i < SPL; ++i)
             if (q * SPL + i < S) row[q * SPL + i] = v[i];
+    }
+}
+
+// Carries a state (or its gradient) over `count` segments from the one at `at` on, `stride` floats from one to the next:
+// x = decay x + result.  Four segments are asked for at a time.
+template <int SPL>
+__device__ __forceinline__ void join_segments(const ScanParams &p, int64_t at, int64_t stride, int count, int S, int q, float (&x)[SPL]) {
+    constexpr int U = SPL <= 4 ? 4 : 2;
+    for (int k = 0; k < count; k += U) {
+        float pr[U][SPL], r[U][SPL];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t o = at + min(k + i, count - 1) * stride;
+            load_states<SPL>(p.seg_decay + o, S, q, pr[i]);
+            load_states<SPL>(p.seg_state + o, S, q, r[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (k + i < count) {
+#pragma unroll
+                for (int s = 0; s < SPL; ++s) x[s] = dropped(pr[i][s]) ? r[i][s] : fmaf(pr[i][s], x[s], r[i][s]);
+            }
     }
 }
 

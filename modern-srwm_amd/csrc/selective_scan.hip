@@ -51,14 +51,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     if (tbeg < tend) fetch(tbeg, tend - tbeg);
     if constexpr (!LOCAL) {
         if (p.state) load_states<SPL>(p.state + w.n * (int64_t)D * S + states, S, w.q, h);
-        for (int k = 0; k < seg; ++k) {   // the segments in front, one after the other
-            const int64_t at = ((int64_t)w.n * p.segments + k) * D * S + states;
-            float pr[SPL], hl[SPL];
-            load_states<SPL>(p.seg_decay + at, S, w.q, pr);
-            load_states<SPL>(p.seg_state + at, S, w.q, hl);
-#pragma unroll
-            for (int s = 0; s < SPL; ++s) h[s] = dropped(pr[s]) ? hl[s] : fmaf(pr[s], h[s], hl[s]);
-        }
+        const int64_t stride = (int64_t)D * S;
+        join_segments<SPL>(p, (int64_t)w.n * p.segments * stride + states, stride, seg, S, w.q, h);   // the segments in front
     }
     float *saved = nullptr;
     if (!LOCAL && p.saved)
@@ -244,9 +238,8 @@ int launch_step(const ScanParams &p, hipStream_t s) {
 int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len) {
     const int64_t waves = ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile * N * G * (kScanThreads / 64);
     int64_t n = (kScanWaves + waves - 1) / waves;
-    const int64_t most = L / kScanMinSegment;
+    const int64_t most = (L + kScanMinSegment - 1) / kScanMinSegment;
     n = n < most ? n : most;
-    if (n < 2) n = 1;
     int l = (int)((L + n - 1) / n);
     l = (l + kScanBlock - 1) / kScanBlock * kScanBlock;
     *len = l;

@@ -195,14 +195,9 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
     };
     if (tbeg < tend) fetch(last, tend - last);
     if (b.glast) load_states<SPL>(b.glast + w.n * (int64_t)D * S + states, S, w.q, gh);
-    for (int k = p.segments - 1; k > seg; --k) {   // the segments behind, one after the other
-        const int64_t at = ((int64_t)w.n * p.segments + k) * D * S + states;
-        float pr[SPL], gl[SPL];
-        load_states<SPL>(p.seg_decay + at, S, w.q, pr);
-        load_states<SPL>(p.seg_state + at, S, w.q, gl);
-#pragma unroll
-        for (int s = 0; s < SPL; ++s) gh[s] = dropped(pr[s]) ? gl[s] : fmaf(pr[s], gh[s], gl[s]);
-    }
+    const int64_t stride = (int64_t)D * S;
+    join_segments<SPL>(p, ((int64_t)w.n * p.segments + p.segments - 1) * stride + states, -stride, p.segments - 1 - seg, S, w.q,
+                       gh);   // the segments behind
     for (int t0 = last; t0 >= tbeg && tbeg < tend; t0 -= kScanBlock) {
         const int n = tend - t0;   // steps of this block, 16 or more: all
         // what a channel needs once per step: lane q holds the steps 4i + q
@@ -376,10 +371,11 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
         }
 }
 
-// Joins the partial sums: those of gB and gC over the tiles of a group, those of gA, gD and gbias over batch and
-// segments.
+// Joins the partial sums, in a fixed order: those of gB and gC over the tiles of a group (an element per thread), those
+// of gA, gD and gbias over batch and segments (32 columns per workgroup, 8 threads over the rows of each).
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bwd_join_kernel(ScanBwdParams b, int tiles, unsigned blocks_bc) {
+    __shared__ float sums[8][32];
     const ScanParams &p = b.f;
     const int S = p.S;
     if (blockIdx.x < blocks_bc) {
@@ -390,21 +386,34 @@ __global__ __launch_bounds__(256) void scan_bwd_join_kernel(ScanBwdParams b, int
         const int64_t r = i / (2 * S);
         const int t = r % p.L, g = r / p.L % p.G, n = r / p.L / p.G;
         float v = 0.f;
-        if (!p.lengths || t < p.lengths[n])
+        if (!p.lengths || t < p.lengths[n]) {
+#pragma unroll 8
             for (int k = 0; k < tiles; ++k) v += b.part_bc[k * per + i];
+        }
         if (c) io_store((T *)b.gC + n * b.gCs.n + g * b.gCs.h + t * b.gCs.l + s, v);
         else io_store((T *)b.gB + n * b.gBs.n + g * b.gBs.h + t * b.gBs.l + s, v);
         return;
     }
     const int64_t D = (int64_t)p.H * p.E, row = scan_part_a_row(D, S);
-    const int64_t i = (int64_t)(blockIdx.x - blocks_bc) * 256 + threadIdx.x;
-    if (i >= D * (S + 2)) return;
-    float *dst = i < D * S ? b.gA + i : i < D * (S + 1) ? (b.gD ? b.gD + (i - D * S) : nullptr)
-                                                        : (b.gbias ? b.gbias + (i - D * (S + 1)) : nullptr);
-    if (!dst) return;
+    const int c = threadIdx.x % 32, r = threadIdx.x / 32, rows = p.N * p.segments;
+    const int64_t i = (int64_t)(blockIdx.x - blocks_bc) * 32 + c;
+    float *dst = nullptr;
+    if (i < D * S) dst = b.gA + i;
+    else if (i < D * (S + 1)) dst = b.gD ? b.gD + (i - D * S) : nullptr;
+    else if (i < D * (S + 2)) dst = b.gbias ? b.gbias + (i - D * (S + 1)) : nullptr;
     float v = 0.f;
-    for (int n = 0; n < p.N * p.segments; ++n) v += b.part_a[n * row + i];
-    *dst = v;
+    if (dst) {
+#pragma unroll 8
+        for (int n = r; n < rows; n += 8) v += b.part_a[n * row + i];
+    }
+    sums[r][c] = v;
+    __syncthreads();
+    if (r == 0 && dst) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += sums[k][c];
+        *dst = v;
+    }
 }
 
 template <typename T, int SPL, typename OFF>
@@ -422,7 +431,7 @@ int launch_bwd_as(const ScanBwdParams &b, hipStream_t s) {
     else scan_bwd_kernel<T, SPL, false, OFF><<<grid, kScanThreads, 0, s>>>(b);
     if ((r = (int)hipGetLastError())) return r;
     const int64_t nbc = ((int64_t)p.N * p.G * p.L * 2 * p.S + 255) / 256;
-    const int64_t na = ((int64_t)p.H * p.E * (p.S + 2) + 255) / 256;
+    const int64_t na = ((int64_t)p.H * p.E * (p.S + 2) + 31) / 32;
     scan_bwd_join_kernel<T><<<(unsigned)(nbc + na), 256, 0, s>>>(b, (int)tiles, (unsigned)nbc);
     return (int)hipGetLastError();
 }
