@@ -237,8 +237,10 @@ int launch_step(const ScanParams &p, hipStream_t s) {
 
 int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len) {
     const int64_t waves = ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile * N * G * (kScanThreads / 64);
-    int64_t n = (kScanWaves + waves - 1) / waves;
-    const int64_t most = (L + kScanMinSegment - 1) / kScanMinSegment;
+    int64_t n = waves >= (backward ? kScanEnoughBwd : kScanEnoughFwd) ? 1 : (kScanWaves + waves - 1) / waves;
+    int64_t most = (L + kScanMinSegment - 1) / kScanMinSegment;
+    while (most * most > (int64_t)L * (backward ? 4 : 1)) most = most * 7 / 8;
+    if (most < 1) most = 1;
     n = n < most ? n : most;
     int l = (int)((L + n - 1) / n);
     l = (l + kScanBlock - 1) / kScanBlock * kScanBlock;
