@@ -6,6 +6,7 @@
                                       calls it FastFFlayer too; it threads the memory as state)
     SMFWPlayer                        reinforcement_learning/torchbeast/layer.py:492-586
     FastFastFFlayer, PseudoSRlayer    reinforcement_learning/torchbeast/layer.py:193-283, :286-336
+    SelectiveLayer, SelectiveStack    no counterpart: selective state-space layers with the same conventions
 
 Same constructor arguments, parameter names and shapes (so state_dicts of the reference load
 unchanged: W_y, W_q, W_k: (1, H, d, d); w_b: (1, H, d, 4); slow_net / out_linear / layer_norm),
@@ -23,6 +24,8 @@ import torch.nn.functional as F
 from fast_weight import delta_layer_inputs
 from fast_weight import fast_weight_delta_rows as fast_weight_delta
 from fast_weight import fast_weight_delta_steps_rows as fast_weight_delta_steps
+from residual_norm import residual_rms_norm, residual_rms_norm_e4m3
+from selective_scan import causal_conv, causal_conv_step, selective_scan, selective_scan_step
 from self_ref_v0 import self_ref_layer, self_ref_layer_steps, self_ref_v0, self_ref_v0_steps, stateful_self_ref_v0
 from self_ref_v1 import self_ref_v1, self_ref_v1_steps
 
@@ -400,3 +403,153 @@ class PseudoSRlayer(nn.Module):
         out = torch.bmm(x, self.W_y).permute(1, 0, 2).reshape(slen, bsz, self.num_head * self.dim_head)
         out = h + self.drop(self.out_linear(out))
         return out, state
+
+
+class SelectiveLayer(nn.Module):
+    """Selective state-space layer: root-mean-square norm, input projection to a branch and its gate, short causal
+    convolution, step sizes and B, C projected from it, selective scan, output projection.  State: (the convolution's last
+    d_conv - 1 inputs (B, H, d_conv-1, d), the scan's states (B, H, d, d_state)), None at the start.
+
+        out = layer(h)                                   h: (len, B, in_dim); h + mixer(norm(h))
+        out, state = layer(h, state, get_state=True)     carries a state over calls (prompts, segments)
+        out, state = layer.forward_steps(h, notdone, state)    an RL unroll: states restart where notdone is 0
+        out = layer.step(h, state)                       one token, h: (B, in_dim); state is OVERWRITTEN; no gradients
+
+    lengths: (B,) int32 steps of each row of a padded batch; packed sequences restart through forward_steps' notdone.
+    `mix` is the part behind the residual stream, for stacks that add the stream inside the norm (SelectiveStack).
+    groups: heads share B and C in groups.  Unlike the other RL layers, gradients flow through the carried state inside an
+    unroll; what comes in and goes out as state is detached by forward_steps."""
+
+    def __init__(self, num_head, dim_head, in_dim, dropout, d_state=16, d_conv=4, dt_rank=None, groups=1, eps=1e-5):
+        super().__init__()
+        self.num_head, self.dim_head, self.in_dim = num_head, dim_head, in_dim
+        self.d_state, self.d_conv, self.groups, self.eps = d_state, d_conv, groups, eps
+        inner = num_head * dim_head
+        self.dt_rank = dt_rank or max(1, math.ceil(in_dim / 16))
+        self.norm_weight = nn.Parameter(torch.ones(in_dim))
+        self.in_linear = nn.Linear(in_dim, 2 * inner, bias=False)
+        self.conv_weight = nn.Parameter(torch.empty(num_head, dim_head, d_conv))
+        self.conv_bias = nn.Parameter(torch.zeros(num_head, dim_head))
+        self.x_linear = nn.Linear(inner, self.dt_rank + 2 * groups * d_state, bias=False)
+        self.dt_linear = nn.Linear(self.dt_rank, inner, bias=False)
+        self.dt_bias = nn.Parameter(torch.empty(num_head, dim_head))
+        self.A_log = nn.Parameter(torch.empty(num_head, dim_head, d_state))
+        self.D = nn.Parameter(torch.ones(num_head, dim_head))
+        self.out_linear = nn.Linear(inner, in_dim, bias=False)
+        self.drop = nn.Dropout(dropout)
+        self._eight = None   # the input projection in e4m3, see serve_e4m3
+        nn.init.uniform_(self.conv_weight, -d_conv ** -0.5, d_conv ** -0.5)
+        # step sizes spread over 1e-3 .. 1e-1 where their projection is zero; decays of 1 .. d_state per unit of time
+        first = torch.exp(torch.rand(num_head, dim_head) * math.log(100.) + math.log(1e-3))
+        with torch.no_grad():
+            self.dt_bias.copy_(torch.log(torch.expm1(first)))
+            self.A_log.copy_(torch.log(torch.arange(1, d_state + 1, dtype=torch.float32)).expand_as(self.A_log))
+
+    def serve_e4m3(self):
+        """From here on the projection in front runs in 8 bits wherever no gradient is recorded: its weight is kept as
+        e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16."""
+        if self.in_dim % 16 or self.num_head * self.dim_head % 8:
+            raise ValueError("the 8-bit projection needs in_dim and 2 * num_head * dim_head divisible by 16")
+        w = self.in_linear.weight.detach().float()
+        scale = w.abs().amax(1, keepdim=True).clamp_min(1e-30) / 448
+        self._eight = ((w / scale).to(torch.float8_e4m3fn), scale.t().contiguous())
+        return self
+
+    def _project_in(self, h, residual):
+        """Norm and input projection: ([x | z] rows (..., 2 * inner), the residual stream with h added)."""
+        weight = self.norm_weight.float()
+        if self._eight is None or torch.is_grad_enabled():
+            y, total = residual_rms_norm(h, residual, weight, self.eps)
+            return self.in_linear(y.to(self.in_linear.weight.dtype)), total
+        y, scale, total = residual_rms_norm_e4m3(h, residual, weight, self.eps)
+        w, w_scale = self._eight
+        rows = torch._scaled_mm(y.reshape(-1, self.in_dim), w.t(), scale_a=scale.reshape(-1, 1), scale_b=w_scale,
+                                out_dtype=torch.bfloat16)
+        return rows.to(h.dtype).view(*h.shape[:-1], -1), total
+
+    def _parameters_of_scan(self):
+        return -torch.exp(self.A_log.float()), self.D.float(), self.dt_bias.float()
+
+    def _split(self, x):
+        """Step sizes and B, C from the convolution's output (..., inner)."""
+        r, gs = self.dt_rank, self.groups * self.d_state
+        p = self.x_linear(x)
+        bc = p[..., r:].unflatten(-1, (2, self.groups, self.d_state))
+        return self.dt_linear(p[..., :r]).unflatten(-1, (self.num_head, self.dim_head)), bc.select(-3, 0), bc.select(-3, 1)
+
+    def mix(self, h, residual=None, state=None, keep=None, lengths=None):
+        """(output without the residual, the residual stream with h added, new state).  h: (len, B, in_dim)."""
+        slen, bsz, _ = h.shape
+        inner = self.num_head * self.dim_head
+        rows, total = self._project_in(h, residual)
+        x, z = rows.view(slen, bsz, 2, self.num_head, self.dim_head).permute(2, 1, 3, 0, 4)
+        conv_state, scan_state = state if state is not None else (None, None)
+        x, conv_state = causal_conv(x, self.conv_weight.float(), self.conv_bias.float(), conv_state, keep, lengths)
+        dt, B, C = self._split(_heads_out(x, bsz, slen, inner))
+        A, D, dt_bias = self._parameters_of_scan()
+        out, scan_state = selective_scan(x, dt.permute(1, 2, 0, 3), A, B.permute(1, 2, 0, 3), C.permute(1, 2, 0, 3), D, z,
+                                         dt_bias, scan_state, keep, lengths)
+        return self.drop(self.out_linear(_heads_out(out, bsz, slen, inner))), total, (conv_state, scan_state)
+
+    def forward(self, h, state=None, get_state=False, lengths=None):
+        out, _, state = self.mix(h, None, state, None, lengths)
+        return (h + out, state) if get_state else h + out
+
+    def forward_steps(self, h, notdone, state=None):
+        """h: (T, B, in_dim); notdone: (T, B), 0 where an episode ended before the step."""
+        if state is not None:
+            state = tuple(s.detach() for s in state)
+        out, _, state = self.mix(h, None, state, _keep_rows(notdone, torch.float32))
+        return h + out, tuple(s.detach() for s in state)
+
+    def start(self, bsz, device, dtype=torch.float32):
+        """A state of zeros for step()."""
+        return (torch.zeros(bsz, self.num_head, self.d_conv - 1, self.dim_head, device=device, dtype=dtype),
+                torch.zeros(bsz, self.num_head, self.dim_head, self.d_state, device=device))
+
+    @torch.no_grad()
+    def mix_step(self, h, residual, state, keep=None):
+        """mix for one token: h (B, in_dim); state is OVERWRITTEN.  Returns the output and the residual stream."""
+        bsz = h.shape[0]
+        rows, total = self._project_in(h, residual)
+        x, z = rows.view(bsz, 2, self.num_head, self.dim_head).unbind(1)
+        x = causal_conv_step(x, state[0], self.conv_weight.float(), self.conv_bias.float(), keep)
+        dt, B, C = self._split(x.view(bsz, -1))
+        A, D, dt_bias = self._parameters_of_scan()
+        out = selective_scan_step(x, dt, state[1], A, B, C, D, z, dt_bias, keep)
+        return self.out_linear(out.view(bsz, -1)), total
+
+    def step(self, h, state, keep=None):
+        return h + self.mix_step(h, None, state, keep)[0]
+
+
+class SelectiveStack(nn.Module):
+    """Layers of the above on one residual stream in float32: every norm adds the layer in front to the stream and
+    normalises it in one pass, and a last one does so behind the stack.  states: one per layer."""
+
+    def __init__(self, num_layers, num_head, dim_head, in_dim, dropout, **kwargs):
+        super().__init__()
+        self.layers = nn.ModuleList(SelectiveLayer(num_head, dim_head, in_dim, dropout, **kwargs) for _ in range(num_layers))
+        self.norm_weight = nn.Parameter(torch.ones(in_dim))
+        self.eps = self.layers[0].eps
+
+    def serve_e4m3(self):
+        for layer in self.layers:
+            layer.serve_e4m3()
+        return self
+
+    def forward(self, h, states=None, keep=None, lengths=None):
+        """h: (len, B, in_dim) -> (normalised output, states)."""
+        residual, new = torch.zeros(h.shape, device=h.device, dtype=torch.float32), []
+        for layer, state in zip(self.layers, states or [None] * len(self.layers)):
+            h, residual, state = layer.mix(h, residual, state, keep, lengths)
+            new.append(state)
+        return residual_rms_norm(h, residual, self.norm_weight.float(), self.eps)[0], new
+
+    @torch.no_grad()
+    def step(self, h, states, keep=None):
+        """One token: h (B, in_dim); states are OVERWRITTEN."""
+        residual = torch.zeros(h.shape, device=h.device, dtype=torch.float32)
+        for layer, state in zip(self.layers, states):
+            h, residual = layer.mix_step(h, residual, state, keep)
+        return residual_rms_norm(h, residual, self.norm_weight.float(), self.eps)[0]

@@ -1,0 +1,168 @@
+"""The selective state-space layers on the GPU: against the same layer written from the oracle's operators in 64 bits, and
+their forms (segments, unrolls, single tokens, padded batches, 8-bit projection) against each other.
+
+Tolerance of the float32 layers: each of the seven operators in a row (norm, four projections, convolution, scan) holds
+1e-5 of its largest value, so a result and its gradients hold 1e-4."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from layer import SelectiveLayer, SelectiveStack
+from oracle import selective
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TOL = 1e-4
+
+
+def close(got, want, name, tol=TOL):
+    got, want = got.detach().cpu().double(), want.detach().cpu().double()
+    err = float((got - want).abs().max()) / max(float(want.abs().max()), 1e-30)
+    assert got.shape == want.shape and err < tol, f"{name}: {err:.3g}"
+
+
+def plain_mix(p, layer, h, residual, keep=None, lengths=None):
+    """mix() in float64 from parameters p (name -> tensor)."""
+    L, B, _ = h.shape
+    H, d, S, G, r = layer.num_head, layer.dim_head, layer.d_state, layer.groups, layer.dt_rank
+    heads = lambda t: t.reshape(L, B, H, d).permute(1, 2, 0, 3)
+    rows = lambda t: t.permute(2, 0, 1, 3).reshape(L, B, H * d)
+    y, total = selective.rms_norm(h, residual, p["norm_weight"], layer.eps)
+    xz = F.linear(y, p["in_linear.weight"])
+    x, z = heads(xz[..., :H * d]), heads(xz[..., H * d:])
+    x, _ = selective.conv(x, p["conv_weight"], p["conv_bias"], None, keep, lengths)
+    q = F.linear(rows(x), p["x_linear.weight"])
+    dt = heads(F.linear(q[..., :r], p["dt_linear.weight"]))
+    Bm, Cm = (t.reshape(L, B, G, S).permute(1, 2, 0, 3) for t in (q[..., r:r + G * S], q[..., r + G * S:]))
+    out, _ = selective.scan(x, dt, -torch.exp(p["A_log"]), Bm, Cm, p["D"], z, p["dt_bias"], None, keep, lengths)
+    return F.linear(rows(out), p["out_linear.weight"]), total
+
+
+def make(seed=0, **kw):
+    torch.manual_seed(seed)
+    layer = SelectiveLayer(4, 8, 24, 0.0, **kw).to(DEV)
+    with torch.no_grad():
+        for q in (layer.A_log, layer.D, layer.norm_weight, layer.conv_bias):
+            q.add_(0.1 * torch.randn_like(q))
+    return layer
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(groups=2, d_state=8, d_conv=3), dict(groups=4, d_state=20, d_conv=2, dt_rank=3)], ids=str)
+def test_layer_and_gradients_against_the_oracle(kw):
+    layer = make(**kw)
+    g = torch.Generator().manual_seed(1)
+    h = torch.randn(19, 3, 24, generator=g)
+    go = torch.randn(19, 3, 24, generator=g)
+    lengths = torch.tensor([19, 7, 1], dtype=torch.int32)
+    p = {k: v.detach().cpu().double().requires_grad_() for k, v in layer.named_parameters()}
+    hd = h.double().requires_grad_()
+    want = hd + plain_mix(p, layer, hd, None, None, lengths)[0]
+    grads = torch.autograd.grad(want, [hd, *p.values()], go.double())
+    hg = h.to(DEV).requires_grad_()
+    out = layer(hg, lengths=lengths.to(DEV))
+    close(out, want, "out")
+    got = torch.autograd.grad(out, [hg, *layer.parameters()], go.to(DEV))
+    for k, a, b in zip(["h", *p], got, grads):
+        close(a, b, "g_" + k)
+
+
+def test_stack_and_gradients_against_the_oracle():
+    torch.manual_seed(3)
+    stack = SelectiveStack(2, 2, 8, 16, 0.0).to(DEV)
+    g = torch.Generator().manual_seed(4)
+    h, go = torch.randn(11, 2, 16, generator=g), torch.randn(11, 2, 16, generator=g)
+    p = {k: v.detach().cpu().double().requires_grad_() for k, v in stack.named_parameters()}
+    x, residual = h.double().requires_grad_(), torch.zeros(11, 2, 16, dtype=torch.float64)
+    h0 = x
+    for i, layer in enumerate(stack.layers):
+        mine = {k.split(".", 2)[2]: v for k, v in p.items() if k.startswith(f"layers.{i}.")}
+        x, residual = plain_mix(mine, layer, x, residual)
+    want = selective.rms_norm(x, residual, p["norm_weight"], stack.eps)[0]
+    hg = h.to(DEV).requires_grad_()
+    out, _ = stack(hg)
+    close(out, want, "out")
+    grads = torch.autograd.grad(want, [h0, *p.values()], go.double())
+    got = torch.autograd.grad(out, [hg, *stack.parameters()], go.to(DEV))
+    for k, a, b in zip(["h", *p], got, grads):
+        close(a, b, "g_" + k)
+
+
+def test_segments_unrolls_and_tokens_agree():
+    """One call, two calls with the state carried, an unroll with resets, and single tokens on the same rows."""
+    layer = make(2)
+    h = torch.randn(21, 3, 24, generator=torch.Generator().manual_seed(5)).to(DEV)
+    notdone = torch.ones(21, 3, device=DEV)
+    notdone[0] = notdone[8, 1] = notdone[20, 2] = 0
+    with torch.no_grad():
+        whole, end = layer(h, get_state=True)
+        first, state = layer(h[:9], get_state=True)
+        second, state = layer(h[9:], state, get_state=True)
+        close(torch.cat((first, second)), whole, "segments")
+        close(state[1], end[1], "scan state")
+        assert torch.equal(state[0], end[0])
+        unroll, ustate = layer.forward_steps(h, notdone, tuple(torch.randn_like(s) for s in end))
+        state = layer.start(3, DEV)
+        tokens = [layer.step(h[t], state, notdone[t].contiguous()) for t in range(21)]
+        close(torch.stack(tokens), unroll, "tokens")
+        close(state[1], ustate[1], "scan state of the tokens")
+    close(unroll[:8], whole[:8], "rows in front of the first reset")
+    lengths = torch.tensor([21, 4, 0], dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        padded, pstate = layer(h, get_state=True, lengths=lengths)
+        short, sstate = layer(h[:4, 1:2], get_state=True)
+    close(padded[:4, 1:2], short, "padded row")
+    close(pstate[1][1:2], sstate[1], "state of the padded row")
+    assert torch.equal(padded[4:, 1], h[4:, 1])            # behind a row's end the layer adds nothing
+
+
+def test_bf16_layer_runs_and_is_near_the_float32_one():
+    layer = make(6)
+    h = torch.randn(33, 2, 24, generator=torch.Generator().manual_seed(7)).to(DEV)
+    with torch.no_grad():
+        want = layer(h)
+    low = make(6).to(torch.bfloat16)
+    x = h.bfloat16().requires_grad_()
+    out = low(x)
+    # seven roundings to bfloat16 in a row, half a step of 2^-8 of the largest value each
+    close(out, want, "out", 7 * 2.0 ** -8)
+    out.float().square().sum().backward()
+    assert all(torch.isfinite(q.grad).all() for q in low.parameters()) and torch.isfinite(x.grad).all()
+
+
+def test_eight_bit_projection():
+    """The rows of the norm and the weight are rounded to e4m3: each factor of the projection is off by at most half a step,
+    2^-4 of itself, so a product by 2 * 2^-4 (and their product), and a projected value by that share of the sum of its
+    terms' sizes; float32 accumulation and the bfloat16 result (2^-8) add to it."""
+    torch.manual_seed(8)
+    layer = SelectiveLayer(4, 16, 32, 0.0).to(DEV).to(torch.bfloat16).serve_e4m3()
+    for rows in (1, 3, 16, 100):
+        h = torch.randn(rows, 2, 32, generator=torch.Generator().manual_seed(rows)).to(DEV).bfloat16()
+        with torch.no_grad():
+            got, total = layer._project_in(h, None)
+            y, _ = selective.rms_norm(h.cpu().double(), None, layer.norm_weight.detach().cpu().double(), layer.eps)
+            w = layer.in_linear.weight.detach().cpu().double()
+            want, size = F.linear(y, w), F.linear(y.abs(), w.abs())
+            bound = size * (2 * 2.0 ** -4 + 2.0 ** -8 + 1e-3) + want.abs() * 2.0 ** -8
+            # values below the smallest normal number of e4m3 are off by 2^-10 of the row's scale at most
+            bound = bound + 2.0 ** -10 / 448 * (F.linear(y.abs().amax(-1, keepdim=True).expand_as(y), w.abs())
+                                                + F.linear(y.abs(), w.abs().amax(1, keepdim=True).expand_as(w)))
+            assert torch.equal(total, h)
+            assert float(((got.cpu().double() - want).abs() - bound).max()) <= 0
+            assert layer(h).shape == h.shape
+            state = layer.start(2, DEV, torch.bfloat16)
+            assert torch.isfinite(layer.step(h[0], state)).all()
+    out = layer(h)                                         # with gradients recorded the 16-bit projection runs
+    assert out.requires_grad
+    with pytest.raises(ValueError, match="divisible"):
+        SelectiveLayer(1, 4, 24, 0.0).serve_e4m3()
+
+
+def test_stack_steps_equal_the_stack():
+    torch.manual_seed(9)
+    stack = SelectiveStack(2, 2, 16, 32, 0.0).to(DEV)
+    h = torch.randn(9, 3, 32, generator=torch.Generator().manual_seed(10)).to(DEV)
+    with torch.no_grad():
+        whole, _ = stack(h)
+        states = [layer.start(3, DEV) for layer in stack.layers]
+        steps = torch.stack([stack.step(h[t], states) for t in range(9)])
+    close(steps, whole, "steps")
