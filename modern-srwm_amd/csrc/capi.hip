@@ -137,7 +137,7 @@ int conv_dims(int N, int H, int L, int E, int W) {
 }
 int norm_dims(int rows, int D) {
     if (rows <= 0 || D <= 0) return SRWM_EINVAL;
-    return rows > kMaxGrid ? SRWM_ESIZE : SRWM_OK;
+    return (D <= 2048 ? (rows + (int64_t)3) / 4 : rows) > kMaxGrid ? SRWM_ESIZE : SRWM_OK;   // a wave or a workgroup per row
 }
 
 int scan_forward(const void *u, const int64_t *us, const void *delta, const int64_t *ds, const void *z, const int64_t *zs,

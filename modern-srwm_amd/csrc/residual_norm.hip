@@ -90,7 +90,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormParams p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) y[i] = v[i] * rstd * w[i];
     };
-    float inv = 1.f;
+    float inv = 1.f, lift = 1.f;
     if constexpr (E4M3) {
         float top = 0.f;
         auto look = [&](int d, const float (&v)[V]) {
@@ -112,8 +112,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormParams p) {
             }
         }
         top = row_reduce<TPR, OpMax>(top, lds);
-        const float scale = top > 0.f ? top / kE4m3Max : 1.f;
-        inv = 1.f / scale;
+        // a scale whose reciprocal would overflow is lifted first, one that would round to zero is the smallest number
+        const float scale = top > 0.f ? fmaxf(top / kE4m3Max, 1.4e-45f) : 1.f;
+        lift = scale < 1e-30f ? 0x1p64f : 1.f;
+        inv = 1.f / (scale * lift);
         if (lane == 0) p.scale[row] = scale;
     }
     auto write = [&](int d, const float (&v)[V]) {
@@ -121,7 +123,7 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormParams p) {
         normed(d, v, y);
         if constexpr (E4M3) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) y[i] *= inv;
+            for (int i = 0; i < V; ++i) y[i] = y[i] * lift * inv;
             store_e4m3<V>((uint8_t *)p.out + base + d, y);
         } else {
             store_vec<V>((TX *)p.out + base + d, y);

@@ -137,7 +137,10 @@ struct ScanBc {
 // The product of decays of a segment with a reset in it: nothing of the state in front passes, not even NaN.  No power
 // of two has these bits.
 constexpr float kDropped = -0.f;
-__device__ __forceinline__ bool dropped(float pr) { return __float_as_uint(pr) == 0x80000000u; }
+// A state of zero passes as zero through decays whose product overflows.
+__device__ __forceinline__ float carried(float decay, float x, float result) {
+    return __float_as_uint(decay) == 0x80000000u || x == 0.f ? result : fmaf(decay, x, result);
+}
 
 // Whether a workgroup's lanes lie 2 GiB or more apart in rows of these strides (64 channels, 16 steps).
 inline bool scan_span(const ScanParams &p, const Strided3 &s, int64_t bytes) {
@@ -160,7 +163,18 @@ __device__ __forceinline__ void load_states(const float *row, int S, int q, floa
         for (int i = 0; i < SPL; ++i) v[i] = q * SPL + i < S ? row[q * SPL + i] : 0.f;
     }
 }
-// the same from a row of fp32 or bf16 elements that may start anywhere
+// A channel's decays, in units of log2(e).  An infinite one is kept finite, so that the steps behind a row's end (dt = 0)
+// pass the state on there too.
+template <int SPL>
+__device__ __forceinline__ void load_decays(const float *row, int S, int q, float (&v)[SPL]) {
+    load_states<SPL>(row, S, q, v);
+#pragma unroll
+    for (int i = 0; i < SPL; ++i) {
+        const float a = v[i] * kLog2e;
+        v[i] = a < -3e38f ? -3e38f : a > 3e38f ? 3e38f : a;
+    }
+}
+// states (or B, C) from a row of fp32 or bf16 elements that may start anywhere
 template <int SPL, typename T>
 __device__ __forceinline__ void load_io_states(const T *row, int S, int q, float (&v)[SPL]) {
     if (S == 4 * SPL && ((uintptr_t)row & (sizeof(T) * SPL - 1)) == 0 && sizeof(T) * SPL <= 16) {
@@ -208,7 +222,7 @@ __device__ __forceinline__ void join_segments(const ScanParams &p, int64_t at, i
 #pragma unroll
                 for (int s = 0; s < SPL; ++s) {
                     const float d = (&pr[i][s / 4].x)[s % 4], v = (&r[i][s / 4].x)[s % 4];
-                    x[s] = dropped(d) ? v : fmaf(d, x[s], v);
+                    x[s] = carried(d, x[s], v);
                 }
         }
     }
@@ -217,7 +231,7 @@ __device__ __forceinline__ void join_segments(const ScanParams &p, int64_t at, i
         load_states<SPL>(p.seg_decay + at + k * stride, S, q, pr);
         load_states<SPL>(p.seg_state + at + k * stride, S, q, r);
 #pragma unroll
-        for (int s = 0; s < SPL; ++s) x[s] = dropped(pr[s]) ? r[s] : fmaf(pr[s], x[s], r[s]);
+        for (int s = 0; s < SPL; ++s) x[s] = carried(pr[s], x[s], r[s]);
     }
 }
 

@@ -25,9 +25,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     const int64_t states = (int64_t)w.d * S;   // this channel's row in [H*E, S]
 
     float A2[SPL], h[SPL], total = 0.f;
-    load_states<SPL>(p.A + states, S, w.q, A2);
+    load_decays<SPL>(p.A + states, S, w.q, A2);
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, h[s] = 0.f;
+    for (int s = 0; s < SPL; ++s) h[s] = 0.f;
     bool alive = true;   // no reset in this segment so far
 
     T ru[4], rd[4], rz[4], rb[Bc::kEach], rc[Bc::kEach];   // the next block as it lies in memory
@@ -193,10 +193,8 @@ __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanParams p) {
         load_io_states<SPL>((const T *)p.C + n * p.Cs.n + w.g * p.Cs.h, S, w.q, c[r]);
         reset[r] = p.keep && is_reset(p.keep[n]);
     }
-    load_states<SPL>(p.A + states, S, w.q, A2);
+    load_decays<SPL>(p.A + states, S, w.q, A2);
     const float bias = p.bias ? p.bias[w.d] : 0.f, Dc = p.D ? p.D[w.d] : 0.f;
-#pragma unroll
-    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e;
 #pragma unroll
     for (int r = 0; r < RN; ++r) {
         float d = dt[r] + bias, sig, y = 0.f;

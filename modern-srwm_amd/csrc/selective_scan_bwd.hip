@@ -63,9 +63,9 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
     const bool gate = p.z != nullptr;
     const float bias = p.bias ? p.bias[w.d] : 0.f;
     float A2[SPL], gh[SPL], total = 0.f;
-    load_states<SPL>(p.A + states, S, w.q, A2);
+    load_decays<SPL>(p.A + states, S, w.q, A2);
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, gh[s] = 0.f;
+    for (int s = 0; s < SPL; ++s) gh[s] = 0.f;
     bool alive = true;
 
     T rd[4], rz[4], rg[4], rb[Bc::kEach], rc[Bc::kEach];
@@ -169,9 +169,9 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
     float *part = b.part_bc + (((int64_t)w.tile * p.N + w.n) * p.G + w.g) * p.L * 2 * S;
 
     float A2[SPL], gh[SPL], gA[SPL];
-    load_states<SPL>(p.A + states, S, w.q, A2);
+    load_decays<SPL>(p.A + states, S, w.q, A2);
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) A2[s] *= kLog2e, gh[s] = 0.f, gA[s] = 0.f;
+    for (int s = 0; s < SPL; ++s) gh[s] = 0.f, gA[s] = 0.f;
     float gDsum = 0.f, gbsum = 0.f;
 
     T ru[4], rd[4], rz[4], rg[4], rb[Bc::kEach], rc[Bc::kEach];   // the next block as it lies in memory

@@ -127,3 +127,18 @@ def test_norm_of_many_rows_and_leading_axes():
         check(a, b, n)
     again = torch.autograd.grad(residual_rms_norm(*leaves)[0], leaves, go.to(DEV))
     assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("size", [1e-20, 1e-36, 1e-40, 3e-44])
+def test_eight_bit_rows_of_tiny_numbers(size):
+    """Values down to the smallest numbers of float32 still fill the type's range; nothing turns into infinity or NaN."""
+    x = torch.zeros(2, 64)
+    x[0] = torch.linspace(-1, 1, 64) * size * 1e-3
+    x[1] = torch.linspace(-1, 1, 64)
+    w = torch.full((64,), 1.0)
+    o, scale, _ = residual_rms_norm_e4m3(x.to(DEV), None, w.to(DEV))
+    o, scale = o.cpu().float(), scale.cpu()
+    assert torch.isfinite(o).all() and torch.isfinite(scale).all() and float(scale.min()) > 0
+    assert float(o[1].abs().max()) == 448.0
+    y = x[0].double() / (1e-5 ** 0.5)                           # the row's mean square vanishes next to eps
+    assert float((o[0].double() * scale[0].double() - y).abs().max()) <= float(y.abs().max()) * 2.0 ** -4 + 2 * 1.4e-45

@@ -123,9 +123,11 @@ def test_scan_step_sizes_from_tiny_to_large():
     assert float((ratio[:, :, :14] - 1).abs().max()) < 1e-4    # tiny steps: the gradient is relative to themselves
 
 
-@pytest.mark.parametrize("N,H,L,E,S,G", [(1, 1, 700, 96, 16, 1), (2, 2, 333, 40, 8, 1)])
-def test_scan_long_rows(N, H, L, E, S, G):
-    got, want = run_scan(*scan_case(N, H, L, E, S, G, keep=True, lengths=[L, L - 100][:N]))
+@pytest.mark.parametrize("N,H,L,E,S,G", [(1, 1, 700, 96, 16, 1), (2, 2, 333, 40, 8, 1), (1, 2, 401, 9, 33, 2), (1, 1, 1500, 3, 16, 1)])
+@pytest.mark.parametrize("keep", [False, True])
+def test_scan_long_rows(N, H, L, E, S, G, keep):
+    """Rows that are cut into segments, with and without resets, one of them ending inside a segment in the middle."""
+    got, want = run_scan(*scan_case(N, H, L, E, S, G, keep=keep, lengths=[L, L - 100][:N]))
     for k in want:
         check(got[k], want[k], k)
 
@@ -158,6 +160,22 @@ def test_nan_passes_where_it_is_not_masked():
     out, last = selective_scan(**a)
     nan = torch.isnan(out[0, 0])
     assert nan[3:, 2].all() and not nan[:, [0, 1, 3]].any() and not nan[:3].any() and torch.isnan(last[0, 0, 2]).all()
+
+
+def test_infinite_decays_and_overflowing_products():
+    """A = -inf forgets at once, in rows of any length; a state of zero stays zero where the decays' product overflows."""
+    L = 75
+    a, m, go, gl = scan_case(2, 1, L, 4, 16, 1, state=True, lengths=[L, 37])
+    a["A"][:, 1] = float("-inf")
+    fast = {**a, "A": torch.where(torch.isinf(a["A"]), torch.full_like(a["A"], -1e30), a["A"])}
+    got = selective_scan(**{k: place(v) for k, v in a.items()}, lengths=m["lengths"].to(DEV))
+    want = selective.scan(**{k: v.double() for k, v in fast.items()}, lengths=m["lengths"])
+    check(got[0], want[0], "out")
+    check(got[1], want[1], "last")
+    u = torch.zeros(1, 1, 4000, 4, device=DEV)
+    B = torch.ones(1, 1, 4000, 16, device=DEV)
+    out, last = selective_scan(u, torch.ones_like(u), torch.ones(1, 4, 16, device=DEV), B, B)     # decays of e a step
+    assert not out.any() and not last.any()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])

@@ -77,7 +77,7 @@ def test_conv_and_norm_argument_validation():
     norm = lambda x=fake(), s=fake(), e=eps, rows=4, D=8, flags=0: L.residual_rms_norm_forward_bf16(
         x, fake(), fake(), fake(), s, P(None), e, rows, D, flags, P(None))
     assert norm(x=P(None)) == -1 and norm(s=P(None)) == -1 and norm(e=None) == -1 and norm(rows=0) == -1 and norm(D=0) == -1
-    assert norm(flags=2) == -1 and norm(rows=(1 << 23) + 1) == -2
+    assert norm(flags=2) == -1 and norm(rows=(1 << 25) + 1) == -2 and norm(rows=(1 << 23) + 1, D=2049) == -2
     assert L.residual_rms_norm_e4m3_f32(fake(), P(None), fake(), fake(), P(None), P(None), eps, 4, 8, 0, P(None)) == -1
     nb = lambda D: L.residual_rms_norm_backward_f32(fake(), fake(), fake(), fake(), P(None), fake(), P(None), fake(), fake(), 4, D,
                                                     1, P(None))
