@@ -132,6 +132,24 @@ def test_scan_long_rows(N, H, L, E, S, G, keep):
         check(got[k], want[k], k)
 
 
+# calls that fill a quarter of the device and more: few segments, tiles of channels that end inside a group
+WIDE = [(2, 1, 37, 2048, 16, 1), (4, 2, 50, 600, 20, 2), (3, 1, 33, 1500, 32, 1), (9, 8, 20, 40, 64, 4), (16, 1, 97, 203, 9, 1)]
+
+
+@pytest.mark.parametrize("shape", WIDE, ids=str)
+@pytest.mark.parametrize("options", [dict(), dict(keep=True, gate=False, state=False), dict(ragged=True, keep=True, order="offset"),
+                                     dict(D=False, bias=False, order="dense")], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_scan_of_many_channels(shape, options, dtype):
+    options = dict(options)
+    N, L = shape[0], shape[2]
+    if options.pop("ragged", False):
+        options["lengths"] = [L, 0, 1, 17, L - 1, 16][:N] + [L] * (N - 6)
+    got, want = run_scan(*scan_case(*shape, dtype=dtype, **options))
+    for k in want:
+        check(got[k], want[k], k)
+
+
 def test_masked_places_may_hold_anything():
     """NaN behind a row's length and in a state that a reset drops change nothing and reach no result."""
     a, m, go, gl = scan_case(2, 2, 21, 6, 16, 1, lengths=[21, 9])
