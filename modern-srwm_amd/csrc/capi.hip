@@ -156,6 +156,7 @@ int scan_forward(const void *u, const int64_t *us, const void *delta, const int6
                  out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS, 1, L, nullptr, nullptr};
     if (!step) {
         p.segments = scan_segments(N, H, L, E, G, false, &p.seg_len);
+        if (p.segments > 1 && lengths) ++p.segments;   // see scan_run
         if (p.segments > 1 && !workspace) return SRWM_EINVAL;
         p.seg_decay = workspace;
         p.seg_state = workspace + scan_segment_floats(N, H, E, S, p.segments);
@@ -187,6 +188,7 @@ int scan_backward(const void *u, const int64_t *us, const void *delta, const int
                      nullptr, {}, nullptr, const_cast<float *>(saved), N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS,
                      1, L, nullptr, nullptr};
     b.f.segments = scan_segments(N, H, L, E, G, true, &b.f.seg_len);
+    if (b.f.segments > 1 && lengths) ++b.f.segments;   // see scan_run
     b.go = go, b.gos = s3(gos), b.glast = glast;
     b.gu = gu, b.gus = s3(gus), b.gdelta = gdelta, b.gds = s3(gds), b.gz = z ? gz : nullptr, b.gzs = s3(z ? gzs : nullptr);
     b.gB = gB, b.gBs = s3(gBs), b.gC = gC, b.gCs = s3(gCs);
@@ -716,7 +718,8 @@ int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int 
     if (!floats) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
     int len;
-    const int segments = scan_segments(N, H, L, E, G, backward != 0, &len);
+    int segments = scan_segments(N, H, L, E, G, backward != 0, &len);
+    if (segments > 1) ++segments;   // one more where the rows' lengths differ
     floats[0] = 2 * scan_segment_floats(N, H, E, S, segments);
     if (backward)
         floats[0] += (int64_t)N * segments * scan_part_a_row((int64_t)H * E, S) + scan_tiles(H, E, G) * N * G * L * 2 * S;

@@ -56,9 +56,9 @@ struct ScanLane {
     int q, lane, wave;
     bool on;              // false: a lane behind the group's last channel (reads the last one, writes nothing)
 };
-__device__ __forceinline__ ScanLane scan_lane(const ScanParams &p) {
+__device__ __forceinline__ ScanLane scan_lane(const ScanParams &p, int n) {
     ScanLane r;
-    r.n = blockIdx.x % p.N, r.tile = blockIdx.x / p.N, r.g = blockIdx.y;
+    r.n = n, r.tile = blockIdx.x / p.N, r.g = blockIdx.y;
     r.lane = threadIdx.x & 63;
     r.wave = threadIdx.x >> 6;
     r.q = r.lane & 3;
@@ -74,6 +74,71 @@ __device__ __forceinline__ ScanLane scan_lane(const ScanParams &p) {
 }
 __device__ __forceinline__ int row_length(const ScanParams &p, int n) {
     return p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
+}
+
+// A workgroup's run of steps: segment `seg` of the `count` that row n is cut into, steps [tbeg, tend); the segments'
+// results stand side by side from slot `first` on.
+struct ScanRun {
+    int n, len, seg, count, tbeg, tend;   // len: steps of the row
+    int64_t first;
+    bool used;
+};
+// Rows of one length: every row has p.segments segments.  Rows of different lengths: the segments are of one length over
+// all rows, so that no workgroup of a short row stands idle beside those of a long one; (slots - N) of them cover all steps,
+// and N more what is left over at the rows' ends.  Every wave works this out for itself (n, seg: the workgroup's place).
+__device__ __forceinline__ ScanRun scan_run(const ScanParams &p, int n, int seg) {
+    ScanRun r;
+    r.used = true;
+    if (!p.lengths || p.segments == 1) {
+        r.n = n, r.seg = seg, r.count = p.segments, r.len = row_length(p, n);
+        r.first = (int64_t)n * p.segments;
+        r.tbeg = seg * p.seg_len, r.tend = min(r.tbeg + p.seg_len, r.len);
+        return r;
+    }
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    for (int b = 0; b < p.N; b += 64) {
+        int v = b + lane < p.N ? row_length(p, b + lane) : 0;
+        int64_t s = v;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor((long long)s, off, kWave);
+        total += s;
+    }
+    const int64_t slots = (int64_t)p.N * p.segments - p.N;
+    int64_t sl = (total + slots - 1) / slots;
+    sl = (sl + kScanBlock - 1) / kScanBlock * kScanBlock;
+    const int seg_len = __builtin_amdgcn_readfirstlane(sl > 0 ? (int)sl : kScanBlock);   // the same in every lane: in a scalar register
+    int at = seg * p.N + n;
+    r.used = false, r.n = 0, r.seg = 0, r.count = 1, r.len = 0, r.first = 0, r.tbeg = 0, r.tend = 0;
+    int64_t before = 0;   // slots of the rows in front of this batch of 64
+    for (int b = 0; b < p.N && !r.used; b += 64) {
+        const int v = b + lane < p.N ? row_length(p, b + lane) : 0;
+        const int c = b + lane < p.N ? max((v + seg_len - 1) / seg_len, 1) : 0;
+        int incl = c;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int t = __shfl_up(incl, off, kWave);
+            incl += lane >= off ? t : 0;
+        }
+        const unsigned long long hit = __ballot(incl > at - before);
+        if (hit) {
+            const int f = __ffsll((long long)hit) - 1;
+            r.used = true;
+            r.n = b + f;
+            r.count = __builtin_amdgcn_readlane(c, f);
+            r.len = __builtin_amdgcn_readlane(v, f);
+            r.first = before + __builtin_amdgcn_readlane(incl, f) - r.count;
+            r.seg = (int)(at - r.first);
+            r.tbeg = r.seg * seg_len, r.tend = min(r.tbeg + seg_len, r.len);
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return r;
+}
+// The share of the steps behind a row's end that a segment fills with zeros.
+__device__ __forceinline__ void behind_share(const ScanParams &p, const ScanRun &r, int &from, int &to) {
+    const int each = (p.L - r.len + r.count - 1) / r.count;
+    from = min(r.len + r.seg * each, p.L), to = min(from + each, p.L);
 }
 
 // Elements (t, channel) of a strided [N,H,L,E] tensor as one address per workgroup and step (scalar registers) plus one

@@ -13,9 +13,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     constexpr int SP = 4 * SPL;
     using Bc = ScanBc<T, SPL>;
     __shared__ float bc[2][2][kScanBlock][SP];   // [buffer][B | C][step][state]
-    const ScanLane w = scan_lane(p);
-    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
-    const int seg = blockIdx.z, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);
+    const ScanRun run = scan_run(p, blockIdx.x % p.N, blockIdx.z);
+    if (!run.used || (LOCAL && run.seg == run.count - 1)) return;   // the whole workgroup; a row's last result is not needed
+    const ScanLane w = scan_lane(p, run.n);
+    const int S = p.S, D = p.H * p.E, tbeg = run.tbeg, tend = run.tend;
 
     ScanRows<const T, OFF> u(p.u, p.us, w, tbeg), dl(p.delta, p.ds, w, tbeg), z(p.z, p.zs, w, tbeg);
     ScanRows<T, OFF> out(p.out, p.os, w, tbeg);
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     if constexpr (!LOCAL) {
         if (p.state) load_states<SPL>(p.state + w.n * (int64_t)D * S + states, S, w.q, h);
         const int64_t stride = (int64_t)D * S;
-        join_segments<SPL>(p, (int64_t)w.n * p.segments * stride + states, stride, seg, S, w.q, h);   // the segments in front
+        join_segments<SPL>(p, run.first * stride + states, stride, run.seg, S, w.q, h);   // the segments in front
     }
     float *saved = nullptr;
     if (!LOCAL && p.saved)
@@ -133,25 +134,25 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     if (!w.on) return;
     if constexpr (LOCAL) {
         total = group_sum<4>(total);
-        const int64_t at = ((int64_t)w.n * p.segments + seg) * D * S + states;
+        const int64_t at = (run.first + run.seg) * D * S + states;
 #pragma unroll
         for (int s = 0; s < SPL; ++s) A2[s] = alive ? __builtin_amdgcn_exp2f(total * A2[s]) : kDropped;
         store_states<SPL>(p.seg_decay + at, S, w.q, A2);
         store_states<SPL>(p.seg_state + at, S, w.q, h);
     } else {
-        // rows behind the sequence's end, and the last state from the last segment (those behind the end pass it on)
-        const int first = max(tbeg, Ln), behind = min(tbeg + p.seg_len, p.L);
+        if (run.seg == run.count - 1) store_states<SPL>(p.last + w.n * (int64_t)D * S + states, S, w.q, h);
+        int first, behind;   // rows behind the sequence's end
+        behind_share(p, run, first, behind);
         ScanRows<T, OFF> rest(p.out, p.os, w, first);
         for (int t = first; t < behind; t += 4, rest.move(4))
             if (t + w.q < behind) io_store(rest.at(0, w.q), 0.f);
-        if (seg == p.segments - 1) store_states<SPL>(p.last + w.n * (int64_t)D * S + states, S, w.q, h);
     }
 }
 
 template <typename T, int SPL, typename OFF>
 int launch_fwd_as(const ScanParams &p, hipStream_t s) {
     const unsigned tiles = (p.H / p.G * p.E + kScanTile - 1) / kScanTile;
-    const dim3 grid(tiles * p.N, p.G, p.segments), before(tiles * p.N, p.G, p.segments - 1);
+    const dim3 grid(tiles * p.N, p.G, p.segments), before(tiles * p.N, p.G, p.lengths ? p.segments : p.segments - 1);
     if (p.segments > 1) {
         if (p.keep) scan_fwd_kernel<T, SPL, true, true, OFF><<<before, kScanThreads, 0, s>>>(p);
         else scan_fwd_kernel<T, SPL, false, true, OFF><<<before, kScanThreads, 0, s>>>(p);
@@ -176,7 +177,7 @@ template <typename T, int SPL, int RN>
 __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanParams p) {
     ScanParams at = p;
     at.N = (p.N + RN - 1) / RN;
-    const ScanLane w = scan_lane(at);
+    const ScanLane w = scan_lane(at, blockIdx.x % at.N);
     if (!w.on) return;
     const int S = p.S, n0 = w.n * RN;
     const int64_t D = (int64_t)p.H * p.E, states = (int64_t)w.d * S;

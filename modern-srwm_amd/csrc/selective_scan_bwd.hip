@@ -53,9 +53,11 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
     using Bc = ScanBc<T, SPL>;
     __shared__ float bc[2][2][kScanBlock][SP];
     const ScanParams &p = b.f;
-    const ScanLane w = scan_lane(p);
-    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
-    const int seg = blockIdx.z + 1, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);   // the first is never needed
+    // a row's first result is never needed
+    const ScanRun run = scan_run(p, blockIdx.x % p.N, p.lengths ? blockIdx.z : blockIdx.z + 1);
+    if (!run.used || run.seg == 0) return;   // the whole workgroup
+    const ScanLane w = scan_lane(p, run.n);
+    const int S = p.S, D = p.H * p.E, tbeg = run.tbeg, tend = run.tend;
     const int64_t states = (int64_t)w.d * S;
     const int last = tbeg + max(tend - tbeg - 1, 0) / kScanBlock * kScanBlock;   // first step of the last block
     ScanRows<const T, OFF> dl(p.delta, p.ds, w, last), z(p.z, p.zs, w, last), go(b.go, b.gos, w, last);
@@ -134,7 +136,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
     }
     if (!w.on) return;
     total = group_sum<4>(total);
-    const int64_t at = ((int64_t)w.n * p.segments + seg) * D * S + states;
+    const int64_t at = (run.first + run.seg) * D * S + states;
 #pragma unroll
     for (int s = 0; s < SPL; ++s) A2[s] = alive ? __builtin_amdgcn_exp2f(total * A2[s]) : kDropped;
     store_states<SPL>(p.seg_decay + at, S, w.q, A2);
@@ -154,9 +156,9 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
     __shared__ float bc[2][kScanBlock][SP];
     __shared__ float red[4][kScanBlock][2][SP];
     const ScanParams &p = b.f;
-    const ScanLane w = scan_lane(p);
-    const int S = p.S, D = p.H * p.E, Ln = row_length(p, w.n);
-    const int seg = blockIdx.z, tbeg = seg * p.seg_len, tend = min(tbeg + p.seg_len, Ln);
+    const ScanRun run = scan_run(p, blockIdx.x % p.N, blockIdx.z);
+    const ScanLane w = scan_lane(p, run.n);
+    const int S = p.S, D = p.H * p.E, tbeg = run.tbeg, tend = run.tend;
     const int64_t states = (int64_t)w.d * S;
     const int last = tbeg + max(tend - tbeg - 1, 0) / kScanBlock * kScanBlock;   // first step of the last block
 
@@ -196,8 +198,9 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
     if (tbeg < tend) fetch(last, tend - last);
     if (b.glast) load_states<SPL>(b.glast + w.n * (int64_t)D * S + states, S, w.q, gh);
     const int64_t stride = (int64_t)D * S;
-    join_segments<SPL>(p, ((int64_t)w.n * p.segments + p.segments - 1) * stride + states, -stride, p.segments - 1 - seg, S, w.q,
-                       gh);   // the segments behind
+    if (run.used)
+        join_segments<SPL>(p, (run.first + run.count - 1) * stride + states, -stride, run.count - 1 - run.seg, S, w.q,
+                           gh);   // the segments behind
     for (int t0 = last; t0 >= tbeg && tbeg < tend; t0 -= kScanBlock) {
         const int n = tend - t0;   // steps of this block, 16 or more: all
         // what a channel needs once per step: lane q holds the steps 4i + q
@@ -353,15 +356,17 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
     gDsum = group_sum<4>(gDsum);
     gbsum = group_sum<4>(gbsum);
     if (!w.on) return;
-    if (b.gstate && seg == 0) store_states<SPL>(b.gstate + w.n * (int64_t)D * S + states, S, w.q, gh);
-    float *pa = b.part_a + ((int64_t)w.n * p.segments + seg) * scan_part_a_row(D, S);
+    // a share of the sums of gA, gD and gbias from every workgroup, of zeros from one without steps
+    float *pa = b.part_a + ((int64_t)blockIdx.z * p.N + blockIdx.x % p.N) * scan_part_a_row(D, S);
     store_states<SPL>(pa + states, S, w.q, gA);
     if (w.q == 0) {
         pa[(int64_t)D * S + w.d] = gDsum;
         pa[(int64_t)D * (S + 1) + w.d] = gbsum;
     }
-    // rows behind the sequence's end
-    const int first = max(tbeg, Ln), behind = min(tbeg + p.seg_len, p.L);
+    if (!run.used) return;
+    if (b.gstate && run.seg == 0) store_states<SPL>(b.gstate + w.n * (int64_t)D * S + states, S, w.q, gh);
+    int first, behind;   // rows behind the sequence's end
+    behind_share(p, run, first, behind);
     ScanRows<T, OFF> qu(b.gu, b.gus, w, first), qd(b.gdelta, b.gds, w, first), qz(b.gz, b.gzs, w, first);
     for (int t = first; t < behind; t += 4, qu.move(4), qd.move(4), qz.move(4))
         if (t + w.q < behind) {
@@ -420,7 +425,7 @@ template <typename T, int SPL, typename OFF>
 int launch_bwd_as(const ScanBwdParams &b, hipStream_t s) {
     const ScanParams &p = b.f;
     const unsigned tiles = (p.H / p.G * p.E + kScanTile - 1) / kScanTile;
-    const dim3 grid(tiles * p.N, p.G, p.segments), behind(tiles * p.N, p.G, p.segments - 1);
+    const dim3 grid(tiles * p.N, p.G, p.segments), behind(tiles * p.N, p.G, p.lengths ? p.segments : p.segments - 1);
     int r = 0;
     if (p.segments > 1) {
         if (p.keep) scan_bwd_local_kernel<T, SPL, true, OFF><<<behind, kScanThreads, 0, s>>>(b);

@@ -150,6 +150,22 @@ def test_scan_of_many_channels(shape, options, dtype):
         check(got[k], want[k], k)
 
 
+@pytest.mark.parametrize("lengths", [[700, 10, 0], [0, 0, 0], [3, 700, 699], [1, 1, 700], [512, 33, 32]], ids=str)
+def test_segments_of_rows_of_different_lengths(lengths):
+    """The segments are shared out over all rows: long ones get more of them, short and empty ones one."""
+    got, want = run_scan(*scan_case(3, 1, 700, 5, 16, 1, lengths=lengths, keep=True))
+    for k in want:
+        check(got[k], want[k], k)
+
+
+def test_segments_of_many_rows_of_different_lengths():
+    g = torch.Generator().manual_seed(12)
+    lengths = torch.randint(0, 150, (70,), generator=g).tolist()
+    got, want = run_scan(*scan_case(70, 1, 150, 3, 16, 1, lengths=lengths))
+    for k in want:
+        check(got[k], want[k], k)
+
+
 def test_masked_places_may_hold_anything():
     """NaN behind a row's length and in a state that a reset drops change nothing and reach no result."""
     a, m, go, gl = scan_case(2, 2, 21, 6, 16, 1, lengths=[21, 9])
