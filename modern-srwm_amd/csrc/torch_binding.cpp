@@ -130,6 +130,7 @@ ScanSizes scan_sizes(const Tensor &u, const Tensor &A, const Tensor &B, bool ste
                       step ? "u must be (N, H, E), A (H, E, S), B and C (N, G, S)" : "u must be (N, H, L, E), A (H, E, S), B and C (N, G, L, S)");
     const ScanSizes z{u.size(0), u.size(1), step ? 1 : u.size(2), u.size(nd - 1), A.size(2), B.size(1)};
     TORCH_CHECK_VALUE(z.G > 0 && z.H % z.G == 0, "the ", z.H, " heads must divide into the ", z.G, " groups of B and C");
+    TORCH_CHECK_VALUE(z.S > 0, "a channel needs at least one state");
     return z;
 }
 struct ScanIn {   // the inputs, checked and laid out

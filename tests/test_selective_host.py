@@ -99,6 +99,10 @@ def test_host_layer_refusals():
         residual_rms_norm(z(2, 4), None, z(4))
     with pytest.raises(ValueError, match="groups"):
         selective_scan(z(1, 3, 2, 4), z(1, 3, 2, 4), z(3, 4, 16), z(1, 2, 2, 16), z(1, 2, 2, 16))
+    with pytest.raises(ValueError, match="at least one state"):    # its output would be D u silu(z), not zeros
+        selective_scan(z(1, 1, 2, 4), z(1, 1, 2, 4), z(1, 4, 0), z(1, 1, 2, 0), z(1, 1, 2, 0))
+    with pytest.raises(ValueError, match="at least one state"):
+        selective_scan_step(z(1, 1, 4), z(1, 1, 4), z(1, 1, 4, 0), z(1, 4, 0), z(1, 1, 0), z(1, 1, 0))
     with pytest.raises(ValueError, match="N, H, L, E"):
         selective_scan(z(1, 2, 4), z(1, 2, 4), z(1, 4, 16), z(1, 2, 16), z(1, 2, 16))
     with pytest.raises(TypeError, match="float32 or torch.bfloat16"):
