@@ -7,6 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/python.h>
 
@@ -106,6 +107,21 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     for (const Tensor &t : ts)
         if (t.defined() && t.requires_grad()) return true;
     return false;
+}
+
+// What a backward returns.  Where a graph of it is recorded (create_graph), a derivative of these gradients raises instead
+// of counting them as constants.
+variable_list once_differentiable(variable_list g, const char *what) {
+    if (!at::GradMode::is_enabled()) return g;
+    variable_list in;
+    for (const Tensor &t : g)
+        if (t.defined()) in.push_back(t.detach().requires_grad_());
+    const auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", (int64_t)in.size());
+    const variable_list out = (*node)(std::move(in));
+    size_t k = 0;
+    for (Tensor &t : g)
+        if (t.defined()) t = out[k++];
+    return g;
 }
 
 // A tensor that a kernel overwrites: itself where it is dense and aligned, else a copy that is written back.
@@ -259,7 +275,7 @@ struct SelectiveScan : Function<SelectiveScan> {
         const Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
         variable_list g = scan_backward(in, s[10], go, grads[1], ctx->saved_data["softplus"].toBool(), ctx->saved_data["state"].toBool());
         g.resize(12);
-        return g;
+        return once_differentiable(std::move(g), "selective_scan");
     }
 };
 
@@ -398,7 +414,7 @@ struct CausalConv : Function<CausalConv> {
             check_code(in.bf16 ? call(causal_conv_backward_bf16, (uint16_t *)nullptr) : call(causal_conv_backward_f32, (float *)nullptr),
                        "causal_conv_backward");
         }
-        return {gx.t, gw, gb, gs, Tensor(), Tensor(), Tensor()};
+        return once_differentiable({gx.t, gw, gb, gs, Tensor(), Tensor(), Tensor()}, "causal_conv");
     }
 };
 
@@ -534,7 +550,7 @@ struct ResidualRMSNorm : Function<ResidualRMSNorm> {
         } else {
             gw.zero_();
         }
-        return {gx, gr, gw, Tensor()};
+        return once_differentiable({gx, gr, gw, Tensor()}, "residual_rms_norm");
     }
 };
 

@@ -423,6 +423,24 @@ def test_replays_from_a_captured_graph():
             assert torch.equal(x, y), k
 
 
+def test_second_derivatives_are_refused():
+    """With a graph of the gradients recorded they have the same values, and a derivative of them raises."""
+    a, _, go, _ = scan_case(1, 2, 20, 8, 16, 1)
+    d = {k: place(v) for k, v in a.items()}
+    w, b = torch.randn(2, 8, 4, device=DEV), torch.randn(16, device=DEV)
+    calls = {"selective_scan": (lambda t: selective_scan(**{**d, "u": t})[0], d["u"]),
+             "causal_conv": (lambda t: causal_conv(t, w)[0], d["u"]),
+             "residual_rms_norm": (lambda t: residual_rms_norm(t, t, b)[0], torch.randn(5, 16, device=DEV))}
+    for name, (call, t) in calls.items():
+        leaf = t.detach().requires_grad_()
+        out = call(leaf)
+        first, = torch.autograd.grad(out.square().sum(), leaf, create_graph=True)
+        plain, = torch.autograd.grad(call(leaf), leaf, 2 * out.detach())
+        assert torch.equal(first.detach(), plain), name
+        with pytest.raises(RuntimeError, match=name + " has no second derivative"):
+            (call(leaf).sum() + first.square().sum()).backward()       # a penalty on the gradient next to a loss
+
+
 def test_offsets_past_32_bits():
     """Rows whose elements lie further than 2^32 bytes (and 2^31 elements) apart."""
     H, E, S, L = 1, 16, 16, 5
