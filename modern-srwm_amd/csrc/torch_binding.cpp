@@ -109,6 +109,24 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
     return false;
 }
 
+// A captured backward joins the streams of the leaves' gradient accumulators.  One that a live graph outside the capture
+// recorded on the default stream cannot be joined: the process would end inside the backward, so the forward refuses.
+void not_held_outside(const char *what, std::initializer_list<Tensor> ts) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const auto dev = ts.begin()->get_device();
+    if (dev < 0 || hipStreamIsCapturing(c10::hip::getCurrentHIPStream(dev).stream(), &status) != hipSuccess ||
+        status == hipStreamCaptureStatusNone)
+        return;
+    for (const Tensor &t : ts) {
+        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        const auto on = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!on || on->id() != c10::Stream(c10::Stream::DEFAULT, on->device()).id(), what,
+                    ": a stream is being captured while a graph recorded on the default stream still holds the gradient of a leaf of "
+                    "this call; drop that graph and its outputs first, or record it on a side stream");
+    }
+}
+
 // What a backward returns.  Where a graph of it is recorded (create_graph), a derivative of these gradients raises instead
 // of counting them as constants.
 variable_list once_differentiable(variable_list g, const char *what) {
@@ -286,6 +304,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor &u, const Tensor &delta, 
     const Tensor D = or_none(D_), z = or_none(z_), bias = or_none(bias_), state = or_none(state_), keep = or_none(keep_),
                  lengths = or_none(lengths_);
     if (wants_grad({u, delta, A, B, C, D, z, bias, state})) {
+        not_held_outside("selective_scan", {u, delta, A, B, C, D, z, bias, state});
         const variable_list r = SelectiveScan::apply(u, delta, A, B, C, D_, z_, bias_, state_, keep_, lengths_, softplus);
         return {r[0], r[1]};
     }
@@ -422,6 +441,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor &x, const Tensor &weight, co
                                        const MaybeTensor &keep_, const MaybeTensor &lengths_, bool silu) {
     const Tensor bias = or_none(bias_), state = or_none(state_), keep = or_none(keep_), lengths = or_none(lengths_);
     if (wants_grad({x, weight, bias, state})) {
+        not_held_outside("causal_conv", {x, weight, bias, state});
         const variable_list r = CausalConv::apply(x, weight, bias_, state_, keep_, lengths_, silu);
         return {r[0], r[1]};
     }
@@ -559,6 +579,7 @@ std::tuple<Tensor, Tensor> residual_rms_norm(const Tensor &x, const MaybeTensor 
     if (wants_grad({x, residual, weight})) {
         TORCH_CHECK_VALUE(x.dim() == 0 || x.size(-1) <= kNormBackwardMax, "residual_rms_norm has no backward for rows longer than ",
                           kNormBackwardMax);
+        not_held_outside("residual_rms_norm", {x, residual, weight});
         const variable_list r = ResidualRMSNorm::apply(x, residual_, weight, eps);
         return {r[0], residual.defined() ? r[1] : x};
     }

@@ -423,6 +423,46 @@ def test_replays_from_a_captured_graph():
             assert torch.equal(x, y), k
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_capture_is_refused_while_an_eager_graph_holds_the_leaves():
+    """A backward captured then would end the process; the forward raises in front of any launch, and with the eager graph
+    gone the same leaves can be captured."""
+    a, _, go, _ = scan_case(2, 2, 20, 8, 16, 1)
+    d = {k: place(v) for k, v in a.items()}
+    w, b = torch.randn(2, 8, 4, device=DEV), torch.randn(16, device=DEV)
+    calls = {"selective_scan": (lambda t: selective_scan(**{**d, "A": t})[0], d["A"]),
+             "causal_conv": (lambda t: causal_conv(d["u"], t)[0], w),
+             "residual_rms_norm": (lambda t: residual_rms_norm(d["B"], d["C"], t)[0], b)}
+    for name, (call, t) in calls.items():
+        leaf = t.detach().requires_grad_()
+        held = call(leaf)
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=name + ": a stream is being captured"):
+            with torch.cuda.graph(graph):
+                call(leaf)
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(graph):     # without gradients there is nothing to join
+            still = call(leaf)
+        graph.replay()
+        assert torch.equal(still, held), name
+        g = torch.randn_like(held)
+        want, = torch.autograd.grad(held, leaf, g)
+        del held
+        side = torch.cuda.Stream()                         # warm-up, as usual in front of a capture
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call(leaf), leaf, g)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(call(leaf), leaf, g)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
 def test_second_derivatives_are_refused():
     """With a graph of the gradients recorded they have the same values, and a derivative of them raises."""
     a, _, go, _ = scan_case(1, 2, 20, 8, 16, 1)
