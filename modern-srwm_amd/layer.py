@@ -437,7 +437,7 @@ class SelectiveLayer(nn.Module):
         self.D = nn.Parameter(torch.ones(num_head, dim_head))
         self.out_linear = nn.Linear(inner, in_dim, bias=False)
         self.drop = nn.Dropout(dropout)
-        self._eight = None   # the input projection in e4m3, see serve_e4m3
+        self._eight = None   # the input projection in e4m3 and what it was made from, see serve_e4m3
         nn.init.uniform_(self.conv_weight, -d_conv ** -0.5, d_conv ** -0.5)
         # step sizes spread over 1e-3 .. 1e-1 where their projection is zero; decays of 1 .. d_state per unit of time
         first = torch.exp(torch.rand(num_head, dim_head) * math.log(100.) + math.log(1e-3))
@@ -447,13 +447,29 @@ class SelectiveLayer(nn.Module):
 
     def serve_e4m3(self):
         """From here on the projection in front runs in 8 bits wherever no gradient is recorded: its weight is kept as
-        e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16."""
+        e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16.  A
+        weight that is changed in place, loaded, replaced or moved afterwards is converted anew (what is written past the
+        version counter, through .data, is not seen: call serve_e4m3 again)."""
         if self.in_dim % 16 or self.num_head * self.dim_head % 8:
             raise ValueError("the 8-bit projection needs in_dim and 2 * num_head * dim_head divisible by 16")
-        w = self.in_linear.weight.detach().float()
+        weight = self.in_linear.weight
+        w = weight.detach().float()
         scale = w.abs().amax(1, keepdim=True).clamp_min(1e-30) / 448
-        self._eight = ((w / scale).to(torch.float8_e4m3fn), scale.t().contiguous())
+        self._eight = (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous(), self._weight_made_from()
         return self
+
+    def _weight_made_from(self):
+        w = self.in_linear.weight
+        return w, 0 if w.is_inference() else w._version, w.dtype, w.device
+
+    def _weight_e4m3(self):
+        if not self._eight or any(a is not b and (torch.is_tensor(a) or a != b)
+                                  for a, b in zip(self._eight[2], self._weight_made_from())):
+            self.serve_e4m3()
+        return self._eight[:2]
+
+    def __getstate__(self):   # a copy converts its own weight at its first use
+        return {**self.__dict__, "_eight": None if self._eight is None else ()}
 
     def _project_in(self, h, residual):
         """Norm and input projection: ([x | z] rows (..., 2 * inner), the residual stream with h added)."""
@@ -462,7 +478,7 @@ class SelectiveLayer(nn.Module):
             y, total = residual_rms_norm(h, residual, weight, self.eps)
             return self.in_linear(y.to(self.in_linear.weight.dtype)), total
         y, scale, total = residual_rms_norm_e4m3(h, residual, weight, self.eps)
-        w, w_scale = self._eight
+        w, w_scale = self._weight_e4m3()
         rows = torch._scaled_mm(y.reshape(-1, self.in_dim), w.t(), scale_a=scale.reshape(-1, 1), scale_b=w_scale,
                                 out_dtype=torch.bfloat16)
         return rows.to(h.dtype).view(*h.shape[:-1], -1), total

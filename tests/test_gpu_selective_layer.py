@@ -3,6 +3,8 @@ their forms (segments, unrolls, single tokens, padded batches, 8-bit projection)
 
 Tolerance of the float32 layers: each of the seven operators in a row (norm, four projections, convolution, scan) holds
 1e-5 of its largest value, so a result and its gradients hold 1e-4."""
+import copy
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -155,6 +157,37 @@ def test_eight_bit_projection():
     assert out.requires_grad
     with pytest.raises(ValueError, match="divisible"):
         SelectiveLayer(1, 4, 24, 0.0).serve_e4m3()
+
+
+def test_eight_bit_projection_follows_its_weight():
+    """A weight that is stepped, loaded, replaced, converted or copied is not served from its old 8-bit form."""
+    fresh = lambda layer: SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(layer.in_linear.weight.dtype)
+    h = torch.randn(5, 2, 32, generator=torch.Generator().manual_seed(3)).to(DEV)
+
+    @torch.no_grad()
+    def served_as_it_is(layer, name):
+        x = h.to(layer.in_linear.weight.dtype)
+        other = fresh(layer)
+        other.load_state_dict(layer.state_dict())
+        assert torch.equal(layer(x), other.serve_e4m3()(x)), name
+    torch.manual_seed(12)
+    layer = SelectiveLayer(2, 16, 32, 0.0).to(DEV).serve_e4m3()
+    served_as_it_is(layer, "as made")
+    opt = torch.optim.SGD(layer.parameters(), lr=0.1)
+    layer(h).square().sum().backward()
+    opt.step()
+    served_as_it_is(layer, "stepped")
+    layer.load_state_dict(fresh(layer).state_dict())
+    served_as_it_is(layer, "loaded")
+    layer.in_linear.weight = torch.nn.Parameter(torch.randn_like(layer.in_linear.weight))
+    served_as_it_is(layer, "replaced")
+    twin = copy.deepcopy(layer)
+    with torch.no_grad():
+        twin.in_linear.weight.mul_(-0.5)
+    served_as_it_is(twin, "copied and changed")
+    served_as_it_is(layer, "the copy's origin")
+    served_as_it_is(layer.to(torch.bfloat16), "converted")
+    served_as_it_is(SelectiveLayer(2, 16, 32, 0.0).serve_e4m3().to(DEV), "moved")
 
 
 def test_stack_steps_equal_the_stack():
