@@ -537,7 +537,8 @@ SRWM_API int delta_layer_prologue_grad_bf16(const uint16_t *gq, const int64_t gq
  *   saved              dense [N, ceil(L/16), H*E, S]: states for the backward, or NULL
  *   workspace          selective_scan_workspace(.., backward = 0) floats, contents ignored (NULL where that is 0).  Two
  *                      calls that may overlap need one each; a captured graph keeps its own
- * S up to 64 (SRWM_ESIZE beyond).  A, state, last, saved, workspace and their gradients start at multiples of 16 bytes.
+ * S up to 64, H*E up to 2^30, N * ceil(H*E / (64 G)) up to 2^23, in the backward N*G*L*S up to 2^30 (SRWM_ESIZE beyond);
+ * no output overlaps an input or another output.  A, state, last, saved, workspace and their gradients start at multiples of 16 bytes.
  * Arithmetic, states and the sums are fp32.
  */
 SRWM_API int selective_scan_forward_f32(const float *u, const int64_t u_strides[3], const float *delta,
@@ -609,7 +610,8 @@ SRWM_API int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides
  *   last       the same behind the last step
  *   keep, lengths as above; inputs before a reset count as zero, in out and in last
  * Backward: grad_x strided [N,H,L,E], grad_last / grad_state like state (either may be NULL), grad_weight [H,E,W] and
- * grad_bias [H,E] (or NULL) fp32; workspace: causal_conv_workspace() floats.  Step: state overwritten in place.
+ * grad_bias [H,E] (or NULL) fp32; workspace: causal_conv_workspace() floats.  H*E up to 2^20, N * ceil(L / 128) up to 2^23
+ * (SRWM_ESIZE beyond); no output overlaps an input.  Step: state overwritten in place.
  */
 SRWM_API int causal_conv_forward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
                              const float *state, const float *keep, const int *lengths, float *out,
@@ -647,8 +649,9 @@ SRWM_API int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E
  * residual_rms_norm_e4m3_*: out holds e4m3 (OCP) bytes of the result divided by scale[row] = max|result| / 448 of the row
  * (1 for a row of zeros), rounded to nearest even.
  * Backward: `sum` is what was normalised, as stored (x without a residual); grad_x like x, grad_residual and grad_sum like
- * sum (either may be NULL) -- both gradients have the same values; grad_weight [D];  D up to 16384 (SRWM_ESIZE beyond);
- * workspace: residual_rms_norm_workspace() floats.
+ * sum (either may be NULL) -- both gradients have the same values; grad_weight [D];  D up to 16384 (SRWM_ESIZE beyond).
+ * Up to 2^25 rows of 2048 elements, 2^23 longer ones; no output overlaps an input.
+ * Workspace: residual_rms_norm_workspace() floats.
  */
 SRWM_API int residual_rms_norm_forward_f32(const float *x, const void *residual, const float *weight, float *out, void *sum,
                              float *rstd, const float eps[1], int rows, int D, unsigned flags, void *stream);

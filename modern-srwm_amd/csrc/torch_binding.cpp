@@ -29,6 +29,7 @@ using MaybeTensor = std::optional<Tensor>;   // autograd's Function takes absent
 Tensor or_none(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
 
 void check_code(int code, const char *what) {
+    TORCH_CHECK(code != SRWM_ESIZE, what, ": sizes beyond what the kernels take");
     TORCH_CHECK(code == 0, what, " failed with code ", code, ": ", srwm_hip_strerror(code));
 }
 

@@ -13,14 +13,12 @@ norm's result; it has no backward.  Rows longer than 16384 have no backward eith
 """
 import srwm_hip
 
-_ops = srwm_hip.binding()
-
 
 def residual_rms_norm(x, residual, weight, eps=1e-5):
     """(out, total); see the module's text."""
-    return _ops.residual_rms_norm(x, residual, weight, eps)
+    return srwm_hip.binding().residual_rms_norm(x, residual, weight, eps)
 
 
 def residual_rms_norm_e4m3(x, residual, weight, eps=1e-5):
     """(out, scale, total) with out in torch.float8_e4m3fn and one scale per row; see the module's text.  No backward."""
-    return _ops.residual_rms_norm_e4m3(x, residual, weight, eps)
+    return srwm_hip.binding().residual_rms_norm_e4m3(x, residual, weight, eps)

@@ -30,26 +30,24 @@ Gradients go to every float tensor, through `last` and into `state` as well; kee
 """
 import srwm_hip
 
-_ops = srwm_hip.binding()
-
 
 def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, state=None, keep=None, lengths=None, softplus=True):
     """The scan over whole sequences: (out, last).  See the module's text.  softplus=False: dt = delta + delta_bias."""
-    return _ops.selective_scan(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus)
+    return srwm_hip.binding().selective_scan(u, delta, A, B, C, D, z, delta_bias, state, keep, lengths, softplus)
 
 
 def selective_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, keep=None, softplus=True):
     """One token: u, delta, z (N, H, E), B and C (N, G, S), keep (N,).  state is OVERWRITTEN; returns out (N, H, E).
     There is no backward: the call raises where a gradient would be asked of it."""
-    return _ops.selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus)
+    return srwm_hip.binding().selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, keep, softplus)
 
 
 def causal_conv(x, weight, bias=None, state=None, keep=None, lengths=None, silu=True):
     """Short causal depthwise convolution over whole sequences: (out, last).  silu=False: no activation behind it."""
-    return _ops.causal_conv(x, weight, bias, state, keep, lengths, silu)
+    return srwm_hip.binding().causal_conv(x, weight, bias, state, keep, lengths, silu)
 
 
 def causal_conv_step(x, state, weight, bias=None, keep=None, silu=True):
     """One token: x (N, H, E), keep (N,).  state (N, H, W-1, E) is OVERWRITTEN; returns out (N, H, E).  No backward: the
     call raises where a gradient would be asked of it."""
-    return _ops.causal_conv_step(x, state, weight, bias, keep, silu)
+    return srwm_hip.binding().causal_conv_step(x, state, weight, bias, keep, silu)

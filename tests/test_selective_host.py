@@ -1,6 +1,9 @@
 """What the selective-scan, convolution and norm operators refuse, checked without a GPU: the C entry points reject bad
 arguments before they touch the device (placeholder pointers are never dereferenced), the host layer before it calls them."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -130,3 +133,14 @@ def test_output_rows_follow_the_input():
     assert out.permute(2, 0, 1, 3).is_contiguous()                                     # step-major, dense
     assert srwm_hip.rows_like(torch.zeros(3, 2, 5, 8)[..., ::2]).stride(-1) == 1
     assert srwm_hip.rows_like(torch.zeros(3, 2, 4, 5).transpose(2, 3)).stride(-1) == 1
+
+
+def test_binding_is_loaded_at_the_first_call():
+    """Importing the layers asks for no library: a missing binding raises where one of its operators is called."""
+    code = ("import sys; sys.path.insert(0, 'modern-srwm_amd'); import srwm_hip; srwm_hip.BINDING_PATH = '/nonexistent.so'\n"
+            "import torch, layer, residual_norm\n"
+            "try: residual_norm.residual_rms_norm(torch.zeros(2, 4), None, torch.zeros(4))\n"
+            "except RuntimeError as e: assert 'is missing' in str(e), e\n"
+            "else: raise AssertionError('no error')\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], cwd=root, check=True, timeout=100)
