@@ -264,8 +264,7 @@ __device__ __forceinline__ void store_states(float *row, int S, int q, const flo
 
 // Carries a state (or its gradient) over `count` segments from the one at `at` on, `stride` floats from one to the next:
 // x = decay x + result.  Four segments are asked for at a time (two above 16 states; eight take the forward from five to
-// three waves a SIMD): one after the
-// other would cost a trip to memory each, as they were written by other dies.
+// three waves a SIMD): one after the other would cost a trip to memory each, as they were written by other dies.
 template <int SPL>
 __device__ __forceinline__ void join_segments(const ScanParams &p, int64_t at, int64_t stride, int count, int S, int q, float (&x)[SPL]) {
     constexpr int U = SPL <= 4 ? 4 : 2;

@@ -8,6 +8,11 @@ namespace {
 // LOCAL: from a zero state, for nothing but the segment's last state and its product of decays.  Otherwise the state
 // comes from the call's state and the segments in front of this one, and the outputs are formed.
 // The inputs of a block are fetched while the block before is computed.
+// Bound by the number of vector instructions (busy 86 - 90 % of the time, LDS 4 %): per state and step a multiplication, an
+// exponential (twice the cycles of the others) and three more are needed, six of 4 cycles a wave; 8.4 are issued with
+// outputs (softplus, gate, conversions, hand-overs between lanes), 5.7 without.  4 x 2048 steps x 2048 channels x 16
+// states, bf16: 60 us (LOCAL) + 91 us, 211 MB read and written by the second; two rows of 12 001 and 8 001 steps: 148 + 217.
+// 16 lanes to a channel, which needs no segments, took 667 us for the latter.
 template <typename T, int SPL, bool KEEP, bool LOCAL, typename OFF>
 __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     constexpr int SP = 4 * SPL;
@@ -171,8 +176,8 @@ int launch_fwd(const ScanParams &p, hipStream_t s) {
 }
 
 // One token: a lane updates SPL states of a channel in place, for RN batch rows whose states are all asked for before the
-// first is used (A, D and the bias are read once for them).  Bound by the states' memory traffic for many rows, by
-// latency for few.
+// first is used (A, D and the bias are read once for them).  Bound by the states' memory traffic for many rows (256 rows x
+// 2048 channels x 16 states: 71 MB in 18 us, 3.9 TB/s; one row a thread 23.7 us), by latency for few (one row: 3.5 us).
 template <typename T, int SPL, int RN>
 __global__ __launch_bounds__(kScanThreads) void scan_step_kernel(ScanParams p) {
     ScanParams at = p;
