@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
             for (int s = 0; s < SPL; ++s) hs[0][s] = h[s];
 #pragma unroll
             for (int k = 0; k < TS; ++k) {
-                const int t = tsub + k, i = k / 4, j = t % 4;
+                const int t = tsub + k, i = k / 4;
                 const float d4 = pick4(dt, tsub / 4 + i), u4 = pick4(uu, tsub / 4 + i);
                 const float dtj = quad_lane(d4, k % 4), duj = quad_lane(d4 * u4, k % 4);
                 const bool reset = KEEP && (resets >> t & 1);
