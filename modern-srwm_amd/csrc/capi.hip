@@ -130,7 +130,7 @@ int scan_dims(int N, int H, int L, int E, int S, int G) {
 }
 int conv_dims(int N, int H, int L, int E, int W) {
     if (!dims_ok(N, H, L, E) || W <= 0) return SRWM_EINVAL;
-    if (W < 2 || W > 4 || L > (1 << 30) || (int64_t)H * E > (1 << 20) || conv_parts(N, L) > kMaxGrid ||
+    if (W < 2 || W > 4 || L > (1 << 30) || (int64_t)H * E > (1 << 20) || conv_parts(N, H, L, E) > kMaxGrid ||
         (int64_t)N * H * E > ((int64_t)1 << 31))
         return SRWM_ESIZE;
     return SRWM_OK;
@@ -728,7 +728,7 @@ int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int 
 int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E, int W) {
     if (!floats) return SRWM_EINVAL;
     if (const int r = conv_dims(N, H, L, E, W)) return r;
-    floats[0] = conv_parts(N, L) * (W + 1) * H * E;
+    floats[0] = conv_parts(N, H, L, E) * (W + 1) * H * E;
     return SRWM_OK;
 }
 int residual_rms_norm_workspace(int64_t floats[1], int rows, int D) {

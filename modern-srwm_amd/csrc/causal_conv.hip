@@ -8,7 +8,15 @@
 namespace fw {
 namespace {
 
-constexpr int kConvLanes = 32, kConvRuns = 8, kConvSteps = 16;   // a workgroup: 32 vectors of channels x 8 runs of 16 steps
+// A workgroup: 32 vectors of channels x 8 runs of ST steps; those beside each other along the channels follow one another,
+// so that whole rows are read at a time (1 x 65536 steps x 2048 channels, bf16: forward 104 us, backward 212; neighbours
+// along the steps first 146 and 280).  Vectors of 8 bytes and 8 steps in the forward (4 x 2048 x 2048: 16.0 us; 16 steps 17.2,
+// 16 bytes 18.8: with fewer waves all of them load, compute and store at the same time), of two channels in the backward
+// (one 33.9, two 31.3, four 35.0 us with neighbours along the steps first).
+constexpr int kConvLanes = 32, kConvRuns = 8, kConvFwdSteps = 8;
+// The backward's runs are of 16 steps, of 8 where those would be fewer than kConvWaves waves (16 / 8 steps: 4 x 2048 x 2048 29.3
+// / 31.9 us; 2 x 1024 steps x 1024 channels 9.6 / 8.2; 32 x 100 x 256, fp32, 11.6 / 8.9).
+constexpr int kConvWaves = 4096;
 
 template <int V>
 __device__ __forceinline__ void zero(float (&v)[V]) {
@@ -21,17 +29,18 @@ __device__ __forceinline__ void widen(const Pack<T, V> &r, float (&v)[V]) {
     for (int i = 0; i < V; ++i) v[i] = (float)r.v[i];
 }
 
-// A thread's run: 16 steps of V channels of one sequence.
+// A thread's run: ST steps of V channels of one sequence.
 struct ConvPlace {
     int64_t d, t0;
     int n, h, e, Ln;
 };
-template <int V>
-__device__ __forceinline__ ConvPlace conv_place(const ConvParams &p, int runs) {
+template <int V, int ST>
+__device__ __forceinline__ ConvPlace conv_place(const ConvParams &p, int runs, unsigned cols) {
     ConvPlace c;
-    c.d = ((int64_t)blockIdx.y * kConvLanes + threadIdx.x) * V;
-    c.n = blockIdx.x / runs;
-    c.t0 = ((int64_t)(blockIdx.x % runs) * kConvRuns + threadIdx.y) * kConvSteps;
+    c.d = ((int64_t)(blockIdx.x % cols) * kConvLanes + threadIdx.x) * V;
+    const unsigned part = blockIdx.x / cols;
+    c.n = part / runs;
+    c.t0 = ((int64_t)(part % runs) * kConvRuns + threadIdx.y) * ST;
     c.h = c.d / p.E, c.e = c.d % p.E;
     c.Ln = p.lengths ? min(max(p.lengths[c.n], 0), p.L) : p.L;
     return c;
@@ -67,12 +76,12 @@ __device__ __forceinline__ uint32_t load_resets(const float *keep, int64_t t, in
 }
 
 // Memory-bound: every input and output once, plus W - 1 rows of the run in front (from the caches).  All of a run's rows
-// are asked for before the first is used (4 x 2048 steps x 2048 channels, 4 taps, bf16: 67 MB in 19 - 20 us, 3.4 TB/s; row
-// after row 24 us).
-template <typename T, int W, int V, bool KEEP>
-__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs) {
-    constexpr int R = kConvSteps + W - 1;
-    const ConvPlace c = conv_place<V>(p, runs);
+// are asked for before the first is used (4 x 2048 steps x 2048 channels, 4 taps, bf16: 67 MB in 16 us, 4.2 TB/s; 1 x 65536
+// steps 537 MB in 104 - 110 us, 5.0 TB/s).
+template <typename T, int W, int V, int ST, bool KEEP>
+__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs, unsigned cols) {
+    constexpr int R = ST + W - 1;
+    const ConvPlace c = conv_place<V, ST>(p, runs, cols);
     if (c.d >= (int64_t)p.H * p.E || (c.t0 >= p.L && c.t0 > 0)) return;
     const T *x = (const T *)p.x + c.n * p.xs.n + c.h * p.xs.h + c.e;
     const int64_t srow = ((int64_t)c.n * p.H + c.h) * (W - 1) * p.E + c.e;
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvPar
         bias[i] = p.bias ? p.bias[c.d + i] : 0.f;
     }
     // the row's last step is in this run (or the row is empty and this is its first run): it hands the carried rows on
-    const bool ends = Ln > 0 ? (c.t0 < Ln && Ln <= c.t0 + kConvSteps) : c.t0 == 0;
+    const bool ends = Ln > 0 ? (c.t0 < Ln && Ln <= c.t0 + ST) : c.t0 == 0;
     const int at_end = (int)(Ln - c.t0);
     T *last = (T *)p.last + srow;
 #pragma unroll
@@ -128,15 +137,15 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvPar
 
 // gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre): a run walks its steps and the W - 1 behind them, carrying the
 // gradients of the last W inputs, each complete when the window leaves it.  Between memory and arithmetic (vector
-// instructions 61 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 35 us, 2.9 TB/s;
-// with the rows one after the other 39 us.
-template <typename T, int W, int V, bool KEEP>
-__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs) {
-    constexpr int RX = kConvSteps + 2 * (W - 1), RG = kConvSteps + W - 1;
+// instructions 61 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 29 us, 3.4 TB/s,
+// 1 x 65536 steps 805 MB in 206 us, 3.9 TB/s.
+template <typename T, int W, int V, int ST, bool KEEP>
+__global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs, unsigned cols) {
+    constexpr int RX = ST + 2 * (W - 1), RG = ST + W - 1;
     const ConvParams &p = b.f;
     const int64_t D = (int64_t)p.H * p.E;
     __shared__ float red[kConvRuns][kConvLanes][V];
-    const ConvPlace c = conv_place<V>(p, runs);
+    const ConvPlace c = conv_place<V, ST>(p, runs, cols);
     float gw[W + 1][V];
 #pragma unroll
     for (int j = 0; j <= W; ++j) zero<V>(gw[j]);
@@ -200,7 +209,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
                 if (!KEEP || j <= since)
 #pragma unroll
                     for (int i = 0; i < V; ++i) acc[j][i] = fmaf(w[W - 1 - j][i], g[i], acc[j][i]);
-            if (s < kConvSteps) {
+            if (s < ST) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -226,7 +235,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
             }
         }
     }
-    float *part = b.part + (int64_t)blockIdx.x * (W + 1) * D;
+    float *part = b.part + (int64_t)(blockIdx.x / cols) * (W + 1) * D;
 #pragma unroll
     for (int j = 0; j <= W; ++j) {
         __syncthreads();
@@ -234,7 +243,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
         for (int i = 0; i < V; ++i) red[threadIdx.y][threadIdx.x][i] = gw[j][i];
         __syncthreads();
         for (int i = threadIdx.y * kConvLanes + threadIdx.x; i < kConvLanes * V; i += kConvLanes * kConvRuns) {
-            const int64_t at = (int64_t)blockIdx.y * kConvLanes * V + i;
+            const int64_t at = (int64_t)(blockIdx.x % cols) * kConvLanes * V + i;
             float v = 0.f;
 #pragma unroll
             for (int r = 0; r < kConvRuns; ++r) v += red[r][i / V][i % V];
@@ -309,46 +318,59 @@ bool conv_vec(const ConvParams &p) {
            vec_ok(p.last, sizeof(T) * V);
 }
 
-int conv_runs(int L) { return (L + kConvRuns * kConvSteps - 1) / (kConvRuns * kConvSteps); }
+int conv_runs(int L, int steps) { return (L + kConvRuns * steps - 1) / (kConvRuns * steps); }
+int conv_bwd_steps(int N, int H, int L, int E) {
+    const int64_t waves = (int64_t)N * conv_runs(L, 16) * (((int64_t)H * E + 63) / 64) * 4;
+    return waves < kConvWaves ? 8 : 16;
+}
+// A launch over runs and columns of `v` channels a lane; false: more workgroups than it takes.
+struct ConvGrid {
+    unsigned cols;
+    int64_t groups;
+    ConvGrid(const ConvParams &p, int runs, int v)
+        : cols((unsigned)(((int64_t)p.H * p.E / v + kConvLanes - 1) / kConvLanes)), groups((int64_t)p.N * runs * cols) {}
+    bool fits() const { return groups < ((int64_t)1 << 24); }   // of 256 threads each, below 2^32 of them
+};
 
+template <typename T, int W, int V>
+int fwd_as(const ConvParams &p, hipStream_t s) {
+    constexpr int ST = kConvFwdSteps;
+    const int runs = conv_runs(p.L, ST);
+    const ConvGrid g(p, runs, V);
+    if (!g.fits()) return -1;
+    const dim3 block(kConvLanes, kConvRuns);
+    if (p.keep) conv_fwd_kernel<T, W, V, ST, true><<<(unsigned)g.groups, block, 0, s>>>(p, runs, g.cols);
+    else conv_fwd_kernel<T, W, V, ST, false><<<(unsigned)g.groups, block, 0, s>>>(p, runs, g.cols);
+    return (int)hipGetLastError();
+}
 template <typename T, int W>
 int fwd(const ConvParams &p, hipStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const int64_t D = (int64_t)p.H * p.E;
+    constexpr int V = 8 / sizeof(T);
+    return conv_vec<T, V>(p) ? fwd_as<T, W, V>(p, s) : fwd_as<T, W, 1>(p, s);
+}
+template <typename T, int W, int V, int ST>
+int bwd_as(const ConvBwdParams &b, hipStream_t s) {
+    const ConvParams &p = b.f;
+    const int runs = conv_runs(p.L, ST);
+    const ConvGrid g(p, runs, V);
+    if (!g.fits()) return -1;
     const dim3 block(kConvLanes, kConvRuns);
-    const int runs = conv_runs(p.L);
-    auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
-    const bool vec = conv_vec<T, V>(p);
-    if (p.keep) {
-        if (vec) conv_fwd_kernel<T, W, V, true><<<grid(V), block, 0, s>>>(p, runs);
-        else conv_fwd_kernel<T, W, 1, true><<<grid(1), block, 0, s>>>(p, runs);
-    } else {
-        if (vec) conv_fwd_kernel<T, W, V, false><<<grid(V), block, 0, s>>>(p, runs);
-        else conv_fwd_kernel<T, W, 1, false><<<grid(1), block, 0, s>>>(p, runs);
-    }
+    if (p.keep) conv_bwd_kernel<T, W, V, ST, true><<<(unsigned)g.groups, block, 0, s>>>(b, runs, g.cols);
+    else conv_bwd_kernel<T, W, V, ST, false><<<(unsigned)g.groups, block, 0, s>>>(b, runs, g.cols);
+    const int r = (int)hipGetLastError();
+    if (r) return r;
+    const int64_t D = (int64_t)p.H * p.E;
+    conv_join_kernel<<<dim3((unsigned)((D + 31) / 32), W + 1), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);
     return (int)hipGetLastError();
 }
 template <typename T, int W>
 int bwd(const ConvBwdParams &b, hipStream_t s) {
-    constexpr int V = 4;
+    constexpr int V = 2;
     const ConvParams &p = b.f;
-    const int64_t D = (int64_t)p.H * p.E;
-    const dim3 block(kConvLanes, kConvRuns);
-    const int runs = conv_runs(p.L);
-    auto grid = [&](int v) { return dim3((unsigned)(p.N * runs), (unsigned)((D / v + kConvLanes - 1) / kConvLanes)); };
     const bool vec = p.E % V == 0 && rows_ok<T, V>(p.x, p.xs) && rows_ok<T, V>(b.go, b.gos) && rows_ok<T, V>(b.gx, b.gxs) &&
                      vec_ok(p.state, sizeof(T) * V) && vec_ok(b.glast, sizeof(T) * V) && vec_ok(b.gstate, sizeof(T) * V);
-    if (p.keep) {
-        if (vec) conv_bwd_kernel<T, W, V, true><<<grid(V), block, 0, s>>>(b, runs);
-        else conv_bwd_kernel<T, W, 1, true><<<grid(1), block, 0, s>>>(b, runs);
-    } else {
-        if (vec) conv_bwd_kernel<T, W, V, false><<<grid(V), block, 0, s>>>(b, runs);
-        else conv_bwd_kernel<T, W, 1, false><<<grid(1), block, 0, s>>>(b, runs);
-    }
-    const int r = (int)hipGetLastError();
-    if (r) return r;
-    conv_join_kernel<<<dim3((unsigned)((D + 31) / 32), W + 1), 256, 0, s>>>(b.part, b.gweight, b.gbias, D, W, p.N * runs);
-    return (int)hipGetLastError();
+    if (conv_bwd_steps(p.N, p.H, p.L, p.E) == 8) return vec ? bwd_as<T, W, V, 8>(b, s) : bwd_as<T, W, 1, 8>(b, s);
+    return vec ? bwd_as<T, W, V, 16>(b, s) : bwd_as<T, W, 1, 16>(b, s);
 }
 template <typename T, int W>
 int step(const ConvParams &p, hipStream_t s) {
@@ -362,7 +384,7 @@ int step(const ConvParams &p, hipStream_t s) {
 
 }  // namespace
 
-int64_t conv_parts(int N, int L) { return (int64_t)N * conv_runs(L); }
+int64_t conv_parts(int N, int H, int L, int E) { return (int64_t)N * conv_runs(L, conv_bwd_steps(N, H, L, E)); }
 
 #define FW_BY_TAPS(FN, W, P)                                        \
     switch (W) {                                                    \

@@ -325,7 +325,7 @@ int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len);
 int launch_scan_fwd(const ScanParams &p, bool bf16, hipStream_t s);
 int launch_scan_step(const ScanParams &p, bool bf16, hipStream_t s);   // u ... out: rows of one step; `last` is the state, in place
 int launch_scan_bwd(const ScanBwdParams &b, bool bf16, hipStream_t s);
-int64_t conv_parts(int N, int L);
+int64_t conv_parts(int N, int H, int L, int E);   // workgroups along the steps: rows of the backward's partial sums
 int launch_conv_fwd(const ConvParams &p, bool bf16, hipStream_t s);    // -1: no kernel for this number of taps
 int launch_conv_step(const ConvParams &p, bool bf16, hipStream_t s);   // as launch_scan_step
 int launch_conv_bwd(const ConvBwdParams &b, bool bf16, hipStream_t s);

@@ -297,6 +297,14 @@ def test_conv_options(options, dtype):
     run_conv(*conv_case(3, 2, 37, 24, 4, dtype=dtype, **options), silu=silu)
 
 
+@pytest.mark.parametrize("E,W,order,dtype", [(2752, 4, "steps", torch.float32), (2752, 2, "dense", torch.bfloat16),
+                                             (2753, 3, "offset", torch.bfloat16)], ids=str)
+@pytest.mark.parametrize("masks", [dict(), dict(keep=True, lengths=[650, 0, 17, 128])], ids=["plain", "masked"])
+def test_conv_of_many_steps_and_channels(E, W, order, dtype, masks):
+    """Calls that fill the device, whose backward walks runs of 16 steps."""
+    run_conv(*conv_case(4, 1, 650, E, W, dtype=dtype, order=order, **masks))
+
+
 def test_conv_masked_places_may_hold_anything():
     a, m, go, gl = conv_case(2, 1, 20, 8, 4, lengths=[20, 6])
     m["keep"] = torch.ones(2, 20)
