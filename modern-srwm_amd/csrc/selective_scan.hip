@@ -94,6 +94,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
             u.move(kScanBlock), dl.move(kScanBlock), z.move(kScanBlock), rows.move(kScanBlock);
             fetch(t0 + kScanBlock, n - kScanBlock);
         }
+        if (!w.busy) continue;
         if (saved) {
             if (w.on) store_states<SPL>(saved, S, w.q, h);
             saved += (int64_t)D * S;

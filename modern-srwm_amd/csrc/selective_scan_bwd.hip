@@ -124,6 +124,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
             dl.move(-kScanBlock), z.move(-kScanBlock), go.move(-kScanBlock), rows.move(-kScanBlock);
             fetch(t0 - kScanBlock, kScanBlock);
         }
+        if (!w.busy) continue;
 #pragma unroll
         for (int t = kScanBlock - 1; t >= 0; --t) {
             const int i = t / 4, j = t % 4;
