@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvPar
 
 // gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre): a run walks its steps and the W - 1 behind them, carrying the
 // gradients of the last W inputs, each complete when the window leaves it.  Between memory and arithmetic (vector
-// instructions 61 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 29 us, 3.4 TB/s,
+// instructions 80 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 29 us, 3.4 TB/s,
 // 1 x 65536 steps 805 MB in 206 us, 3.9 TB/s.
 template <typename T, int W, int V, int ST, bool KEEP>
 __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs, unsigned cols) {
