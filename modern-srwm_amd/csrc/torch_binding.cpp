@@ -115,9 +115,10 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
 void not_held_outside(const char *what, std::initializer_list<Tensor> ts) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     const auto dev = ts.begin()->get_device();
-    if (dev < 0 || hipStreamIsCapturing(c10::hip::getCurrentHIPStream(dev).stream(), &status) != hipSuccess ||
-        status == hipStreamCaptureStatusNone)
-        return;
+    if (dev < 0) return;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(dev).stream(), &status) != hipSuccess)
+        (void)hipGetLastError();   // the default stream while another one is captured: the launch will say so
+    if (status == hipStreamCaptureStatusNone) return;
     for (const Tensor &t : ts) {
         if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(t);

@@ -293,7 +293,8 @@ def test_conv_and_gradients(shape, W, dtype):
     dict(lengths=[99, -1, 33]), dict(order="dense"), dict(order="offset"), dict(silu=False), dict(keep=True, lengths=[2, 3, 17])], ids=str)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_conv_options(options, dtype):
-    silu = options.pop("silu", True) if "silu" in options else True
+    options = dict(options)
+    silu = options.pop("silu", True)
     run_conv(*conv_case(3, 2, 37, 24, 4, dtype=dtype, **options), silu=silu)
 
 
