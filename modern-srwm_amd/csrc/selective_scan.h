@@ -31,6 +31,11 @@ constexpr int kScanThreads = 256;   // 4 waves
 // with: forward 8 x 2048 steps (1 024 waves) 0.253 / 0.258, 4 x 2048 (512 waves) 0.55 / 0.147; backward 16 x 1024 (2 048
 // waves) 0.53 / 0.60, 8 x 2048 0.76 / 0.63.
 constexpr int kScanWaves = 4096, kScanEnoughFwd = 1024, kScanEnoughBwd = 2048;
+// The backward's main pass runs kScanBwdWaves at a time (two on each SIMD).  Segments shorter than kScanBwdShort are not
+// worth a second round of them, long ones are, as their rounds overlap (both kernels of the pass, us with segments for two
+// rounds / one: 32 x 100 steps x 8 groups of 32 channels 46.7 / 43.0, 4 x 512 x 2048 with 64 states 507 / 482; 4 x 2048 x
+// 2048 328 / 332, 8 x 1000 x 16 groups of 32 155 / 162).
+constexpr int kScanBwdWaves = 2048, kScanBwdShort = 96;
 // Shortest segment.  A segment also joins those in front of it one after the other, so their number n is bounded by their
 // length: n^2 <= steps forward, 4 steps backward (1 x 100000 steps of 64 channels, the two kernels of a pass, ms: n^2 <=
 // steps 0.130 + 0.236, 4 steps 0.139 + 0.224, 16 steps 0.189 + 0.254).

@@ -247,6 +247,8 @@ int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len) {
     while (most * most > (int64_t)L * (backward ? 4 : 1)) most = most * 7 / 8;
     if (most < 1) most = 1;
     n = n < most ? n : most;
+    const int64_t fits = (kScanBwdWaves + waves - 1) / waves;
+    if (backward && n > fits && L / n < kScanBwdShort) n = fits;
     int l = (int)((L + n - 1) / n);
     l = (l + kScanBlock - 1) / kScanBlock * kScanBlock;
     *len = l;
