@@ -142,3 +142,27 @@ def test_eight_bit_rows_of_tiny_numbers(size):
     assert float(o[1].abs().max()) == 448.0
     y = x[0].double() / (1e-5 ** 0.5)                           # the row's mean square vanishes next to eps
     assert float((o[0].double() * scale[0].double() - y).abs().max()) <= float(y.abs().max()) * 2.0 ** -4 + 2 * 1.4e-45
+
+
+@pytest.mark.parametrize("xt,rt", [t[1:] for t in TYPES], ids=[t[0] for t in TYPES])
+@pytest.mark.parametrize("D", [100, 1024, 2051, 9000])
+def test_eight_bit_values_are_the_quotients(D, xt, rt):
+    """Rows of ones with eps = 0 have a norm of exactly 1, so that a row's results are the weight's values and the quotients
+    by the row's scale are known to the last bit: many lie on a border of two e4m3 values, or a rounding beside one, and
+    have to fall to the side that the division gives them."""
+    g = torch.Generator().manual_seed(D)
+    x = torch.ones(3, D).to(xt)
+    r = None if rt is None else torch.zeros(3, D).to(rt)
+    for k in range(8):
+        top = 448 * float(1 + torch.rand((), generator=g))               # the scale, between 1 and 2
+        scale = torch.tensor(top, dtype=torch.float32) / 448
+        grid = torch.randint(0, 126, (D,), generator=g, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+        step = torch.where(grid < 2.0 ** -6, 2.0 ** -9, torch.exp2(torch.frexp(grid).exponent - 4.0))
+        border = grid + step / 2                                        # exact: e4m3 values have four bits
+        w = (border * scale) * torch.where(torch.rand(D, generator=g) < 0.5, -1.0, 1.0)
+        w[int(torch.randint(0, D, (), generator=g))] = top
+        assert float(w.abs().max()) == float(torch.tensor(top, dtype=torch.float32))
+        o, s, _ = residual_rms_norm_e4m3(x.to(DEV), None if r is None else r.to(DEV), w.to(DEV), 0.0)
+        assert torch.equal(s.cpu(), scale.expand(3, 1))
+        want = (w / scale).to(torch.float8_e4m3fn).float()
+        assert torch.equal(o.cpu().float(), want.expand(3, D)), f"{int((o.cpu().float() != want).sum())} of {3 * D} differ"
