@@ -114,9 +114,10 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormParams p) {
             }
         }
         top = row_reduce<TPR, OpMax>(top, lds);
-        // a small scale is lifted, so that neither its reciprocal nor the quotients' remainders leave the normal numbers; one
-        // that would round to zero is the smallest number
-        const float scale = top > 0.f ? fmaxf(top / kE4m3Max, 1.4e-45f) : 1.f;
+        float scale = top > 0.f ? top / kE4m3Max : 1.f;
+        // below the normal numbers max / 448 may be off by half of itself: rounded up, or the quotients would pass 448
+        if (scale < 0x1p-126f && scale * kE4m3Max < top) scale += 0x1p-149f;
+        // a small scale is lifted, so that neither its reciprocal nor the quotients' remainders leave the normal numbers
         lift = scale < 1e-20f ? 0x1p64f : 1.f;
         by = scale * lift;
         inv = 1.f / by;

@@ -166,3 +166,19 @@ def test_eight_bit_values_are_the_quotients(D, xt, rt):
         assert torch.equal(s.cpu(), scale.expand(3, 1))
         want = (w / scale).to(torch.float8_e4m3fn).float()
         assert torch.equal(o.cpu().float(), want.expand(3, D)), f"{int((o.cpu().float() != want).sum())} of {3 * D} differ"
+
+
+def test_eight_bit_scales_among_the_smallest_numbers():
+    """A row's largest value is a few hundred times float32's smallest number, where max / 448 is off by up to half of
+    itself: the scale is then the next number above it, so that no quotient passes the type's largest value."""
+    tops = list(range(1, 1200, 7)) + [449, 465, 600, 671, 672, 673, 1119, 1120, 5000, 6271, 6272, 6273]
+    x, least = torch.ones(1, 64, device=DEV), 2.0 ** -149
+    for k in tops:
+        w = (torch.arange(64) * k // 63).double() * least * torch.where(torch.arange(64) % 2 == 0, 1.0, -1.0)
+        o, scale, _ = residual_rms_norm_e4m3(x, None, w.float().to(DEV), 0.0)
+        o, scale = o.cpu().double(), float(scale)
+        assert torch.isfinite(o).all(), k
+        assert scale == -(-k // 448) * least, (k, scale / least)
+        # half a step of the type: 2^-4 of the value, or 2^-10 of the scale; the quotient is rounded once before, by 2^-24
+        bound = torch.maximum(w.abs() * 2.0 ** -4, torch.tensor(scale * 2.0 ** -10, dtype=torch.float64)) * (1 + 2.0 ** -20)
+        assert float(((o * scale - w).abs() - bound).max()) <= 0, k
