@@ -26,7 +26,8 @@ state is zeroed before the step, as in the step mode of the other operators; seq
 row get a 0 at their first steps.  lengths: (N,) int32 or None, the steps of each row of a padded batch: steps behind them
 are not read, their rows of out and of the gradients are zeros, and `last` is the state at the row's end.
 
-Gradients go to every float tensor, through `last` and into `state` as well; keep and lengths get none.
+Gradients go to every float tensor, through `last` and into `state` as well; keep and lengths get none.  There are no second
+derivatives and none in forward mode: such calls raise.
 """
 import srwm_hip
 

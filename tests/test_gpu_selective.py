@@ -490,6 +490,23 @@ def test_second_derivatives_are_refused():
             (call(leaf).sum() + first.square().sum()).backward()       # a penalty on the gradient next to a loss
 
 
+def test_gradients_with_tangents_are_refused():
+    """Forward mode over the backward: a gradient that comes in with a tangent raises instead of losing it."""
+    import torch.autograd.forward_ad as forward_ad
+    a, _, go, _ = scan_case(1, 2, 20, 8, 16, 1)
+    d = {k: place(v) for k, v in a.items()}
+    w, b = torch.randn(2, 8, 4, device=DEV), torch.randn(16, device=DEV)
+    calls = {"selective_scan": (lambda t: selective_scan(**{**d, "u": t})[0], d["u"]),
+             "causal_conv": (lambda t: causal_conv(t, w)[0], d["u"]),
+             "residual_rms_norm": (lambda t: residual_rms_norm(t, t, b)[0], torch.randn(5, 16, device=DEV))}
+    for name, (call, t) in calls.items():
+        leaf = t.detach().requires_grad_()
+        out = call(leaf)
+        g = torch.randn_like(out)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match=name + " has no derivative in forward mode"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(g, g))
+
+
 def test_offsets_past_32_bits():
     """Rows whose elements lie further than 2^32 bytes (and 2^31 elements) apart."""
     H, E, S, L = 1, 16, 16, 5

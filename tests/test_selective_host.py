@@ -124,6 +124,29 @@ def test_host_layer_refusals():
         residual_rms_norm(z(1, 16385), None, z(16385).requires_grad_())
 
 
+def test_derivatives_in_forward_mode_are_refused():
+    """A dual tensor asks for no gradient by itself: every operator raises for it, with and without gradients recorded."""
+    import torch.autograd.forward_ad as forward_ad
+    from residual_norm import residual_rms_norm, residual_rms_norm_e4m3
+    from selective_scan import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+    z = torch.zeros
+    scan = dict(u=z(1, 1, 2, 4), delta=z(1, 1, 2, 4), A=z(1, 4, 16), B=z(1, 1, 2, 16), C=z(1, 1, 2, 16), D=z(1, 4), z=z(1, 1, 2, 4),
+                delta_bias=z(1, 4), state=z(1, 1, 4, 16))
+    step = dict(scan, **{k: scan[k][:, :, 0] for k in ("u", "delta", "B", "C", "z")})
+    conv = dict(x=z(1, 1, 2, 4), weight=z(1, 4, 4), bias=z(1, 4), state=z(1, 1, 3, 4))
+    norm = dict(x=z(2, 4), residual=z(2, 4), weight=z(4))
+    calls = [(selective_scan, scan), (selective_scan_step, step), (causal_conv, conv),
+             (causal_conv_step, dict(conv, x=z(1, 1, 4))), (residual_rms_norm, norm), (residual_rms_norm_e4m3, norm)]
+    with forward_ad.dual_level():
+        for fn, args in calls:
+            for k in args:
+                dual = dict(args, **{k: forward_ad.make_dual(args[k], torch.ones_like(args[k]))})
+                for recorded in (True, False):
+                    with torch.set_grad_enabled(recorded):
+                        with pytest.raises(RuntimeError, match=fn.__name__ + " has no derivative in forward mode"):
+                            fn(**dual)
+
+
 def test_output_rows_follow_the_input():
     import srwm_hip
     srwm_hip = srwm_hip.binding()
