@@ -4,8 +4,10 @@
 // and a backward pass then waits for the interpreter in autograd's own thread.  No kernel is launched other than through the
 // C entry points, and there is no CPU path.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -117,6 +119,20 @@ void no_tangents(const char *what, std::initializer_list<Tensor> ts) {
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const Tensor &t : ts)
         TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, " has no derivative in forward mode");
+}
+
+// A trace holds the allocations of a call and not its kernels: run again, it would return memory that nobody wrote.
+void not_traced(const char *what) {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Mode = c10::impl::TorchDispatchModeKey;
+    bool traced = at::tracer::impl::is_dispatch_enabled();
+    if (Modes::any_modes_set())
+        for (const Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL}) traced = traced || Modes::get_mode(m).has_value();
+    TORCH_CHECK(!traced, what, " cannot be traced: its kernels are launched outside torch's dispatcher");
+}
+void plain_call(const char *what, std::initializer_list<Tensor> ts) {
+    no_tangents(what, ts);
+    not_traced(what);
 }
 
 // A captured backward joins the streams of the leaves' gradient accumulators.  One that a live graph outside the capture
@@ -299,7 +315,7 @@ struct SelectiveScan : Function<SelectiveScan> {
         return {out, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_tangents("the backward of selective_scan", {grads[0], grads[1]});
+        plain_call("the backward of selective_scan", {grads[0], grads[1]});
         const variable_list s = ctx->get_saved_variables();
         ScanIn in(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], false);
         const Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
@@ -315,7 +331,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor &u, const Tensor &delta, 
                                           bool softplus) {
     const Tensor D = or_none(D_), z = or_none(z_), bias = or_none(bias_), state = or_none(state_), keep = or_none(keep_),
                  lengths = or_none(lengths_);
-    no_tangents("selective_scan", {u, delta, A, B, C, D, z, bias, state});
+    plain_call("selective_scan", {u, delta, A, B, C, D, z, bias, state});
     if (wants_grad({u, delta, A, B, C, D, z, bias, state})) {
         not_held_outside("selective_scan", {u, delta, A, B, C, D, z, bias, state});
         const variable_list r = SelectiveScan::apply(u, delta, A, B, C, D_, z_, bias_, state_, keep_, lengths_, softplus);
@@ -331,7 +347,7 @@ Tensor selective_scan_step(const Tensor &u, const Tensor &delta, const Tensor &s
                            const Tensor &C, const MaybeTensor &D_, const MaybeTensor &z_, const MaybeTensor &bias_,
                            const MaybeTensor &keep_, bool softplus) {
     const Tensor D = or_none(D_), z = or_none(z_), bias = or_none(bias_);
-    no_tangents("selective_scan_step", {u, delta, A, B, C, D, z, bias, state});
+    plain_call("selective_scan_step", {u, delta, A, B, C, D, z, bias, state});
     TORCH_CHECK(!wants_grad({u, delta, A, B, C, D, z, bias, state}),
                 "selective_scan_step has no backward: call it under torch.no_grad(), or selective_scan with L = 1");
     const at::NoGradGuard none;
@@ -420,7 +436,7 @@ struct CausalConv : Function<CausalConv> {
         return {out, last};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        no_tangents("the backward of causal_conv", {grads[0], grads[1]});
+        plain_call("the backward of causal_conv", {grads[0], grads[1]});
         const variable_list s = ctx->get_saved_variables();
         const ConvIn in(s[0], s[1], s[2], s[4], s[5], false);
         const Tensor &x = in.x.t;
@@ -455,7 +471,7 @@ struct CausalConv : Function<CausalConv> {
 std::tuple<Tensor, Tensor> causal_conv(const Tensor &x, const Tensor &weight, const MaybeTensor &bias_, const MaybeTensor &state_,
                                        const MaybeTensor &keep_, const MaybeTensor &lengths_, bool silu) {
     const Tensor bias = or_none(bias_), state = or_none(state_), keep = or_none(keep_), lengths = or_none(lengths_);
-    no_tangents("causal_conv", {x, weight, bias, state});
+    plain_call("causal_conv", {x, weight, bias, state});
     if (wants_grad({x, weight, bias, state})) {
         not_held_outside("causal_conv", {x, weight, bias, state});
         const variable_list r = CausalConv::apply(x, weight, bias_, state_, keep_, lengths_, silu);
@@ -468,7 +484,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor &x, const Tensor &weight, co
 Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weight, const MaybeTensor &bias_, const MaybeTensor &keep_,
                         bool silu) {
     const Tensor bias = or_none(bias_);
-    no_tangents("causal_conv_step", {x, weight, bias, state});
+    plain_call("causal_conv_step", {x, weight, bias, state});
     TORCH_CHECK(!wants_grad({x, weight, bias, state}),
                 "causal_conv_step has no backward: call it under torch.no_grad(), or causal_conv with L = 1");
     const at::NoGradGuard none;
@@ -555,7 +571,7 @@ struct ResidualRMSNorm : Function<ResidualRMSNorm> {
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const variable_list s = ctx->get_saved_variables();
         const bool with_residual = ctx->saved_data["residual"].toBool();
-        no_tangents("the backward of residual_rms_norm", {grads[0], with_residual ? grads[1] : Tensor()});
+        plain_call("the backward of residual_rms_norm", {grads[0], with_residual ? grads[1] : Tensor()});
         const auto io = ctx->saved_data["bf16"].toBool() ? at::kBFloat16 : at::kFloat;
         return run(s[0].contiguous(), s[1], s[2], grads[0], with_residual ? grads[1] : Tensor(), io, with_residual, s[0].device());
     }
@@ -594,7 +610,7 @@ struct ResidualRMSNorm : Function<ResidualRMSNorm> {
 
 std::tuple<Tensor, Tensor> residual_rms_norm(const Tensor &x, const MaybeTensor &residual_, const Tensor &weight, double eps) {
     const Tensor residual = or_none(residual_);
-    no_tangents("residual_rms_norm", {x, residual, weight});
+    plain_call("residual_rms_norm", {x, residual, weight});
     if (wants_grad({x, residual, weight})) {
         TORCH_CHECK_VALUE(x.dim() == 0 || x.size(-1) <= kNormBackwardMax, "residual_rms_norm has no backward for rows longer than ",
                           kNormBackwardMax);
@@ -610,7 +626,7 @@ std::tuple<Tensor, Tensor> residual_rms_norm(const Tensor &x, const MaybeTensor 
 
 std::tuple<Tensor, Tensor, Tensor> residual_rms_norm_e4m3(const Tensor &x, const MaybeTensor &residual_, const Tensor &weight, double eps_) {
     const Tensor residual = or_none(residual_);
-    no_tangents("residual_rms_norm_e4m3", {x, residual, weight});
+    plain_call("residual_rms_norm_e4m3", {x, residual, weight});
     TORCH_CHECK(!wants_grad({x, residual, weight}), "residual_rms_norm_e4m3 has no backward: call it under torch.no_grad()");
     const at::NoGradGuard none;
     const NormIn in(x, residual, weight);

@@ -10,7 +10,8 @@ itself); weight: (D,) float32.  out has the type of x and total that of residual
 rounded to that type.  The second form serves layers whose projection runs in 8 bits: out is torch.float8_e4m3fn,
 each row divided by scale = max|row| / 448 (1 for a row of zeros) and rounded to nearest even, so that out * scale is the
 norm's result; it has no backward.  Rows longer than 16384 have no backward either.
-There are no second derivatives and none in forward mode: such calls raise.
+There are no second derivatives and none in forward mode, and a call cannot be traced (torch.jit.trace, make_fx): such calls
+raise.
 """
 import srwm_hip
 

@@ -27,7 +27,7 @@ row get a 0 at their first steps.  lengths: (N,) int32 or None, the steps of eac
 are not read, their rows of out and of the gradients are zeros, and `last` is the state at the row's end.
 
 Gradients go to every float tensor, through `last` and into `state` as well; keep and lengths get none.  There are no second
-derivatives and none in forward mode: such calls raise.
+derivatives and none in forward mode, and a call cannot be traced (torch.jit.trace, make_fx): such calls raise.
 """
 import srwm_hip
 

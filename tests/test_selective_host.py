@@ -124,9 +124,8 @@ def test_host_layer_refusals():
         residual_rms_norm(z(1, 16385), None, z(16385).requires_grad_())
 
 
-def test_derivatives_in_forward_mode_are_refused():
-    """A dual tensor asks for no gradient by itself: every operator raises for it, with and without gradients recorded."""
-    import torch.autograd.forward_ad as forward_ad
+def every_operator():
+    """(operator, its arguments) for each one, on the CPU."""
     from residual_norm import residual_rms_norm, residual_rms_norm_e4m3
     from selective_scan import causal_conv, causal_conv_step, selective_scan, selective_scan_step
     z = torch.zeros
@@ -135,16 +134,40 @@ def test_derivatives_in_forward_mode_are_refused():
     step = dict(scan, **{k: scan[k][:, :, 0] for k in ("u", "delta", "B", "C", "z")})
     conv = dict(x=z(1, 1, 2, 4), weight=z(1, 4, 4), bias=z(1, 4), state=z(1, 1, 3, 4))
     norm = dict(x=z(2, 4), residual=z(2, 4), weight=z(4))
-    calls = [(selective_scan, scan), (selective_scan_step, step), (causal_conv, conv),
+    return [(selective_scan, scan), (selective_scan_step, step), (causal_conv, conv),
              (causal_conv_step, dict(conv, x=z(1, 1, 4))), (residual_rms_norm, norm), (residual_rms_norm_e4m3, norm)]
+
+
+def test_derivatives_in_forward_mode_are_refused():
+    """A dual tensor asks for no gradient by itself: every operator raises for it, with and without gradients recorded."""
+    import torch.autograd.forward_ad as forward_ad
     with forward_ad.dual_level():
-        for fn, args in calls:
+        for fn, args in every_operator():
             for k in args:
                 dual = dict(args, **{k: forward_ad.make_dual(args[k], torch.ones_like(args[k]))})
                 for recorded in (True, False):
                     with torch.set_grad_enabled(recorded):
                         with pytest.raises(RuntimeError, match=fn.__name__ + " has no derivative in forward mode"):
                             fn(**dual)
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_tracing_is_refused():
+    """A trace would hold the call's allocations without its kernels."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for fn, args in every_operator():
+        error = pytest.raises(RuntimeError, match=fn.__name__ + " cannot be traced")
+        call = lambda *t: fn(**dict(zip(args, t)))
+        for recorded in (True, False):
+            with torch.set_grad_enabled(recorded):
+                with error:
+                    torch.jit.trace(call, tuple(args.values()), check_trace=False)
+                for mode in ("real", "fake"):
+                    with error:
+                        make_fx(call, tracing_mode=mode)(*args.values())
+                with FakeTensorMode(allow_non_fake_inputs=True), error:
+                    call(*args.values())
 
 
 def test_output_rows_follow_the_input():
