@@ -449,13 +449,21 @@ class SelectiveLayer(nn.Module):
         """From here on the projection in front runs in 8 bits wherever no gradient is recorded: its weight is kept as
         e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16.  A
         weight that is changed in place, loaded, replaced or moved afterwards is converted anew (what is written past the
-        version counter, through .data, is not seen: call serve_e4m3 again)."""
+        version counter, through .data, is not seen: call serve_e4m3 again).  The 8-bit weight is overwritten where it lies, so
+        that replays of a captured graph follow it from the next call of the layer or of serve_e4m3 on."""
         if self.in_dim % 16 or self.num_head * self.dim_head % 8:
             raise ValueError("the 8-bit projection needs in_dim and 2 * num_head * dim_head divisible by 16")
-        weight = self.in_linear.weight
-        w = weight.detach().float()
-        scale = w.abs().amax(1, keepdim=True).clamp_min(1e-30) / 448
-        self._eight = (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous(), self._weight_made_from()
+        weight, made_from = self.in_linear.weight, self._weight_made_from()
+        with torch.inference_mode(False), torch.no_grad():
+            w = weight.detach().float()
+            scale = w.abs().amax(1, keepdim=True).clamp_min(1e-30) / 448
+            new = (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous()
+            old = self._eight[:2] if self._eight else ()
+            if old and old[0].shape == new[0].shape and old[0].device == new[0].device:
+                for a, b in zip(old, new):   # where they lie: a captured graph reads them there
+                    a.copy_(b)
+                new = old
+        self._eight = *new, made_from
         return self
 
     def _weight_made_from(self):

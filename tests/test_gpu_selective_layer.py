@@ -199,3 +199,45 @@ def test_stack_steps_equal_the_stack():
         states = [layer.start(3, DEV) for layer in stack.layers]
         steps = torch.stack([stack.step(h[t], states) for t in range(9)])
     close(steps, whole, "steps")
+
+
+def test_replays_follow_the_8_bit_weight():
+    """A graph captured with the 8-bit projection gives what the layer gives, also once the weight was stepped, loaded or
+    replaced and the layer called (or serve_e4m3) in between."""
+    torch.manual_seed(14)
+    layer = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(torch.bfloat16).serve_e4m3()
+    h = torch.randn(5, 3, 32, generator=torch.Generator().manual_seed(15)).to(DEV).bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        layer(h)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        out = layer(h)
+
+    def load():
+        layer.load_state_dict({**layer.state_dict(), "in_linear.weight": torch.randn_like(layer.in_linear.weight)})
+
+    def step():
+        with torch.no_grad():
+            layer.in_linear.weight.mul_(-1.5)
+
+    def replace():
+        layer.in_linear.weight = torch.nn.Parameter(torch.randn_like(layer.in_linear.weight))
+    for change in (lambda: None, step, load, replace, step):
+        change()
+        with torch.no_grad():
+            want = layer(h)
+        junk = [torch.full((64, 32), 1e4, device=DEV).to(torch.float8_e4m3fn) for _ in range(4)]   # where a freed weight lay
+        for _ in range(3):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+        del junk
+    step()
+    layer.serve_e4m3()
+    graph.replay()
+    with torch.no_grad():
+        assert torch.equal(out, layer(h))
