@@ -241,3 +241,34 @@ def test_replays_follow_the_8_bit_weight():
     graph.replay()
     with torch.no_grad():
         assert torch.equal(out, layer(h))
+
+
+def test_the_8_bit_weight_is_not_converted_in_a_capture():
+    """Recorded into a graph, the conversion would not have run when the next eager call takes the weight for converted."""
+    h = torch.randn(5, 3, 32, generator=torch.Generator().manual_seed(16)).to(DEV).bfloat16()
+    torch.manual_seed(17)
+    layer = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(torch.bfloat16).serve_e4m3()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        layer(h)
+    torch.cuda.current_stream().wait_stream(side)
+    twin = copy.deepcopy(layer)                            # has no 8-bit weight yet
+    with torch.no_grad():
+        layer.in_linear.weight.mul_(-0.5)
+        twin.in_linear.weight.mul_(-0.5)
+    for each in (layer, twin):
+        for call in (lambda: each(h), each.serve_e4m3):
+            with pytest.raises(RuntimeError, match="while a stream is being captured"):
+                with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    call()
+        with torch.no_grad():
+            want = each(h)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = each(h)
+            for _ in range(3):
+                out.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(out, want)
