@@ -469,6 +469,8 @@ class SelectiveLayer(nn.Module):
                 for a, b in zip(old, new):   # where they lie: a captured graph reads them there
                     a.copy_(b)
                 new = old
+        if weight.is_cuda:   # it counts as converted for the calls of every stream
+            torch.cuda.current_stream(weight.device).synchronize()
         self._eight = *new, made_from
         return self
 

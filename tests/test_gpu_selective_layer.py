@@ -272,3 +272,25 @@ def test_the_8_bit_weight_is_not_converted_in_a_capture():
                 graph.replay()
                 torch.cuda.synchronize()
                 assert torch.equal(out, want)
+
+
+def test_the_8_bit_weight_is_ready_for_other_streams():
+    """Converted on a stream that is busy, then used on another one without a wait between them."""
+    torch.manual_seed(18)
+    layer = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(torch.bfloat16).serve_e4m3()
+    h = torch.randn(5, 3, 32, generator=torch.Generator().manual_seed(19)).to(DEV).bfloat16()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.no_grad():
+            layer(h)
+            layer.in_linear.weight.copy_(torch.randn_like(layer.in_linear.weight))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            layer.serve_e4m3()
+        with torch.no_grad():
+            got = layer(h)
+            side.synchronize()
+            want = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(torch.bfloat16)
+            want.load_state_dict(layer.state_dict())
+            assert torch.equal(got, want.serve_e4m3()(h))
