@@ -449,7 +449,8 @@ class SelectiveLayer(nn.Module):
         """From here on the projection in front runs in 8 bits wherever no gradient is recorded: its weight is kept as
         e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16.  A
         weight that is changed in place, loaded, replaced or moved afterwards is converted anew (what is written past the
-        version counter, through .data, is not seen: call serve_e4m3 again).  The 8-bit weight is overwritten where it lies, so
+        version counter, through .data or into parameters made under torch.inference_mode(), which have none, is not seen: call
+        serve_e4m3 again).  The 8-bit weight is overwritten where it lies, so
         that replays of a captured graph follow it from the next call of the layer or of serve_e4m3 on; a capture that would
         have to convert it raises."""
         if self.in_dim % 16 or self.num_head * self.dim_head % 8:
@@ -479,10 +480,15 @@ class SelectiveLayer(nn.Module):
         return w, 0 if w.is_inference() else w._version, w.dtype, w.device
 
     def _weight_e4m3(self):
-        if not self._eight or any(a is not b and (torch.is_tensor(a) or a != b)
+        if not self._eight or not self._eight[2] or any(a is not b and (torch.is_tensor(a) or a != b)
                                   for a, b in zip(self._eight[2], self._weight_made_from())):
             self.serve_e4m3()
         return self._eight[:2]
+
+    def _apply(self, fn, recurse=True):   # .to() and its like write parameters past the version counter
+        if self._eight:
+            self._eight = *self._eight[:2], ()
+        return super()._apply(fn, recurse)
 
     def __getstate__(self):   # a copy converts its own weight at its first use
         return {**self.__dict__, "_eight": None if self._eight is None else ()}

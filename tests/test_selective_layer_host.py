@@ -28,3 +28,17 @@ def test_the_8_bit_weight_is_overwritten_where_it_lies():
         assert other.serve_e4m3()._weight_e4m3()[0].data_ptr() == at
     with torch.inference_mode():
         assert other.serve_e4m3()._weight_e4m3()[0].data_ptr() == at
+
+
+def test_the_8_bit_weight_follows_conversions_and_back():
+    """Rounded to 16 bits and widened again, the weight has the same type, device and version as before."""
+    torch.manual_seed(2)
+    layer = SelectiveLayer(2, 16, 32, 0.0).serve_e4m3()
+    at = layer._weight_e4m3()[0].data_ptr()
+    layer.to(torch.bfloat16).to(torch.float32)
+    fresh = SelectiveLayer(2, 16, 32, 0.0)
+    fresh.load_state_dict(layer.state_dict())
+    for a, b in zip(layer._weight_e4m3(), fresh.serve_e4m3()._weight_e4m3()):
+        assert torch.equal(a.float(), b.float())
+    assert layer._weight_e4m3()[0].data_ptr() == at
+    assert SelectiveLayer(2, 16, 32, 0.0).to(torch.bfloat16)._eight is None
