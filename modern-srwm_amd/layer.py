@@ -503,7 +503,7 @@ class SelectiveLayer(nn.Module):
         w, w_scale = self._weight_e4m3()
         rows = torch._scaled_mm(y.reshape(-1, self.in_dim), w.t(), scale_a=scale.reshape(-1, 1), scale_b=w_scale,
                                 out_dtype=torch.bfloat16)
-        return rows.to(h.dtype).view(*h.shape[:-1], -1), total
+        return rows.to(self.in_linear.weight.dtype).view(*h.shape[:-1], -1), total
 
     def _parameters_of_scan(self):
         return -torch.exp(self.A_log.float()), self.D.float(), self.dt_bias.float()

@@ -294,3 +294,23 @@ def test_the_8_bit_weight_is_ready_for_other_streams():
             want = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(torch.bfloat16)
             want.load_state_dict(layer.state_dict())
             assert torch.equal(got, want.serve_e4m3()(h))
+
+
+@pytest.mark.parametrize("rows,weights", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)], ids=str)
+def test_eight_bit_projection_with_rows_of_another_type(rows, weights):
+    """The projection's result has the type of the layer's weights, in 8 bits as in 16 or 32: the same calls run, and their
+    states have the same types."""
+    torch.manual_seed(20)
+    layer = SelectiveLayer(2, 16, 32, 0.0).to(DEV).to(weights)
+    stack = SelectiveStack(2, 2, 16, 32, 0.0).to(DEV).to(weights)
+    h = torch.randn(9, 3, 32, generator=torch.Generator().manual_seed(21)).to(DEV).to(rows)
+    with torch.no_grad():
+        want, state = layer(h, get_state=True)
+        swant, sstates = stack(h)
+        layer.serve_e4m3(), stack.serve_e4m3()
+        got, state8 = layer(h, get_state=True)
+        sgot, sstates8 = stack(h)
+        assert torch.isfinite(layer.step(h[0], layer.start(3, DEV, weights))).all()
+        assert torch.isfinite(stack.step(h[0], [each.start(3, DEV, weights) for each in stack.layers])).all()
+    for a, b in [(got, want), (sgot, swant), *zip(state8, state), *((x, y) for p, q in zip(sstates8, sstates) for x, y in zip(p, q))]:
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.isfinite(a).all()
