@@ -10,12 +10,15 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/python.h>
 
 #include <string>
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/srwm_hip.h"
 
@@ -135,22 +138,39 @@ void plain_call(const char *what, std::initializer_list<Tensor> ts) {
     not_traced(what);
 }
 
-// A captured backward joins the streams of the leaves' gradient accumulators.  One that a live graph outside the capture
-// recorded on the default stream cannot be joined: the process would end inside the backward, so the forward refuses.
-void not_held_outside(const char *what, std::initializer_list<Tensor> ts) {
+// A captured backward joins the streams of the leaves' gradient accumulators, those of leaves that reach the call through
+// other operations among them.  One that a live graph outside the capture recorded on the default stream cannot be joined:
+// the process would end inside the backward, so the forward refuses.  The graph behind the inputs is walked in captures only.
+void not_held_outside(const char *what, c10::ArrayRef<Tensor> ts) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    const auto dev = ts.begin()->get_device();
+    int dev = -1;
+    for (const Tensor &t : ts)
+        if (dev < 0 && t.defined() && t.is_cuda()) dev = t.get_device();
     if (dev < 0) return;
     if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(dev).stream(), &status) != hipSuccess)
         (void)hipGetLastError();   // the default stream while another one is captured: the launch will say so
     if (status == hipStreamCaptureStatusNone) return;
+    std::vector<torch::autograd::Node *> open;
+    std::vector<std::shared_ptr<torch::autograd::Node>> leaves;   // hold what the open list points to
     for (const Tensor &t : ts) {
-        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-        const auto on = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!on || on->id() != c10::Stream(c10::Stream::DEFAULT, on->device()).id(), what,
-                    ": a stream is being captured while a graph recorded on the default stream still holds the gradient of a leaf of "
-                    "this call; drop that graph and its outputs first, or record it on a side stream");
+        if (!t.defined() || !t.requires_grad()) continue;
+        if (auto node = t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn()) {
+            open.push_back(node.get());
+            leaves.push_back(std::move(node));
+        }
+    }
+    std::unordered_set<torch::autograd::Node *> seen(open.begin(), open.end());
+    while (!open.empty()) {
+        torch::autograd::Node *node = open.back();
+        open.pop_back();
+        if (dynamic_cast<torch::autograd::AccumulateGrad *>(node)) {
+            const auto on = node->stream();
+            TORCH_CHECK(!on || on->id() != c10::Stream(c10::Stream::DEFAULT, on->device()).id(), what,
+                        ": a stream is being captured while a graph recorded on the default stream still holds the gradient of a leaf of "
+                        "this call; drop that graph and its outputs first, or record it on a side stream");
+        }
+        for (const torch::autograd::Edge &e : node->next_edges())
+            if (e.function && seen.insert(e.function.get()).second) open.push_back(e.function.get());
     }
 }
 
@@ -653,6 +673,7 @@ std::tuple<Tensor, Tensor, Tensor> residual_rms_norm_e4m3(const Tensor &x, const
 PYBIND11_MODULE(srwm_torch, m) {
     using release = py::call_guard<py::gil_scoped_release>;
     m.def("abi_version", &srwm_hip_abi_version);
+    m.def("not_held_outside", [](const std::string &what, const std::vector<Tensor> &ts) { not_held_outside(what.c_str(), ts); });
     m.def("rows_like", &rows_like, release());
     m.def("selective_scan", &selective_scan, release());
     m.def("selective_scan_step", &selective_scan_step, release());

@@ -21,6 +21,7 @@ import torch.nn.functional as F
 
 # the delta-rule operators with `out` in the memory order of the step-major views these layers hand in, so that the
 # reshape chain behind them (_heads_out) is a view; the plain operators return the reference's dense (N, H, L, M)
+import srwm_hip
 from fast_weight import delta_layer_inputs
 from fast_weight import fast_weight_delta_rows as fast_weight_delta
 from fast_weight import fast_weight_delta_steps_rows as fast_weight_delta_steps
@@ -519,6 +520,9 @@ class SelectiveLayer(nn.Module):
         """(output without the residual, the residual stream with h added, new state).  h: (len, B, in_dim)."""
         slen, bsz, _ = h.shape
         inner = self.num_head * self.dim_head
+        if h.is_cuda and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+            # the operators check what reaches them; the projection behind them does not
+            srwm_hip.binding().not_held_outside("SelectiveLayer", list(self.parameters()))
         rows, total = self._project_in(h, residual)
         x, z = rows.view(slen, bsz, 2, self.num_head, self.dim_head).permute(2, 1, 3, 0, 4)
         conv_state, scan_state = state if state is not None else (None, None)

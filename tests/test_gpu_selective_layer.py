@@ -314,3 +314,47 @@ def test_eight_bit_projection_with_rows_of_another_type(rows, weights):
         assert torch.isfinite(stack.step(h[0], [each.start(3, DEV, weights) for each in stack.layers])).all()
     for a, b in [(got, want), (sgot, swant), *zip(state8, state), *((x, y) for p, q in zip(sstates8, sstates) for x, y in zip(p, q))]:
         assert a.dtype == b.dtype and a.shape == b.shape and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_capture_is_refused_while_an_eager_graph_holds_a_parameter(dtype):
+    """The layer hands its parameters to the operators converted, or to its projections: they are found behind the inputs."""
+    layer = make(22).to(dtype)
+    stack = SelectiveStack(2, 2, 16, 32, 0.0).to(DEV).to(dtype)
+    h = torch.randn(7, 2, 24, generator=torch.Generator().manual_seed(23)).to(DEV).to(dtype)
+    hs = torch.randn(7, 2, 32, generator=torch.Generator().manual_seed(24)).to(DEV).to(dtype)
+    for model, x in ((layer, h), (stack, hs)):
+        side = torch.cuda.Stream()                         # warm-up: the projections' library makes its handles
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.no_grad(), torch.cuda.stream(side):
+            model(x)
+        torch.cuda.current_stream().wait_stream(side)
+        for held in model.parameters():                    # each of them alone
+            eager = held * 2
+            with pytest.raises(RuntimeError, match="a stream is being captured"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    model(x)
+            with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+                model(x)
+            del eager
+        side = torch.cuda.Stream()                         # held by a graph of a side stream: may be joined
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = model(x)
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            model(x)
+        del eager
+
+
+def test_capture_is_refused_for_leaves_behind_the_inputs():
+    """A leaf that reaches an operator through other operations counts as its leaf."""
+    from residual_norm import residual_rms_norm
+    leaf, w = torch.randn(4, 16, device=DEV).requires_grad_(), torch.randn(16, device=DEV)
+    eager = leaf.exp()
+    with pytest.raises(RuntimeError, match="residual_rms_norm: a stream is being captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            residual_rms_norm(-torch.exp(leaf.double().float()), None, w)
+    del eager
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        residual_rms_norm(-torch.exp(leaf.double().float()), None, w)
