@@ -19,7 +19,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
     using Bc = ScanBc<T, SPL>;
     __shared__ float bc[2][2][kScanBlock][SP];   // [buffer][B | C][step][state]
     const ScanRun run = scan_run(p, blockIdx.x % p.N, blockIdx.z);
-    if (!run.used || (LOCAL && run.seg == run.count - 1)) return;   // the whole workgroup; a row's last result is not needed
+    if (LOCAL && (!run.used || run.seg == run.count - 1)) return;   // the whole workgroup; a row's last result is not needed
     const ScanLane w = scan_lane(p, run.n);
     const int S = p.S, D = p.H * p.E, tbeg = run.tbeg, tend = run.tend;
 
@@ -146,10 +146,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_fwd_kernel(ScanParams p) {
         store_states<SPL>(p.seg_decay + at, S, w.q, A2);
         store_states<SPL>(p.seg_state + at, S, w.q, h);
     } else {
-        if (run.seg == run.count - 1) store_states<SPL>(p.last + w.n * (int64_t)D * S + states, S, w.q, h);
-        int first, behind;   // rows behind the sequence's end
-        behind_share(p, run, first, behind);
-        ScanRows<T, OFF> rest(p.out, p.os, w, first);
+        if (run.used && run.seg == run.count - 1) store_states<SPL>(p.last + w.n * (int64_t)D * S + states, S, w.q, h);
+        if (!p.lengths) return;
+        int first, behind;   // rows behind a sequence's end
+        ScanLane at = w;
+        at.n = blockIdx.x % p.N;
+        behind_share(p, at.n, blockIdx.z, first, behind);
+        ScanRows<T, OFF> rest(p.out, p.os, at, first);
         for (int t = first; t < behind; t += 4, rest.move(4))
             if (t + w.q < behind) io_store(rest.at(0, w.q), 0.f);
     }

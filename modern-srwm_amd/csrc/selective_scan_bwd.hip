@@ -368,11 +368,13 @@ __global__ __launch_bounds__(kScanThreads, SPL <= 8 ? 2 : 1) void scan_bwd_kerne
         pa[(int64_t)D * S + w.d] = gDsum;
         pa[(int64_t)D * (S + 1) + w.d] = gbsum;
     }
-    if (!run.used) return;
-    if (b.gstate && run.seg == 0) store_states<SPL>(b.gstate + w.n * (int64_t)D * S + states, S, w.q, gh);
-    int first, behind;   // rows behind the sequence's end
-    behind_share(p, run, first, behind);
-    ScanRows<T, OFF> qu(b.gu, b.gus, w, first), qd(b.gdelta, b.gds, w, first), qz(b.gz, b.gzs, w, first);
+    if (b.gstate && run.used && run.seg == 0) store_states<SPL>(b.gstate + w.n * (int64_t)D * S + states, S, w.q, gh);
+    if (!p.lengths) return;
+    int first, behind;   // rows behind a sequence's end
+    ScanLane at = w;
+    at.n = blockIdx.x % p.N;
+    behind_share(p, at.n, blockIdx.z, first, behind);
+    ScanRows<T, OFF> qu(b.gu, b.gus, at, first), qd(b.gdelta, b.gds, at, first), qz(b.gz, b.gzs, at, first);
     for (int t = first; t < behind; t += 4, qu.move(4), qd.move(4), qz.move(4))
         if (t + w.q < behind) {
             io_store(qu.at(0, w.q), 0.f);
