@@ -153,7 +153,7 @@ int scan_forward(const void *u, const int64_t *us, const void *delta, const int6
         !al16(state) || !al16(last) || !al16(saved) || !al16(workspace))
         return SRWM_ESTRIDE;
     ScanParams p{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, state, keep, lengths,
-                 out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS, 1, L, nullptr, nullptr};
+                 out, s3(os), last, saved, N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS, 1, L, kScanJoinFwd, nullptr, nullptr};
     if (!step) {
         p.segments = scan_segments(N, H, L, E, G, false, &p.seg_len);
         if (p.segments > 1 && lengths) ++p.segments;   // see scan_run
@@ -186,7 +186,7 @@ int scan_backward(const void *u, const int64_t *us, const void *delta, const int
     ScanBwdParams b{};
     b.f = ScanParams{u, delta, z, B, C, s3(us), s3(ds), s3(zs), s3(Bs), s3(Cs), A, D, bias, nullptr, keep, lengths,
                      nullptr, {}, nullptr, const_cast<float *>(saved), N, H, L, E, S, G, flags & SRWM_FLAG_SOFTPLUS,
-                     1, L, nullptr, nullptr};
+                     1, L, kScanJoinBwd, nullptr, nullptr};
     b.f.segments = scan_segments(N, H, L, E, G, true, &b.f.seg_len);
     if (b.f.segments > 1 && lengths) ++b.f.segments;   // see scan_run
     b.go = go, b.gos = s3(gos), b.glast = glast;

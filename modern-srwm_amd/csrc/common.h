@@ -167,6 +167,7 @@ struct ScanParams {
     int N, H, L, E, S, G;
     unsigned softplus;
     int segments, seg_len;               // steps are cut into `segments` runs of seg_len (a multiple of 16)
+    int seg_join;                        // a row of L steps has at most sqrt(seg_join * L) segments
     float *seg_decay, *seg_state;        // [N, segments, H*E, S]: a run's product of decays and its result from zero
 };
 
@@ -318,6 +319,8 @@ int launch_delta_bwd_generic(const DeltaBwdParams &p, hipStream_t s);
 
 // Selective scan, short convolution, norm.  bf16: the io tensors' type (else fp32).
 constexpr int kScanTile = 64;       // channels of a workgroup of the scan kernels
+constexpr int kScanMinSegment = 32; // steps of the shortest segment
+constexpr int kScanJoinFwd = 1, kScanJoinBwd = 4;   // ScanParams::seg_join
 // floats of a row of ScanBwdParams::part_a, a multiple of four so that every row can be written as float4
 inline __host__ __device__ int64_t scan_part_a_row(int64_t D, int S) { return (D * (S + 2) + 3) / 4 * 4; }
 // segments of the steps for a call (1: none) and their length, forward or backward

@@ -39,7 +39,9 @@ constexpr int kScanBwdWaves = 2048, kScanBwdShort = 96;
 // Shortest segment.  A segment also joins those in front of it one after the other, so their number n is bounded by their
 // length: n^2 <= steps forward, 4 steps backward (1 x 100000 steps of 64 channels, the two kernels of a pass, ms: n^2 <=
 // steps 0.130 + 0.236, 4 steps 0.139 + 0.224, 16 steps 0.189 + 0.254).
-constexpr int kScanMinSegment = 32;
+// Rows of different lengths keep both bounds, by the longest of them (64 channels, 12001 steps and 31 rows of 64, forward and
+// with the backward: up to 751 segments of the long row 141 and 344 us, within the bounds 54 and 190; 100000 steps and three
+// rows of one 198 and 517 against 131 and 412).
 
 // From four values per lane to one: lane j of each quad ends up with the quad's sum of v[j].
 __device__ __forceinline__ float quad_sum_scatter(float v0, float v1, float v2, float v3, int lane) {
@@ -94,7 +96,8 @@ struct ScanRun {
 };
 // Rows of one length: every row has p.segments segments.  Rows of different lengths: the segments are of one length over
 // all rows, so that no workgroup of a short row stands idle beside those of a long one; (slots - N) of them cover all steps,
-// and N more what is left over at the rows' ends.  Every wave works this out for itself (n, seg: the workgroup's place).
+// and N more what is left over at the rows' ends.  Longer segments, where the longest row would join too many, leave slots
+// empty.  Every wave works this out for itself (n, seg: the workgroup's place).
 __device__ __forceinline__ ScanRun scan_run(const ScanParams &p, int n, int seg) {
     ScanRun r;
     r.used = true;
@@ -106,17 +109,24 @@ __device__ __forceinline__ ScanRun scan_run(const ScanParams &p, int n, int seg)
     }
     const int lane = threadIdx.x & 63;
     int64_t total = 0;
+    int longest = 0;
     for (int b = 0; b < p.N; b += 64) {
-        int v = b + lane < p.N ? row_length(p, b + lane) : 0;
+        const int v = b + lane < p.N ? row_length(p, b + lane) : 0;
         int64_t s = v;
+        int most = v;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor((long long)s, off, kWave);
+        for (int off = 32; off > 0; off >>= 1) {
+            s += __shfl_xor((long long)s, off, kWave);
+            most = max(most, __shfl_xor(most, off, kWave));
+        }
         total += s;
+        longest = max(longest, most);
     }
     const int64_t slots = (int64_t)p.N * p.segments - p.N;
     int64_t sl = (total + slots - 1) / slots;
-    sl = (sl + kScanBlock - 1) / kScanBlock * kScanBlock;
-    const int seg_len = __builtin_amdgcn_readfirstlane(sl > 0 ? (int)sl : kScanBlock);   // the same in every lane: in a scalar register
+    sl = max((sl + kScanBlock - 1) / kScanBlock * kScanBlock, (int64_t)kScanMinSegment);
+    while (sl * sl * p.seg_join < longest) sl += kScanBlock;   // (longest / sl)^2 <= seg_join * longest
+    const int seg_len = __builtin_amdgcn_readfirstlane((int)sl);   // the same in every lane: in a scalar register
     int at = seg * p.N + n;
     r.used = false, r.n = 0, r.seg = 0, r.count = 1, r.len = 0, r.first = 0, r.tbeg = 0, r.tend = 0;
     int64_t before = 0;   // slots of the rows in front of this batch of 64

@@ -247,7 +247,7 @@ int scan_segments(int N, int H, int L, int E, int G, bool backward, int *len) {
     const int64_t waves = ((int64_t)(H / G) * E + kScanTile - 1) / kScanTile * N * G * (kScanThreads / 64);
     int64_t n = waves >= (backward ? kScanEnoughBwd : kScanEnoughFwd) ? 1 : (kScanWaves + waves - 1) / waves;
     int64_t most = (L + kScanMinSegment - 1) / kScanMinSegment;
-    while (most * most > (int64_t)L * (backward ? 4 : 1)) most = most * 7 / 8;
+    while (most * most > (int64_t)L * (backward ? kScanJoinBwd : kScanJoinFwd)) most = most * 7 / 8;
     if (most < 1) most = 1;
     n = n < most ? n : most;
     const int64_t fits = (kScanBwdWaves + waves - 1) / waves;

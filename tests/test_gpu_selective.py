@@ -202,6 +202,22 @@ def scan_time(N, L, lengths, backward):
 
 
 @pytest.mark.parametrize("backward", [False, True])
+def test_segments_of_a_long_row_are_bounded(backward):
+    """A segment joins those in front of it one after the other: a row of 12001 steps beside 31 of 64 is cut into about as many as
+    alone (measured: 141 and 344 us with up to 751 of them, 54 and 190 now, and 43 and 106 alone, where the padded rows' zeros
+    take 20 and 60 us)."""
+    alone = scan_time(1, 12001, None, backward)
+    pad = torch.empty(4 if backward else 1, 32, 12001, 64, device=DEV)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for _ in range(3):
+        start.record()
+        pad.zero_()
+        end.record()
+        torch.cuda.synchronize()
+    assert scan_time(32, 12001, [12001] + [64] * 31, backward) < 1.7 * (alone + start.elapsed_time(end) * 1e3)
+
+
+@pytest.mark.parametrize("backward", [False, True])
 def test_padding_behind_short_rows_costs_what_it_is(backward):
     """Zeros behind short rows are filled by all workgroups: a row of 100000 steps beside three of one step takes at most three
     times what it takes alone (measured: ten times where each row's own workgroups filled them, 1.7 times now)."""
