@@ -128,6 +128,10 @@ int scan_dims(int N, int H, int L, int E, int S, int G) {
     if (S > 64 || L > (1 << 30) || (int64_t)H * E > (1 << 30) || G > 65535 || scan_tiles(H, E, G) * N > kMaxGrid) return SRWM_ESIZE;
     return SRWM_OK;
 }
+// the workgroups of the backward's join of partial sums
+bool scan_join_fits(int N, int H, int L, int E, int S, int G) {
+    return (int64_t)N * G * L * 2 * S / 256 + (int64_t)H * E * (S + 2) / 32 + 2 <= kMaxGrid;
+}
 int conv_dims(int N, int H, int L, int E, int W) {
     if (!dims_ok(N, H, L, E) || W <= 0) return SRWM_EINVAL;
     if (W < 2 || W > 4 || L > (1 << 30) || (int64_t)H * E > (1 << 20) || conv_parts(N, H, L, E) > kMaxGrid ||
@@ -176,7 +180,7 @@ int scan_backward(const void *u, const int64_t *us, const void *delta, const int
         return SRWM_EINVAL;
     if (flags & ~SRWM_FLAG_SOFTPLUS) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
-    if ((int64_t)N * G * L * 2 * S / 256 + (int64_t)H * E * (S + 2) / 32 + 2 > kMaxGrid) return SRWM_ESIZE;   // the join's workgroups
+    if (!scan_join_fits(N, H, L, E, S, G)) return SRWM_ESIZE;
     if (!stride_ok(us, N, H, L, E) || !stride_ok(ds, N, H, L, E) || (z && !stride_ok(zs, N, H, L, E)) ||
         !stride_ok(Bs, N, G, L, S) || !stride_ok(Cs, N, G, L, S) || !stride_ok(gos, N, H, L, E) ||
         !out_stride_ok(gus, N, H, L, E) || !out_stride_ok(gds, N, H, L, E) || (z && !out_stride_ok(gzs, N, H, L, E)) ||
@@ -717,6 +721,7 @@ int residual_rms_norm_backward_bf16(const void *sum, const float *weight, const 
 int selective_scan_workspace(int64_t floats[1], int N, int H, int L, int E, int S, int G, int backward) {
     if (!floats) return SRWM_EINVAL;
     if (const int r = scan_dims(N, H, L, E, S, G)) return r;
+    if (backward && !scan_join_fits(N, H, L, E, S, G)) return SRWM_ESIZE;
     int len;
     int segments = scan_segments(N, H, L, E, G, backward != 0, &len);
     if (segments > 1) ++segments;   // one more where the rows' lengths differ

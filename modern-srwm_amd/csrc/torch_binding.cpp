@@ -257,6 +257,10 @@ void check_ints(std::initializer_list<int64_t> sizes) {
 std::tuple<Tensor, Tensor, Tensor> scan_forward(ScanIn &in, const Tensor &state_, bool softplus, bool save) {
     const ScanSizes &z = in.z;
     const Tensor &u = in.u.t;
+    if (save && !in.empty()) {   // what the backward could not take is refused in front of it
+        check_ints({z.N, z.H, z.L, z.E, z.S});
+        scan_workspace(z, 1);
+    }
     const Tensor state = dense_in(state_, "state", in.state_shape(), at::kFloat, u.device());
     Tensor out = rows_like(u), last = at::empty(in.state_shape(), f32_on(u));
     Tensor saved = save ? at::empty({z.N, (z.L + 15) / 16, z.H * z.E, z.S}, f32_on(u)) : Tensor();

@@ -583,6 +583,15 @@ def test_offsets_past_32_bits():
     assert torch.equal(causal_conv(**c)[0], causal_conv(**{**c, "x": u})[0])
 
 
+def test_scan_refuses_a_forward_that_no_backward_could_follow():
+    """N G L S beyond 2^30, with gradients recorded; the long axes are broadcast ones."""
+    wide = lambda *s: torch.ones(*s, device=DEV)
+    u, b = wide(32, 1, 1, 1).expand(32, 1, 1 << 20, 1), wide(32, 1, 1, 64).expand(32, 1, 1 << 20, 64)
+    A = -wide(1, 1, 64).requires_grad_()
+    with pytest.raises(RuntimeError, match="sizes beyond what the kernels take"):
+        selective_scan(u, u, A, b, b)
+
+
 def test_empty_calls():
     z = lambda *s: torch.zeros(*s, device=DEV)
     state = torch.randn(2, 1, 4, 16, device=DEV)

@@ -190,3 +190,11 @@ def test_binding_is_loaded_at_the_first_call():
             "else: raise AssertionError('no error')\n")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     subprocess.run([sys.executable, "-c", code], cwd=root, check=True, timeout=100)
+
+
+def test_scan_limit_of_the_backward_is_known_in_front():
+    """N G L S beyond 2^30: the forward runs, the backward's workspace cannot be asked for."""
+    import srwm_hip
+    n = (ctypes.c_int64 * 1)()
+    size = lambda backward: srwm_hip.lib().selective_scan_workspace(n, 32, 1, 1 << 20, 1, 64, 1, backward)
+    assert size(0) == 0 and size(1) == -2
