@@ -610,8 +610,8 @@ SRWM_API int selective_scan_step_bf16(const uint16_t *u, const int64_t u_strides
  *   last       the same behind the last step
  *   keep, lengths as above; inputs before a reset count as zero, in out and in last
  * Backward: grad_x strided [N,H,L,E], grad_last / grad_state like state (either may be NULL), grad_weight [H,E,W] and
- * grad_bias [H,E] (or NULL) fp32; workspace: causal_conv_workspace() floats.  H*E up to 2^20, N * ceil(L / 64) * ceil(H*E / 32)
- * below 2^24 (SRWM_ESIZE else; where vectors can be read, up to four times that); no output overlaps an input.  Step: state overwritten in place.
+ * grad_bias [H,E] (or NULL) fp32; workspace: causal_conv_workspace() floats.  H*E up to 2^20, N*H*E up to 2^31,
+ * N * ceil(L / 128) up to 2^23 (SRWM_ESIZE beyond), in both directions; no output overlaps an input.  Step: state overwritten in place.
  */
 SRWM_API int causal_conv_forward_f32(const float *x, const int64_t x_strides[3], const float *weight, const float *bias,
                              const float *state, const float *keep, const int *lengths, float *out,

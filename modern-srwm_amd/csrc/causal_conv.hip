@@ -34,15 +34,19 @@ struct ConvPlace {
     int64_t d, t0;
     int n, h, e, Ln;
 };
+// A workgroup's number among the N * runs * cols of a launch, which may take more than one row of the grid (the last one then
+// holds workgroups behind them: n >= N).
+constexpr int64_t kConvRow = 1 << 23;   // workgroups along x: 256 threads each must stay below 2^32
+__device__ __forceinline__ unsigned conv_group() { return blockIdx.y * (unsigned)kConvRow + blockIdx.x; }
 template <int V, int ST>
 __device__ __forceinline__ ConvPlace conv_place(const ConvParams &p, int runs, unsigned cols) {
     ConvPlace c;
-    c.d = ((int64_t)(blockIdx.x % cols) * kConvLanes + threadIdx.x) * V;
-    const unsigned part = blockIdx.x / cols;
+    c.d = ((int64_t)(conv_group() % cols) * kConvLanes + threadIdx.x) * V;
+    const unsigned part = conv_group() / cols;
     c.n = part / runs;
     c.t0 = ((int64_t)(part % runs) * kConvRuns + threadIdx.y) * ST;
     c.h = c.d / p.E, c.e = c.d % p.E;
-    c.Ln = p.lengths ? min(max(p.lengths[c.n], 0), p.L) : p.L;
+    c.Ln = p.lengths && c.n < p.N ? min(max(p.lengths[c.n], 0), p.L) : p.L;
     return c;
 }
 
@@ -82,7 +86,7 @@ template <typename T, int W, int V, int ST, bool KEEP>
 __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs, unsigned cols) {
     constexpr int R = ST + W - 1;
     const ConvPlace c = conv_place<V, ST>(p, runs, cols);
-    if (c.d >= (int64_t)p.H * p.E || (c.t0 >= p.L && c.t0 > 0)) return;
+    if (c.n >= p.N || c.d >= (int64_t)p.H * p.E || (c.t0 >= p.L && c.t0 > 0)) return;
     const T *x = (const T *)p.x + c.n * p.xs.n + c.h * p.xs.h + c.e;
     const int64_t srow = ((int64_t)c.n * p.H + c.h) * (W - 1) * p.E + c.e;
     T *out = (T *)p.out + c.n * p.os.n + c.h * p.os.h + c.e + c.t0 * p.os.l;
@@ -146,6 +150,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
     const int64_t D = (int64_t)p.H * p.E;
     __shared__ float red[kConvRuns][kConvLanes][V];
     const ConvPlace c = conv_place<V, ST>(p, runs, cols);
+    if (c.n >= p.N) return;   // the whole workgroup
     float gw[W + 1][V];
 #pragma unroll
     for (int j = 0; j <= W; ++j) zero<V>(gw[j]);
@@ -235,7 +240,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
             }
         }
     }
-    float *part = b.part + (int64_t)(blockIdx.x / cols) * (W + 1) * D;
+    float *part = b.part + (int64_t)(conv_group() / cols) * (W + 1) * D;
 #pragma unroll
     for (int j = 0; j <= W; ++j) {
         __syncthreads();
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwd
         for (int i = 0; i < V; ++i) red[threadIdx.y][threadIdx.x][i] = gw[j][i];
         __syncthreads();
         for (int i = threadIdx.y * kConvLanes + threadIdx.x; i < kConvLanes * V; i += kConvLanes * kConvRuns) {
-            const int64_t at = (int64_t)(blockIdx.x % cols) * kConvLanes * V + i;
+            const int64_t at = (int64_t)(conv_group() % cols) * kConvLanes * V + i;
             float v = 0.f;
 #pragma unroll
             for (int r = 0; r < kConvRuns; ++r) v += red[r][i / V][i % V];
@@ -329,7 +334,10 @@ struct ConvGrid {
     int64_t groups;
     ConvGrid(const ConvParams &p, int runs, int v)
         : cols((unsigned)(((int64_t)p.H * p.E / v + kConvLanes - 1) / kConvLanes)), groups((int64_t)p.N * runs * cols) {}
-    bool fits() const { return groups < ((int64_t)1 << 24); }   // of 256 threads each, below 2^32 of them
+    bool fits() const { return groups < ((int64_t)1 << 32) - kConvRow; }
+    dim3 grid() const {
+        return groups <= kConvRow ? dim3((unsigned)groups) : dim3((unsigned)kConvRow, (unsigned)((groups + kConvRow - 1) / kConvRow));
+    }
 };
 
 template <typename T, int W, int V>
@@ -339,8 +347,8 @@ int fwd_as(const ConvParams &p, hipStream_t s) {
     const ConvGrid g(p, runs, V);
     if (!g.fits()) return -1;
     const dim3 block(kConvLanes, kConvRuns);
-    if (p.keep) conv_fwd_kernel<T, W, V, ST, true><<<(unsigned)g.groups, block, 0, s>>>(p, runs, g.cols);
-    else conv_fwd_kernel<T, W, V, ST, false><<<(unsigned)g.groups, block, 0, s>>>(p, runs, g.cols);
+    if (p.keep) conv_fwd_kernel<T, W, V, ST, true><<<g.grid(), block, 0, s>>>(p, runs, g.cols);
+    else conv_fwd_kernel<T, W, V, ST, false><<<g.grid(), block, 0, s>>>(p, runs, g.cols);
     return (int)hipGetLastError();
 }
 template <typename T, int W>
@@ -355,8 +363,8 @@ int bwd_as(const ConvBwdParams &b, hipStream_t s) {
     const ConvGrid g(p, runs, V);
     if (!g.fits()) return -1;
     const dim3 block(kConvLanes, kConvRuns);
-    if (p.keep) conv_bwd_kernel<T, W, V, ST, true><<<(unsigned)g.groups, block, 0, s>>>(b, runs, g.cols);
-    else conv_bwd_kernel<T, W, V, ST, false><<<(unsigned)g.groups, block, 0, s>>>(b, runs, g.cols);
+    if (p.keep) conv_bwd_kernel<T, W, V, ST, true><<<g.grid(), block, 0, s>>>(b, runs, g.cols);
+    else conv_bwd_kernel<T, W, V, ST, false><<<g.grid(), block, 0, s>>>(b, runs, g.cols);
     const int r = (int)hipGetLastError();
     if (r) return r;
     const int64_t D = (int64_t)p.H * p.E;

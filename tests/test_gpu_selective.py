@@ -592,6 +592,24 @@ def test_scan_refuses_a_forward_that_no_backward_could_follow():
         selective_scan(u, u, A, b, b)
 
 
+def test_conv_of_more_workgroups_than_a_row_of_the_grid():
+    """2^23 rows of one step and 128 channels: what the forward takes, the backward takes.  All numbers are whole and below 2^24,
+    so that the sums are exact."""
+    N, E, W = 1 << 23, 128, 2
+    x = torch.arange(E, device=DEV).remainder(2).to(torch.bfloat16).view(1, 1, 1, E).expand(N, 1, 1, E).requires_grad_()
+    w = torch.tensor([3.0, 2.0], device=DEV).expand(1, E, W).contiguous().requires_grad_()
+    bias = torch.ones(1, E, device=DEV).requires_grad_()
+    out, last = causal_conv(x, w, bias, silu=False)
+    g = torch.ones(1, 1, 1, E, device=DEV, dtype=torch.bfloat16).expand(N, 1, 1, E)
+    with torch.no_grad():
+        first = x[0, 0, 0].float()
+        assert bool((out == (1 + 2 * first)).all()) and bool((last == first).all())
+        del last
+    gx, gw, gb = torch.autograd.grad(out, (x, w, bias), g)
+    assert bool((gx == 2).all())
+    assert torch.equal(gw[0, :, 1], N * first) and not gw[0, :, 0].any() and bool((gb == N).all())
+
+
 def test_empty_calls():
     z = lambda *s: torch.zeros(*s, device=DEV)
     state = torch.randn(2, 1, 4, 16, device=DEV)
