@@ -539,7 +539,8 @@ SRWM_API int delta_layer_prologue_grad_bf16(const uint16_t *gq, const int64_t gq
  *                      calls that may overlap need one each; a captured graph keeps its own
  * S up to 64, H*E up to 2^30, N * ceil(H*E / (64 G)) up to 2^23, in the backward N*G*L*S up to 2^30 (SRWM_ESIZE beyond);
  * no output overlaps an input or another output.  A, state, last, saved, workspace and their gradients start at multiples of 16 bytes.
- * Arithmetic, states and the sums are fp32.
+ * Arithmetic, states and the sums are fp32.  Long rows are cut into segments where waves are few; a state passes them by the
+ * product of their decays, which may lie between 2^-252 and 2^252 whatever the decays are (beyond it, zero or infinity).
  */
 SRWM_API int selective_scan_forward_f32(const float *u, const int64_t u_strides[3], const float *delta,
                              const int64_t delta_strides[3], const float *z, const int64_t z_strides[3],

@@ -168,7 +168,7 @@ struct ScanParams {
     unsigned softplus;
     int segments, seg_len;               // steps are cut into `segments` runs of seg_len (a multiple of 16)
     int seg_join;                        // a row of L steps has at most sqrt(seg_join * L) segments
-    float *seg_decay, *seg_state;        // [N, segments, H*E, S]: a run's product of decays and its result from zero
+    float *seg_decay, *seg_state;        // [N, segments, H*E, S]: the root of a run's product of decays, its result from zero
 };
 
 struct ScanBwdParams {

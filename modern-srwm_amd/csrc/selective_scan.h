@@ -220,12 +220,14 @@ struct ScanBc {
     }
 };
 
-// The product of decays of a segment with a reset in it: nothing of the state in front passes, not even NaN.  No power
-// of two has these bits.
+// A segment's product of decays 2^e is handed on as its root: the product itself may leave float32's range where the state that
+// it is applied to, in two steps, does not.  After a reset in the segment nothing of the state in front passes, not even NaN.
+// No power of two has these bits.
 constexpr float kDropped = -0.f;
-// A state of zero passes as zero through decays whose product overflows.
-__device__ __forceinline__ float carried(float decay, float x, float result) {
-    return __float_as_uint(decay) == 0x80000000u || x == 0.f ? result : fmaf(decay, x, result);
+__device__ __forceinline__ float decay_root(float e, bool alive) { return alive ? __builtin_amdgcn_exp2f(0.5f * e) : kDropped; }
+// A state of zero passes as zero through decays whose product overflows all the same.
+__device__ __forceinline__ float carried(float root, float x, float result) {
+    return __float_as_uint(root) == 0x80000000u || x == 0.f ? result : fmaf(root * x, root, result);
 }
 
 // Whether a workgroup's lanes lie 2 GiB or more apart in rows of these strides (64 channels, 16 steps).
@@ -284,7 +286,7 @@ __device__ __forceinline__ void store_states(float *row, int S, int q, const flo
 }
 
 // Carries a state (or its gradient) over `count` segments from the one at `at` on, `stride` floats from one to the next:
-// x = decay x + result.  Four segments are asked for at a time (two above 16 states; eight take the forward from five to
+// x = root^2 x + result.  Four segments are asked for at a time (two above 16 states; eight take the forward from five to
 // three waves a SIMD): one after the other would cost a trip to memory each, as they were written by other dies.
 template <int SPL>
 __device__ __forceinline__ void join_segments(const ScanParams &p, int64_t at, int64_t stride, int count, int S, int q, float (&x)[SPL]) {

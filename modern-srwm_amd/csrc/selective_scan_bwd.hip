@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_local_kernel(ScanBwdPar
     total = group_sum<4>(total);
     const int64_t at = (run.first + run.seg) * D * S + states;
 #pragma unroll
-    for (int s = 0; s < SPL; ++s) A2[s] = alive ? __builtin_amdgcn_exp2f(total * A2[s]) : kDropped;
+    for (int s = 0; s < SPL; ++s) A2[s] = decay_root(total * A2[s], alive);
     store_states<SPL>(p.seg_decay + at, S, w.q, A2);
     store_states<SPL>(p.seg_state + at, S, w.q, gh);
 }

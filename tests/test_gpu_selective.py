@@ -270,6 +270,27 @@ def test_infinite_decays_and_overflowing_products():
     assert not out.any() and not last.any()
 
 
+@pytest.mark.parametrize("sign", [1.0, -1.0], ids=["growing", "shrinking"])
+@pytest.mark.parametrize("L,at", [(2048, (3, 10, 17, 30)), (700, (5, 300, 301, 699))], ids=str)
+def test_states_whose_decays_multiply_beyond_float32(sign, L, at):
+    """A state of e^-69 that grows by e^92 (or of e^69 that shrinks by it), and the same for its gradient: the steps' product leaves
+    float32's range, the state does not, in rows that are cut into segments as in short ones.  Tolerance: the exponent of 92 is
+    rounded three times (the decay, its product with the step size or their sum, log2 e), by 2^-24 of itself each, 1.7e-5 in all;
+    the exponentials and products add a few roundings of 2^-24."""
+    a, m, go, gl = scan_case(1, 1, L, 4, 16, 1, gate=False, D=False, bias=False)
+    a["delta"] = torch.zeros(1, 1, L, 4)
+    a["delta"][:, :, list(at)] = 23.0
+    a["A"] = torch.full_like(a["A"], sign)
+    small = 1e-30 if sign > 0 else 1e30
+    a["u"], a["state"], gl = torch.zeros_like(a["u"]), a["state"] * small, gl * small
+    go = torch.zeros_like(go)
+    got, want = run_scan(a, m, go, gl, softplus=False)
+    for k in ("out", "last", "g_state", "g_A"):
+        top = float(want[k].detach().abs().max())
+        assert torch.isfinite(got[k]).all(), k
+        assert float((got[k].detach().cpu().double() - want[k].detach()).abs().max()) <= 2e-5 * top, k
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_packed_rows_equal_single_sequences(dtype):
     a, _, _, _ = scan_case(1, 2, 45, 24, 16, 1, dtype=dtype, state=False)
