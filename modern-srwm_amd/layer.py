@@ -517,7 +517,8 @@ class SelectiveLayer(nn.Module):
         return self.dt_linear(p[..., :r]).unflatten(-1, (self.num_head, self.dim_head)), bc.select(-3, 0), bc.select(-3, 1)
 
     def mix(self, h, residual=None, state=None, keep=None, lengths=None):
-        """(output without the residual, the residual stream with h added, new state).  h: (len, B, in_dim)."""
+        """(output without the residual, the residual stream with h added, new state).  h: (len, B, in_dim); keep: (B, len)
+        float32, 0 where a row's states restart before the step; lengths: (B,) int32."""
         slen, bsz, _ = h.shape
         inner = self.num_head * self.dim_head
         if h.is_cuda and torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
@@ -581,7 +582,8 @@ class SelectiveStack(nn.Module):
         return self
 
     def forward(self, h, states=None, keep=None, lengths=None):
-        """h: (len, B, in_dim) -> (normalised output, states)."""
+        """h: (len, B, in_dim) -> (normalised output, states).  keep: (B, len) float32, 0 where a row's states restart before the
+        step (the transpose of forward_steps' notdone); lengths: (B,) int32."""
         residual, new = torch.zeros(h.shape, device=h.device, dtype=torch.float32), []
         for layer, state in zip(self.layers, states or [None] * len(self.layers)):
             h, residual, state = layer.mix(h, residual, state, keep, lengths)
@@ -590,7 +592,7 @@ class SelectiveStack(nn.Module):
 
     @torch.no_grad()
     def step(self, h, states, keep=None):
-        """One token: h (B, in_dim); states are OVERWRITTEN."""
+        """One token: h (B, in_dim), keep (B,); states are OVERWRITTEN."""
         residual = torch.zeros(h.shape, device=h.device, dtype=torch.float32)
         for layer, state in zip(self.layers, states):
             h, residual = layer.mix_step(h, residual, state, keep)

@@ -132,6 +132,13 @@ def test_scan_long_rows(N, H, L, E, S, G, keep):
         check(got[k], want[k], k)
 
 
+@pytest.mark.parametrize("N,H,L,E,S,G", [(1, 1, 700, 96, 16, 1), (2, 2, 333, 40, 8, 1), (1, 2, 401, 9, 33, 2)])
+def test_scan_long_rows_in_16_bits(N, H, L, E, S, G):
+    got, want = run_scan(*scan_case(N, H, L, E, S, G, dtype=torch.bfloat16, keep=True, lengths=[L, L - 100][:N]))
+    for k in want:
+        check(got[k], want[k], k)
+
+
 # calls that fill a quarter of the device and more: few segments, tiles of channels that end inside a group
 WIDE = [(2, 1, 37, 2048, 16, 1), (4, 2, 50, 600, 20, 2), (3, 1, 33, 1500, 32, 1), (9, 8, 20, 40, 64, 4), (16, 1, 97, 203, 9, 1)]
 
@@ -602,6 +609,41 @@ def test_offsets_past_32_bits():
     c = {k: place(v) for k, v in ca.items()}
     u.copy_(c["x"])
     assert torch.equal(causal_conv(**c)[0], causal_conv(**{**c, "x": u})[0])
+
+
+@pytest.mark.parametrize("gate", [True, False])
+def test_gradients_of_rows_past_32_bits(gate):
+    """The backward on rows whose 16 steps span 2 GiB and more, of different lengths, with resets, cut into segments whose last
+    blocks are partial: the same bits as on compact rows."""
+    N, H, L, E, S, W = 2, 1, 70, 16, 16, 4
+    far = (1 << 26) + 64                                       # elements between two steps: 16 of them pass 2^31 bytes
+    store = torch.empty(far * (L - 1) + 8 * E * N, device=DEV, dtype=torch.bfloat16)
+    views = iter(store.as_strided((N, H, L, E), (E, E, far, 1), k * E * N) for k in range(8))
+
+    def spread(t):
+        v = next(views)
+        v.copy_(t)
+        return v
+    a, m, go, gl = scan_case(N, H, L, E, S, 1, dtype=torch.bfloat16, gate=gate, keep=True, lengths=[L, 45])
+    near = {k: place(v) for k, v in a.items() if v is not None}
+    wide = {k: spread(v) if k in ("u", "delta", "z") else v for k, v in near.items()}
+    mask = {k: v.to(DEV) for k, v in m.items()}
+    results = []
+    for d, g in ((near, place(go)), (wide, spread(go))):
+        leaves = {k: v.detach().requires_grad_() for k, v in d.items()}
+        out, last = selective_scan(**leaves, **mask)
+        results.append((out, last, *torch.autograd.grad((out, last), list(leaves.values()), (g, gl.to(DEV)))))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
+    a, m, go, gl = conv_case(N, H, L, E, W, dtype=torch.bfloat16, keep=True, lengths=[L, 45])
+    near = {k: place(v) for k, v in a.items()}
+    wide = {**near, "x": spread(near["x"])}
+    mask = {k: v.to(DEV) for k, v in m.items()}
+    results = []
+    for d, g in ((near, place(go)), (wide, spread(go))):
+        leaves = {k: v.detach().requires_grad_() for k, v in d.items()}
+        out, last = causal_conv(**leaves, **mask)
+        results.append((out, last, *torch.autograd.grad((out, last), list(leaves.values()), (g, gl.to(DEV)))))
+    assert all(torch.equal(x, y) for x, y in zip(*results))
 
 
 def test_scan_refuses_a_forward_that_no_backward_could_follow():

@@ -358,3 +358,30 @@ def test_capture_is_refused_for_leaves_behind_the_inputs():
     del eager
     with torch.cuda.graph(torch.cuda.CUDAGraph()):
         residual_rms_norm(-torch.exp(leaf.double().float()), None, w)
+
+
+def test_stack_with_resets_equals_its_parts():
+    """keep is (batch, steps): a row with a reset is the two sequences in front of it and behind it."""
+    torch.manual_seed(25)
+    stack = SelectiveStack(2, 2, 16, 32, 0.0).to(DEV)
+    h = torch.randn(9, 3, 32, generator=torch.Generator().manual_seed(26)).to(DEV)
+    keep = torch.ones(3, 9, device=DEV)
+    keep[1, 4] = 0
+    with torch.no_grad():
+        out, states = stack(h, keep=keep)
+        plain, plain_states = stack(h)
+        front, _ = stack(h[:4])
+        back, back_states = stack(h[4:])
+        step_states = [layer.start(3, DEV) for layer in stack.layers]
+        steps = torch.stack([stack.step(h[t], step_states, keep[:, t].contiguous()) for t in range(9)])
+    close(out[:, [0, 2]], plain[:, [0, 2]], "rows without a reset")
+    close(out[:4, 1], front[:, 1], "in front of the reset")
+    close(out[4:, 1], back[:, 1], "behind the reset")
+    close(steps, out, "single tokens")
+    for a, b, c, d in zip(states, back_states, plain_states, step_states):
+        for k in range(2):
+            close(a[k][1], b[k][1], "state behind the reset")
+            close(a[k][0], c[k][0], "state without a reset")
+            close(d[k], a[k], "state of the single tokens")
+    with pytest.raises(ValueError, match="keep"):
+        stack(h, keep=keep.t())
