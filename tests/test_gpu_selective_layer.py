@@ -385,3 +385,35 @@ def test_stack_with_resets_equals_its_parts():
             close(d[k], a[k], "state of the single tokens")
     with pytest.raises(ValueError, match="keep"):
         stack(h, keep=keep.t())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_training_step_replays_from_a_captured_graph(dtype):
+    layer = make(27).to(dtype)
+    g = torch.Generator().manual_seed(28)
+    h, go = (torch.randn(33, 2, 24, generator=g).to(DEV).to(dtype) for _ in range(2))
+    leaves = list(layer.parameters())
+
+    def step():
+        out = layer(h)
+        return [out.detach(), *torch.autograd.grad(out, leaves, go)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        with torch.no_grad():
+            h.copy_(torch.randn(33, 2, 24, generator=g))
+        for t in got:
+            t.zero_()
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for name, a, b in zip(["out", *(n for n, _ in layer.named_parameters())], got, want):
+            assert torch.equal(a, b), (k, name)
+        del want
