@@ -651,6 +651,7 @@ SRWM_API int causal_conv_workspace(int64_t floats[1], int N, int H, int L, int E
  * (1 for a row of zeros), rounded to nearest even.
  * Backward: `sum` is what was normalised, as stored (x without a residual); grad_x like x, grad_residual and grad_sum like
  * sum (either may be NULL) -- both gradients have the same values; grad_weight [D];  D up to 16384 (SRWM_ESIZE beyond).
+ * SRWM_FLAG_RESIDUAL_F32 tells the backward the type of sum; without a residual (sum is x) it is not given.
  * Up to 2^25 rows of 2048 elements, 2^23 longer ones; no output overlaps an input.
  * Workspace: residual_rms_norm_workspace() floats.
  */

@@ -80,8 +80,8 @@ __device__ __forceinline__ uint32_t load_resets(const float *keep, int64_t t, in
 }
 
 // Memory-bound: every input and output once, plus W - 1 rows of the run in front (from the caches).  All of a run's rows
-// are asked for before the first is used (4 x 2048 steps x 2048 channels, 4 taps, bf16: 67 MB in 16 us, 4.2 TB/s; 1 x 65536
-// steps 537 MB in 104 - 110 us, 5.0 TB/s).
+// are asked for before the first is used (4 x 2048 steps x 2048 channels, 4 taps, bf16: 67 MB in 15.3 us, 4.4 TB/s; 1 x 65536
+// steps 537 MB in 101 us, 5.3 TB/s).
 template <typename T, int W, int V, int ST, bool KEEP>
 __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvParams p, int runs, unsigned cols) {
     constexpr int R = ST + W - 1;
@@ -141,8 +141,8 @@ __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_fwd_kernel(ConvPar
 
 // gx_t = sum_j w[W-1-j] gp_{t+j} with gp = g f'(pre): a run walks its steps and the W - 1 behind them, carrying the
 // gradients of the last W inputs, each complete when the window leaves it.  Between memory and arithmetic (vector
-// instructions 80 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 29 us, 3.4 TB/s,
-// 1 x 65536 steps 805 MB in 206 us, 3.9 TB/s.
+// instructions 76 - 80 % of the time, the sigmoid's and 2 W products per step and channel): same sizes 101 MB in 28 us, 3.6 TB/s,
+// 1 x 65536 steps 805 MB in 192 us, 4.2 TB/s.
 template <typename T, int W, int V, int ST, bool KEEP>
 __global__ __launch_bounds__(kConvLanes *kConvRuns) void conv_bwd_kernel(ConvBwdParams b, int runs, unsigned cols) {
     constexpr int RX = ST + 2 * (W - 1), RG = ST + W - 1;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(256) void conv_join_kernel(const float *part, float
     }
 }
 
-// One token: V channels of one row per thread.  Latency: one row of 2048 channels 4.0 us, 256 rows (9 MB) 6.6 us.
+// One token: V channels of one row per thread.  Latency: one row of 2048 channels 3.9 us, 256 rows (9 MB) 6.9 us.
 template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void conv_step_kernel(ConvParams p) {
     const int64_t D = (int64_t)p.H * p.E;

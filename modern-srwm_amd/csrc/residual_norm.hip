@@ -3,7 +3,7 @@
 // elements, one workgroup of 4 waves per row beyond; a row stays in registers up to 32 elements per lane and is read a
 // second time beyond that.  Memory-bound, every element once: 8192 rows of 1024 (bf16, fp32 residual) forward 101 MB in
 // 21 us (4.8 TB/s), backward 134 MB in 27.5 us (4.9) and 7 us for the join of the weight's gradient; to e4m3, 12 001 rows,
-// 135 MB in 23.9 us (5.6); one row 3.5 us, which is a launch.
+// 135 MB in 23.7 us (5.7); one row 3.6 us, which is a launch.
 #include "common.h"
 #include "vec_io.h"
 #include "xlane.h"
@@ -131,8 +131,8 @@ __global__ __launch_bounds__(kNormThreads) void norm_fwd_kernel(NormParams p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 // y / scale: the product with the reciprocal may be a rounding beside a border of two e4m3 values, the remainder
-                // puts it right (equal to the division for every scale's mantissa and all floats around each border; a
-                // division takes 12 001 rows of 1024 from 23.9 to 26 us)
+                // puts it right (equal to the division for every scale's mantissa and all floats around each border; with a
+                // division a call of 12 001 rows of 1024 takes 29.2 us in place of 27.3)
                 const float a = y[i] * lift, q = a * inv;
                 y[i] = fmaf(fmaf(-q, by, a), inv, q);
             }

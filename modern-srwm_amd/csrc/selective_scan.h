@@ -26,10 +26,14 @@ namespace fw {
 
 constexpr int kScanBlock = 16;      // steps between two saved states, and per stage of B and C in LDS
 constexpr int kScanThreads = 256;   // 4 waves
+// Times in these files: single figures are of long runs (300 passes).  Figures that compare two forms are of runs of about ten
+// passes, at lower clocks, which makes those of the scan up to a fifth longer; where they are of long runs they say so.
+//
 // A call of few waves is cut into segments until it has kScanWaves (four on each SIMD), at the price of the pass that
-// forms the segments' own results, 0.6 of the forward and 0.2 of the backward.  2048 channels and 16 states, ms without /
-// with: forward 8 x 2048 steps (1 024 waves) 0.253 / 0.258, 4 x 2048 (512 waves) 0.55 / 0.147; backward 16 x 1024 (2 048
-// waves) 0.53 / 0.60, 8 x 2048 0.76 / 0.63.
+// forms the segments' own results, 0.6 of the forward and 0.2 of the backward.  2048 channels and 16 states, long runs, ms
+// without / with: forward 16 x 1024 steps (2 048 waves) 0.186 / 0.219, 8 x 2048 (1 024 waves) 0.245 / 0.232, 4 x 2048 (512
+// waves) 0.244 / 0.132; backward 16 x 1024 0.475 / 0.540, 8 x 2048 0.694 / 0.567.  At 1 024 waves the forward gains a
+// twentieth by segments, and the call would need their workspace: it is left whole.
 constexpr int kScanWaves = 4096, kScanEnoughFwd = 1024, kScanEnoughBwd = 2048;
 // The backward's main pass runs kScanBwdWaves at a time (two on each SIMD).  Segments shorter than kScanBwdShort are not
 // worth a second round of them, long ones are, as their rounds overlap (both kernels of the pass, us with segments for two

@@ -4,8 +4,8 @@
 //     gA += dt_t w_t;     gdt_t = w_t . A + x_t u_t;     gu_t = x_t dt_t + D gy_t
 //     gh_{t-1} = a_t gh_t   (0 where keep_t == 0)
 // The states h_t are formed again from the ones that the forward saved every 16 steps.
-// Bound by vector instructions like the forward (busy 82 - 85 %): 4 x 2048 steps x 2048 channels x 16 states, bf16: 67 us for
-// the segments' own results, 259 us for the main pass (24.6 instructions per state and step: 5 for the states again, 8 for
+// Bound by vector instructions like the forward (busy 82 - 85 %): 4 x 2048 steps x 2048 channels x 16 states, bf16: 61 us for
+// the segments' own results, 239 us for the main pass (24.9 instructions per state and step: 5 for the states again, 8 for
 // the formulas above, the rest sums over channels and what a channel has once per step), 9 us for the joins.
 #include "selective_scan.h"
 
