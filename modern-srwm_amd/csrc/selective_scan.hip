@@ -9,8 +9,8 @@ namespace {
 // comes from the call's state and the segments in front of this one, and the outputs are formed.
 // The inputs of a block are fetched while the block before is computed.
 // Bound by the number of vector instructions (busy 86 - 90 % of the time, LDS 4 %): per state and step a multiplication, an
-// exponential (twice the cycles of the others) and three more are needed, six of 4 cycles a wave; 8.4 are issued with
-// outputs (softplus, gate, conversions, hand-overs between lanes), 5.7 without.  4 x 2048 steps x 2048 channels x 16
+// exponential (twice the cycles of the others) and three more are needed, 5 instructions in 6 issue slots of 4 cycles a wave;
+// 8.4 in 9.4 are issued with outputs (softplus, gate, conversions, hand-overs between lanes), 5.7 in 6.7 without.  4 x 2048 steps x 2048 channels x 16
 // states, bf16: 56 us (LOCAL) + 83 us, 212 MB read and written by the second; two rows of 12 001 and 8 001 steps: 132 + 195.
 // 16 lanes to a channel, which needs no segments, took 667 us for the latter beside 148 + 217 (short runs).
 template <typename T, int SPL, bool KEEP, bool LOCAL, typename OFF>

@@ -451,9 +451,8 @@ class SelectiveLayer(nn.Module):
         e4m3 with a scale per row, its input comes as e4m3 from the norm.  Needs in_dim and 2 * H * d divisible by 16.  A
         weight that is changed in place, loaded, replaced or moved afterwards is converted anew (what is written past the
         version counter, through .data or into parameters made under torch.inference_mode(), which have none, is not seen: call
-        serve_e4m3 again).  The 8-bit weight is overwritten where it lies, so
-        that replays of a captured graph follow it from the next call of the layer or of serve_e4m3 on; a capture that would
-        have to convert it raises."""
+        serve_e4m3 again).  The 8-bit weight is overwritten where it lies, so that replays of a captured graph follow it from the
+        next call of the layer or of serve_e4m3 on; a capture that would have to convert it raises."""
         if self.in_dim % 16 or self.num_head * self.dim_head % 8:
             raise ValueError("the 8-bit projection needs in_dim and 2 * num_head * dim_head divisible by 16")
         weight, made_from = self.in_linear.weight, self._weight_made_from()
