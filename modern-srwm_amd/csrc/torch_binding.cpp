@@ -11,7 +11,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/python.h>
 
@@ -175,17 +174,26 @@ void not_held_outside(const char *what, c10::ArrayRef<Tensor> ts) {
 }
 
 // What a backward returns.  Where a graph of it is recorded (create_graph), a derivative of these gradients raises instead
-// of counting them as constants.
-variable_list once_differentiable(variable_list g, const char *what) {
+// of counting them as constants.  The node that raises leads on to the inputs of the forward and to the gradients that came in:
+// a derivative that is asked for some tensors only follows the paths to them and would pass a node without any by.
+struct NoDerivative : torch::autograd::Node {
+    std::string what;
+    NoDerivative(const char *what, torch::autograd::edge_list &&next) : Node(std::move(next)), what(what) {}
+    variable_list apply(variable_list &&) override { TORCH_CHECK(false, what, " has no second derivative"); }
+};
+variable_list once_differentiable(variable_list g, const char *what, const variable_list &incoming) {
     if (!at::GradMode::is_enabled()) return g;
-    variable_list in;
-    for (const Tensor &t : g)
-        if (t.defined()) in.push_back(t.detach().requires_grad_());
-    const auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has no second derivative", (int64_t)in.size());
-    const variable_list out = (*node)(std::move(in));
-    size_t k = 0;
-    for (Tensor &t : g)
-        if (t.defined()) t = out[k++];
+    torch::autograd::edge_list next;
+    if (const auto forward = torch::autograd::get_current_node()) next = forward->next_edges();
+    for (const Tensor &t : incoming)
+        if (t.defined() && t.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(t));
+    const std::shared_ptr<NoDerivative> node(new NoDerivative(what, std::move(next)), torch::autograd::deleteNode);
+    for (Tensor &t : g) {
+        if (!t.defined()) continue;
+        t = t.detach();
+        const uint32_t nr = node->add_input_metadata(t);
+        torch::autograd::impl::set_gradient_edge(t, {node, nr});
+    }
     return g;
 }
 
@@ -345,7 +353,7 @@ struct SelectiveScan : Function<SelectiveScan> {
         const Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(s[0]);
         variable_list g = scan_backward(in, s[10], go, grads[1], ctx->saved_data["softplus"].toBool(), ctx->saved_data["state"].toBool());
         g.resize(12);
-        return once_differentiable(std::move(g), "selective_scan");
+        return once_differentiable(std::move(g), "selective_scan", grads);
     }
 };
 
@@ -488,7 +496,7 @@ struct CausalConv : Function<CausalConv> {
             check_code(in.bf16 ? call(causal_conv_backward_bf16, (uint16_t *)nullptr) : call(causal_conv_backward_f32, (float *)nullptr),
                        "causal_conv_backward");
         }
-        return once_differentiable({gx.t, gw, gb, gs, Tensor(), Tensor(), Tensor()}, "causal_conv");
+        return once_differentiable({gx.t, gw, gb, gs, Tensor(), Tensor(), Tensor()}, "causal_conv", grads);
     }
 };
 
@@ -628,7 +636,7 @@ struct ResidualRMSNorm : Function<ResidualRMSNorm> {
         } else {
             gw.zero_();
         }
-        return once_differentiable({gx, gr, gw, Tensor()}, "residual_rms_norm");
+        return once_differentiable({gx, gr, gw, Tensor()}, "residual_rms_norm", {go_, gt_});
     }
 };
 

@@ -576,6 +576,28 @@ def test_second_derivatives_are_refused():
             (call(leaf).sum() + first.square().sum()).backward()       # a penalty on the gradient next to a loss
 
 
+def test_second_derivatives_of_chosen_tensors_are_refused():
+    """Asked for the derivative of a gradient by some tensors only, autograd follows the paths to them: there is one to every
+    tensor that the gradient was computed from."""
+    a, _, _, _ = scan_case(1, 2, 20, 8, 16, 1)
+    d = {k: place(v) for k, v in a.items()}
+    conv = dict(x=d["u"], weight=torch.randn(2, 8, 4, device=DEV), bias=torch.randn(2, 8, device=DEV))
+    norm = dict(x=torch.randn(5, 16, device=DEV), residual=torch.randn(5, 16, device=DEV), weight=torch.randn(16, device=DEV))
+    for op, args in ((selective_scan, d), (causal_conv, conv), (residual_rms_norm, norm),
+                     (residual_rms_norm, {**norm, "residual": None})):
+        leaves = {k: v.detach().requires_grad_() for k, v in args.items() if v is not None}
+        out = op(**{**args, **leaves})[0]
+        g = torch.randn_like(out).requires_grad_()
+        for k, by in leaves.items():
+            first, = torch.autograd.grad(out, by, g, create_graph=True)
+            for second in [*leaves.values(), g]:
+                with pytest.raises(RuntimeError, match=op.__name__ + " has no second derivative"):
+                    torch.autograd.grad(first.sum(), second, allow_unused=True, retain_graph=True)
+    w = norm["weight"]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.functional.hessian(lambda t: residual_rms_norm(t, None, w)[0].sum(), norm["x"])
+
+
 def test_gradients_with_tangents_are_refused():
     """Forward mode over the backward: a gradient that comes in with a tangent raises instead of losing it."""
     import torch.autograd.forward_ad as forward_ad
